@@ -126,8 +126,10 @@ def _power(e):
 def _quantise(x):
     """Rows [..., hd] -> (e4m3 values, exponent bytes [...])."""
     x = x.float()
-    e = torch.frexp(x.abs().amax(-1) / TOP)
+    a = x.abs().amax(-1)
+    e = torch.frexp(a / TOP)
     e = (e.exponent - (e.mantissa == 0.5).int()).clamp(E_MIN, E_MAX)            # smallest e with amax / 448 <= 2^e
+    e = e.masked_fill(a == 0, E_MIN)
     return (x * _power(-e)[..., None]).clamp(-TOP, TOP).to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
 
 
