@@ -596,6 +596,118 @@ def paged_prefill(qkv, kc, vc, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
                   max_ctx, C.addressof(rows), C.addressof(lens), len(runs), _stream())
 
 
+# ------------------------------------------------------------------------------ paged KV in 8 bits
+KV8_HEAD_DIMS = (16, 32, 64, 128)
+
+
+def kv8_record_bytes(bs, hd):
+    """Bytes of one (block, head) record of the 8-bit cache: ``bs * hd`` e4m3 codes of k, as many of v, ``bs`` pairs of exponent
+    bytes, padded to a multiple of 32.  A layer's cache is uint8 ``[n_blocks, H, kv8_record_bytes(bs, hd)]``, zeroed once.  A row of
+    ``hd`` numbers is kept as code * 2^(byte - 127) with the smallest exponent in [-63, 63] for which no magnitude exceeds 448;
+    what lies above 448 * 2^63 (infinities too) becomes the largest code, NaN stays NaN."""
+    return (2 * bs * hd + 2 * bs + 31) // 32 * 32
+
+
+def _kv8_check(name, x, kv, pos, slot, btab, bs, H, hd, ntok):
+    """Argument checks of the 8-bit cache's operators; positions, sequences and blocks are checked in the kernels (status code 8)."""
+    if hd not in KV8_HEAD_DIMS or bs < 1:
+        raise ValueError("%s: head width %d (of %s) or block size %d is not supported" % (name, hd, KV8_HEAD_DIMS, bs))
+    if kv.dtype != torch.uint8 or kv.dim() != 3 or kv.shape[1] != H or kv.shape[2] != kv8_record_bytes(bs, hd) or not kv.is_contiguous():
+        raise ValueError("%s: the cache must be contiguous uint8 [blocks, %d, %d]" % (name, H, kv8_record_bytes(bs, hd)))
+    if pos.dtype != torch.int32 or slot.dtype != torch.int32 or btab.dtype != torch.int32 or btab.dim() != 2 or not btab.is_contiguous():
+        raise ValueError("%s: positions, sequences and the block table must be int32, the table contiguous" % name)
+    if not 0 <= ntok <= x.shape[0] or pos.numel() < ntok or slot.numel() < ntok or not (pos.is_contiguous() and slot.is_contiguous()):
+        raise ValueError("%s: %d tokens of rows %s, positions %s, sequences %s" % (name, ntok, tuple(x.shape), tuple(pos.shape), tuple(slot.shape)))
+    dev = kv.device
+    if x.device != dev or pos.device != dev or slot.device != dev or btab.device != dev or (x.is_cuda and dev.index != torch.cuda.current_device()):
+        raise ValueError("%s: the tensors must be on one device, the current one" % name)
+
+
+def _kv8_rows(name, x, width, dtype):
+    if x.dim() != 2 or x.shape[1] < width or x.dtype != dtype or x.stride(1) != 1:
+        raise ValueError("%s: rows of %d contiguous %s are needed, not %s %s" % (name, width, dtype, tuple(x.shape), x.dtype))
+
+
+def append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok):
+    """``append_kv`` into the 8-bit cache: quantises k and v of each listed token (``qkv`` rows q | k | v) and stores them at their positions.
+    Two tokens of one call must not share a position of a block."""
+    _kv8_check("append_kv8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+    if _use_reference(qkv):
+        return ref.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+    _kv8_rows("append_kv8", qkv, 3 * H * hd, torch.bfloat16)
+    _call(_lib().kh_append_kv8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2], pos.data_ptr(),
+          slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, ntok, _stream())
+
+
+def read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok):
+    """The inverse of ``append_kv8``: rows ``k``, ``v`` [ntok, H * hd] (bf16, which holds the stored values exactly, or fp32) of the listed
+    positions, for handing a cached sequence on (another engine, another block size, a bf16 cache)."""
+    _kv8_check("read_kv8", k, kv, pos, slot, btab, bs, H, hd, ntok)
+    if k.dtype not in (torch.bfloat16, torch.float32) or v.device != k.device or v.shape[0] < ntok or v.stride(0) != k.stride(0):
+        raise ValueError("read_kv8: k and v must be bf16 or fp32 rows of one pitch, not %s %s and %s %s" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
+    _kv8_rows("read_kv8", k, H * hd, k.dtype)
+    _kv8_rows("read_kv8", v, H * hd, k.dtype)
+    if not kv.is_cuda:
+        return ref.read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok)
+    _call(_lib().kh_read_kv8, 1, kv.data_ptr(), kv.shape[0], kv.shape[2], k.data_ptr(), v.data_ptr(), k.stride(0), int(k.dtype == torch.float32),
+          pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, ntok, _stream())
+
+
+def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=False):
+    """``paged_attn`` over the 8-bit cache: causal attention of each listed token over positions 0..pos of its own sequence as the cache
+    holds them.  ``append``: the kernel first quantises and stores each token's own k, v (valid when no two listed tokens belong to
+    one sequence, i.e. decode steps); otherwise ``append_kv8`` must have run.  Few tokens over long contexts: the keys of a
+    token are shared out to the thread blocks of a cluster; no workspace."""
+    _kv8_check("paged_attn8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+    if _use_reference(qkv):
+        if append:
+            ref.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+        return ref.paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx)
+    _kv8_rows("paged_attn8", qkv, 3 * H * hd, torch.bfloat16)
+    _kv8_rows("paged_attn8", out, H * hd, torch.bfloat16)
+    if out.shape[0] < ntok or out.device != qkv.device:
+        raise ValueError("paged_attn8: %d rows of output for %d tokens" % (out.shape[0], ntok))
+    _call(_lib().kh_paged_attn8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2], out.data_ptr(), out.stride(0),
+          pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, 1.0 / math.sqrt(hd), ntok, max_ctx,
+          int(append), _stream())
+
+
+def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
+    """``paged_prefill`` over the 8-bit cache: ``paged_attn8`` for runs of consecutive positions of one sequence each,
+    ``runs = [(first row, length), ...]``, whose K/V are in the cache already (``append_kv8``).  Head widths 32, 64 and 128."""
+    _kv8_check("paged_prefill8", qkv, kv, pos, slot, btab, bs, H, hd, 0)
+    if hd == 16:
+        raise ValueError("paged_prefill8: head width 16 is not supported")
+    limit = min(qkv.shape[0], out.shape[0], pos.numel(), slot.numel())
+    if any(r < 0 or n < 1 or r + n > limit for r, n in runs):
+        raise ValueError("paged_prefill8: runs %s within %d rows" % (list(runs)[:8], limit))
+    if _use_reference(qkv):
+        for r, n in runs:
+            ref.paged_attn8(qkv[r:r + n], kv, out[r:r + n], pos[r:r + n], slot[r:r + n], btab, bs, H, hd, n, max_ctx)
+        return
+    _kv8_rows("paged_prefill8", qkv, 3 * H * hd, torch.bfloat16)
+    _kv8_rows("paged_prefill8", out, H * hd, torch.bfloat16)
+    if out.device != qkv.device:
+        raise ValueError("paged_prefill8: the tensors must be on one device, the current one")
+    rows, lens = _row_lists(runs, limit)
+    _call_keeping((rows, lens), _lib().kh_paged_prefill8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2],
+                  out.data_ptr(), out.stride(0), pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd,
+                  1.0 / math.sqrt(hd), max_ctx, C.addressof(rows), C.addressof(lens), len(runs), _stream())
+
+
+def copy_blocks8(kv, pairs, npairs):
+    """kv: [n_layer, n_blocks, H, record]; copies block pairs[2i] -> pairs[2i+1] in all layers."""
+    if kv.dtype != torch.uint8 or kv.dim() != 4 or not kv.is_contiguous() or pairs.dtype != torch.int32 or pairs.numel() < 2 * npairs or pairs.device != kv.device:
+        raise ValueError("copy_blocks8: contiguous uint8 [layers, blocks, H, record] and %d int32 pairs on its device are needed" % npairs)
+    if npairs == 0:
+        return
+    if not kv.is_cuda:
+        for i in range(npairs):
+            kv[:, int(pairs[2 * i + 1])].copy_(kv[:, int(pairs[2 * i])])
+        return
+    _call(_lib().kh_copy_blocks8, 1, kv.data_ptr(), pairs.data_ptr(), npairs, kv.shape[0], kv.shape[1], kv.stride(1), kv.stride(0), _stream())
+
+
 def gather_rows(x, rows, out, nseq):
     if _use_reference(x):
         out[:nseq].copy_(x[rows[:nseq].long()])

@@ -227,6 +227,75 @@ def paged_attn(qkv, kc, vc, out, pos, slot, btab, bs, H, hd, ntok):
     out[:ntok] = torch.einsum("thj,tjhe->the", torch.softmax(s, -1), Vv).reshape(ntok, d).to(out.dtype)
 
 
+def kv8_views(kv, bs, hd):
+    """(codes of k, codes of v [..., bs, hd], exponent bytes [..., bs, 2]) of records [..., record]."""
+    n = bs * hd
+    return kv[..., :n].unflatten(-1, (bs, hd)), kv[..., n:2 * n].unflatten(-1, (bs, hd)), kv[..., 2 * n:2 * n + 2 * bs].unflatten(-1, (bs, 2))
+
+
+def kv8_quantise(x):
+    """Rows [..., hd] -> (e4m3 codes, exponent bytes [...]): the smallest exponent in [-63, 63] for which no magnitude exceeds 448."""
+    x = x.float()
+    a = x.abs().nan_to_num(nan=0.0, posinf=math.inf).amax(-1)
+    m, e = torch.frexp(a.clamp(max=2.0 ** 100))                                  # a = m 2^e, m in [0.5, 1); 448 = 0.875 * 2^9
+    e = torch.where(a > 0, e - 9 + (m > 0.875).int(), torch.full_like(e, -63)).clamp(-63, 63)
+    y = x * ((127 - e) << 23).view(torch.float32)[..., None]
+    return y.clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8), (e + 127).to(torch.uint8)
+
+
+def _kv8_places(kv, pos, slot, btab, bs, ntok):
+    p, s = pos[:ntok].long(), slot[:ntok].long()
+    if ntok and (int(p.min()) < 0 or int(p.max()) >= btab.shape[1] * bs or int(s.min()) < 0 or int(s.max()) >= btab.shape[0]):
+        raise IndexError("a position or a sequence outside the block table")
+    blk = btab[s, p // bs].long()
+    if ntok and (int(blk.min()) < 0 or int(blk.max()) >= kv.shape[0]):
+        raise IndexError("a block outside the cache")
+    return blk, p % bs
+
+
+def append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok):
+    d = H * hd
+    blk, at = _kv8_places(kv, pos, slot, btab, bs, ntok)
+    ck, cv, ce = kv8_views(kv, bs, hd)
+    for codes, which in ((ck, 0), (cv, 1)):
+        q, e = kv8_quantise(qkv[:ntok, (which + 1) * d:(which + 2) * d].reshape(ntok, H, hd))
+        codes[blk, :, at] = q
+        ce[..., which][blk, :, at] = e
+
+
+def _kv8_load(kv, blk, at, bs, hd):
+    """k, v [*blk.shape, H, hd] in fp32."""
+    ck, cv, ce = kv8_views(kv, bs, hd)
+    s = (ce[blk, :, at].int() << 23).view(torch.float32)
+    f = lambda c, which: c[blk, :, at].view(torch.float8_e4m3fn).float() * s[..., which, None]
+    return f(ck, 0), f(cv, 1)
+
+
+def read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok):
+    blk, at = _kv8_places(kv, pos, slot, btab, bs, ntok)
+    x, y = _kv8_load(kv, blk, at, bs, hd)
+    k[:ntok, :H * hd] = x.reshape(ntok, H * hd).to(k.dtype)
+    v[:ntok, :H * hd] = y.reshape(ntok, H * hd).to(v.dtype)
+
+
+def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx):
+    if ntok == 0:
+        return
+    d = H * hd
+    _kv8_places(kv, pos, slot, btab, bs, ntok)
+    p = pos[:ntok].long()
+    if int(p.max()) >= max_ctx:
+        raise IndexError("a position beyond max_ctx")
+    for t in range(ntok):
+        j = torch.arange(int(p[t]) + 1, device=kv.device)
+        blk = btab[slot[t].long(), j // bs].long()
+        if int(blk.min()) < 0 or int(blk.max()) >= kv.shape[0]:
+            raise IndexError("a block outside the cache")
+        k, v = _kv8_load(kv, blk, j % bs, bs, hd)                                # [ctx, H, hd]
+        s = torch.einsum("he,jhe->hj", qkv[t, :d].float().reshape(H, hd), k) / math.sqrt(hd)
+        out[t, :d] = torch.einsum("hj,jhe->he", torch.softmax(s, -1), v).reshape(d).to(out.dtype)
+
+
 def sample(logits, V, temperature, seed, step, rep, out, nseq):
     lg = logits[:nseq, :V].float()
     if temperature <= 0:

@@ -1,0 +1,64 @@
+"""The 8-bit cache's operators from their definition, in 64 bits and without the package's code, and how far a kernel may be from them."""
+import math
+
+import torch
+
+E_LO, E_HI = -63, 63
+
+
+def grid():
+    """Value of each of the 256 e4m3 codes."""
+    v = [m * 2.0 ** -9 for m in range(8)] + [(8 + m) * 2.0 ** (e - 10) for e in range(1, 16) for m in range(8)]
+    v[127] = math.nan
+    return torch.tensor(v + [-x for x in v], dtype=torch.float64)
+
+
+def quantise(x):
+    """Rows [n, hd] -> (values on the grid times 2^e, e [n]); one number at a time."""
+    g = grid()[:127].tolist()
+    out, exps = [], []
+    for row in x.double().tolist():
+        a = max([abs(t) for t in row if t == t], default=0.0)
+        e = next((k for k in range(E_LO, E_HI) if a <= 448.0 * 2.0 ** k), E_HI)
+        vals = []
+        for t in row:
+            if t != t:
+                vals.append(math.nan)
+                continue
+            y = min(abs(t) / 2.0 ** e, 448.0)
+            i = min(range(127), key=lambda i: (abs(g[i] - y), i % 2))            # nearest, the even index of two
+            vals.append(math.copysign(g[i] * 2.0 ** e, t))
+        out.append(vals)
+        exps.append(e)
+    return torch.tensor(out, dtype=torch.float64), torch.tensor(exps)
+
+
+def rows_of(kv, table, bs, hd, n):
+    """Keys and values [n, H, hd] (float64) of a sequence's first n positions, from the bytes of a cache on the CPU."""
+    g, out = grid(), []
+    rec = kv.reshape(kv.shape[0], kv.shape[1], -1)
+    for which in range(2):
+        x = torch.empty(n, kv.shape[1], hd, dtype=torch.float64)
+        for j in range(n):
+            r, at = rec[int(table[j // bs])], j % bs
+            code = r[:, (which * bs + at) * hd:(which * bs + at + 1) * hd].long()
+            x[j] = g[code] * torch.pow(2.0, r[:, 2 * bs * hd + 2 * at + which].double() - 127)[:, None]
+        out.append(x)
+    return out
+
+
+def attend(q, k, v, p_half_step=0.0):
+    """One token: q [H, hd], k, v [ctx, H, hd], all float64.  Returns (o [H, hd], bound [H, hd] on a kernel's error).
+
+    A kernel sums hd products for a score in fp32, in any order: off by at most hd * 2^-24 * sum |q k| (one more rounding each for the two scales and
+    the reference, 2^-22 for the exponential), which moves p_j by that factor and o by twice it (numerator and normaliser).  The
+    sums over ctx positions add ctx * 2^-24, counted on sum p |v|; `p_half_step` is a rounding of the probabilities before P V.  The output is
+    rounded to bf16: half a step, 2^-8 of the value."""
+    hd, ctx = q.shape[-1], k.shape[0]
+    s = torch.einsum("he,jhe->hj", q, k) / math.sqrt(hd)
+    p = torch.softmax(s, -1)
+    o = torch.einsum("hj,jhe->he", p, v)
+    mag = torch.einsum("hj,jhe->he", p, v.abs())
+    top = torch.einsum("he,jhe->hj", q.abs(), k.abs()).amax(-1) / math.sqrt(hd)
+    c = 2 * ((hd + 4) * 2.0 ** -24 * top + 2.0 ** -21) + 2 * (ctx + 8) * 2.0 ** -24 + p_half_step
+    return o, 2.0 ** -8 * o.abs() + (1 + 2.0 ** -8) * c[:, None] * mag + 1e-30
