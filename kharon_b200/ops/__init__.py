@@ -31,7 +31,8 @@ def _lib():
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    """Handle of the current device's current stream (without the Stream object of torch.cuda.current_stream())."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 #: when a list, every native call is also appended as (function, args, launches) -- see ``LaunchPlan``
@@ -612,19 +613,20 @@ def _kv8_check(name, x, kv, pos, slot, btab, bs, H, hd, ntok):
     """Argument checks of the 8-bit cache's operators; positions, sequences and blocks are checked in the kernels (status code 8)."""
     if hd not in KV8_HEAD_DIMS or bs < 1:
         raise ValueError("%s: head width %d (of %s) or block size %d is not supported" % (name, hd, KV8_HEAD_DIMS, bs))
-    if kv.dtype != torch.uint8 or kv.dim() != 3 or kv.shape[1] != H or kv.shape[2] != kv8_record_bytes(bs, hd) or not kv.is_contiguous():
+    if kv.dtype != torch.uint8 or kv.dim() != 3 or kv.shape[1:] != (H, (2 * bs * hd + 2 * bs + 31) // 32 * 32) or not kv.is_contiguous():
         raise ValueError("%s: the cache must be contiguous uint8 [blocks, %d, %d]" % (name, H, kv8_record_bytes(bs, hd)))
-    if pos.dtype != torch.int32 or slot.dtype != torch.int32 or btab.dtype != torch.int32 or btab.dim() != 2 or not btab.is_contiguous():
+    i32 = torch.int32
+    if pos.dtype != i32 or slot.dtype != i32 or btab.dtype != i32 or btab.dim() != 2 or not btab.is_contiguous():
         raise ValueError("%s: positions, sequences and the block table must be int32, the table contiguous" % name)
-    if not 0 <= ntok <= x.shape[0] or pos.numel() < ntok or slot.numel() < ntok or not (pos.is_contiguous() and slot.is_contiguous()):
+    if not 0 <= ntok <= len(x) or pos.numel() < ntok or slot.numel() < ntok or not (pos.is_contiguous() and slot.is_contiguous()):
         raise ValueError("%s: %d tokens of rows %s, positions %s, sequences %s" % (name, ntok, tuple(x.shape), tuple(pos.shape), tuple(slot.shape)))
-    dev = kv.device
-    if x.device != dev or pos.device != dev or slot.device != dev or btab.device != dev or (x.is_cuda and dev.index != torch.cuda.current_device()):
+    dev = kv.get_device()                          # -1: the CPU
+    if x.get_device() != dev or pos.get_device() != dev or slot.get_device() != dev or btab.get_device() != dev or (dev >= 0 and dev != torch._C._cuda_getDevice()):
         raise ValueError("%s: the tensors must be on one device, the current one" % name)
 
 
 def _kv8_rows(name, x, width, dtype):
-    if x.dim() != 2 or x.shape[1] < width or x.dtype != dtype or x.stride(1) != 1:
+    if x.dtype != dtype or x.dim() != 2 or x.shape[1] < width or x.stride(1) != 1:
         raise ValueError("%s: rows of %d contiguous %s are needed, not %s %s" % (name, width, dtype, tuple(x.shape), x.dtype))
 
 
