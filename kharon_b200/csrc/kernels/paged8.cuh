@@ -240,7 +240,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
 
 // One token and head by one warp.
 template <int HD>
-__device__ __noinline__ void attend_row8(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, bf16* dst) {
+__device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, bf16* dst) {
   float m = -INFINITY, l = 0.f;
   f32x2 o[8];
   bool bad = false;

@@ -35,7 +35,7 @@ __device__ __forceinline__ void decode16(const uint4& u, float s, uint4& a, uint
 
 template <int HD>
 __global__ void __launch_bounds__(128)
-paged_prefill8_k(const __grid_constant__ Pieces tiles, const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float scale, int max_ctx) {
+paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float scale, int max_ctx) {
   constexpr int PITCH = HD * 2 + 16, TILE = P8_ROWS * PITCH, PC = HD / 16, NL = P8_ROWS * PC / 128;     // bytes per row, per tile; 16-code pieces per row, per thread
   extern __shared__ __align__(16) uint8_t smem[];                               // [K, V][64 rows]
   pdl_wait();
@@ -203,17 +203,26 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const Cache c, const bf16
   }
 }
 // ------------------------------------------------------------------------------- runs of new tokens on tcgen05
-// A work item is (up to 256 consecutive tokens of a run, head).  Warps 0-3 and 4-7 are two groups of one thread per query row, warps 8-11 fetch the
-// codes of 128 positions at a time through the block table and turn them into bf16 tiles (exact: four bits of mantissa, a power-of-two
-// scale) in the swizzled layout that the tensor core reads, one lane of warp 12 issues every tcgen05.mma:
-//   S_w = Q_w K_j^T -> TMEM;  group w: online softmax, P_w -> TMEM over S_w as bf16;  O_w += P_w V_j in TMEM.
-// Items of more than 128 tokens: group w has query rows 128 w .. and every key tile.  Items of up to 128: both groups have the same
-// rows and alternate key tiles.  While one group works on its scores, the tensor core does the other's products.  The key tiles of an item
-// are shared by the S CTAs of a cluster, in contiguous ranges, where the items alone would leave SMs idle.  Groups and CTAs that share
-// rows leave (maximum, normaliser, O) in shared memory and join them in a fixed order.
-// A row is rescaled only when its maximum grows by more than 2^8 (the older maximum stays the reference of its exponentials).
+// A work item is (up to 256 consecutive tokens of a run, head).  Warps 0-3 and 4-7 are two groups of one thread per query row; warps 8-11 fetch the
+// codes of K, 128 positions at a time, through the block table and turn them into f16 tiles in the swizzled layout that the tensor core reads,
+// warps 12-15 those of V.  One lane of each group issues the group's products:
+//   S_w = Q_w K_j^T -> TMEM;  group w: online softmax, P_w -> TMEM over S_w as f16;  O_w += P_w V_j in TMEM.
+// Items of more than 128 tokens: group w has query rows 128 w .. and every key tile.  Items of up to 128: both groups have the same rows and
+// alternate key tiles.  While one group works on its scores, the tensor core does the other's products.  The key tiles of an item are shared
+// by the S CTAs of a cluster, in contiguous ranges, where the items alone would leave SMs idle.  Groups and CTAs that share rows leave (reference,
+// normaliser, O) in shared memory and join them in a fixed order.
+//
+// Why f16: a code times a power of two is one conversion and one half2 product for two numbers, where bf16 with its own scale takes five instructions, and
+// P keeps 11 bits.  f16 has few exponents, so every power of two that is common to a row or a tile is taken out and put back in fp32:
+//   q = q' 2^eq (row; largest |q'| in [2^14, 2^15)),  k = k' 2^(EK - 7),  v = v' 2^(EV - 7)  with EK, EV the tile's largest exponents,
+//   P' = 2^(s + EV - R),  O = sum P' v' = 2^(7 - R) sum 2^s v,  l = sum over tiles of 2^(EB - EV) sum P' = 2^(EB - R) sum 2^s,
+// where R is the row's running maximum of (largest score + EV), in log2 units, and EB the first tile's EV.  What f16 rounds:
+//   q', k' below 2^-14: off by 2^-25, a score by less than fp32's own rounding of its largest terms;
+//   v' of positions whose exponent is more than 22 below the tile's largest: the item's rows are done anew, one by one, in fp32;
+//   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
+// A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
 namespace {
-constexpr int CH_ROWS = 256, CH_MAX = 1024, CH_THREADS = 416;
+constexpr int CH_ROWS = 256, CH_MAX = 1024, CH_THREADS = 512;
 struct Runs { int row0[CH_MAX]; uint16_t n[CH_MAX]; };
 
 template <int HD>
@@ -222,7 +231,14 @@ struct Chunk {
   static constexpr int TILE = 128 * HP * 2, NS = 2;
   static constexpr int DATA = 2 * TILE + NS * 2 * TILE;      // Q of both groups, NS stages of K and V
   static constexpr int PITCH = HD + 4;                       // floats per row of a group's O when it is shared
-  static constexpr int ML = DATA, BARS = ML + 2 * 128 * 8, SMEM = BARS + 256;
+  static constexpr int ML = DATA;                            // (R, normaliser) of 256 group rows
+  static constexpr int QE = ML + 256 * 8;                    // 2^eq of 256 rows
+  static constexpr int ADDR = QE + 256 * 4;                  // [K, V][2 tiles][128] addresses, then as many factors
+  static constexpr int FAC = ADDR + 2 * 2 * 128 * 8;
+  static constexpr int WMAX = FAC + 2 * 2 * 128 * 4;            // [K, V][2 tiles][4 warps] largest exponents, of K and of V
+  static constexpr int TMAX = WMAX + 2 * 2 * 4 * 4;          // [4 tiles] of the tile
+  static constexpr int AGAIN = TMAX + 4 * 4;                 // rows to be done anew, as bits
+  static constexpr int BARS = AGAIN + 8 * 4, SMEM = BARS + 8 * (4 * NS + 6) + 16;
   static_assert(2 * 128 * PITCH * 4 <= DATA, "the shared O takes the tiles' place");
 };
 __device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int row, int ch) {      // 16-byte chunk `ch` of a row of a [128 x HP] tile
@@ -231,53 +247,96 @@ __device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int row, int ch) {
 __device__ __forceinline__ void st_shared_16(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+template <int N>
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[N]) {
+  if constexpr (N == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
+  else if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+  else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
+template <int ID, int N>
+__device__ __forceinline__ void named_barrier() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ uint32_t pack_f16(f32x2 v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi2(v)), "f"(lo2(v)));
+  return r;
 }
-__device__ __forceinline__ float ld_cluster_1(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// loads whose value is used a turn later, and which the compiler would move down to that use
+__device__ __forceinline__ int ld_early_i32(const int* p) {
+  int r;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
 }
-__device__ __forceinline__ void rows_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the two groups
+__device__ __forceinline__ uint32_t ld_early_u16(const uint8_t* p) {
+  uint16_t r;
+  asm volatile("ld.global.b16 %0, [%1];" : "=h"(r) : "l"(p));
+  return r;
+}
+// four codes times f (twice in a word), as f16
+__device__ __forceinline__ void scale4(uint32_t codes, uint32_t f, uint32_t& a, uint32_t& b) {
+  asm("{\n\t.reg .b16 l, h;\n\t.reg .b32 x, y;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 x, l;\n\tcvt.rn.f16x2.e4m3x2 y, h;\n\t"
+      "mul.rn.f16x2 %0, x, %3;\n\tmul.rn.f16x2 %1, y, %3;\n\t}" : "=r"(a), "=r"(b) : "r"(codes), "r"(f));
+}
+// 2^x as f16, for x <= 7
+__device__ __forceinline__ uint32_t f16_pow2(int x) { return x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u; }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// A warp's rows of O times al.
+template <int HD>
+__device__ __forceinline__ void rescale(uint32_t tO, float al) {
+  uint32_t r[16];
+#pragma unroll 1
+  for (int i = 0; i < HD; i += 16) {
+    tmem_ld16(tO + i, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 16; k++) r[k] = __float_as_uint(__uint_as_float(r[k]) * al);
+    tmem_st16(tO + i, r);
+  }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^x for two numbers on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2, a polynomial of degree 4 for 2^f (its largest relative error,
+// 2^-18, is the least for the degree), n added to the exponent.  Below 2^-126: 2^-126.  NaN: no finite f16.
+__device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
+  constexpr float P0 = 0.9999992847f, P1 = 0.6931217909f, P2 = 0.2402474433f, P3 = 0.0559178591f, P4 = 0.0095701013f;
+  x = mk2(max_nan(lo2(x), -126.f), max_nan(hi2(x), -126.f));
+  const f32x2 t = add2(x, mk2(12582912.f, 12582912.f)), f = fma2(add2(t, mk2(-12582912.f, -12582912.f)), mk2(-1.f, -1.f), x);
+  f32x2 p = mk2(P4, P4);
+  p = fma2(p, f, mk2(P3, P3));
+  p = fma2(p, f, mk2(P2, P2));
+  p = fma2(p, f, mk2(P1, P1));
+  p = fma2(p, f, mk2(P0, P0));
+  return mk2(__int_as_float((int)((uint32_t)t << 23) + __float_as_int(lo2(p))), __int_as_float((int)((uint32_t)(t >> 32) << 23) + __float_as_int(hi2(p))));
+}
+// f16 x f16 -> fp32
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major) {
+  return umma_idesc_bf16(M, N, 0, b_mn_major) & ~((1u << 7) | (1u << 10));
+}
 }  // namespace
 
 template <int HD>
 __global__ void __launch_bounds__(CH_THREADS, 1)
-paged_chunk8_k(const __grid_constant__ Runs runs, const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float sl2, int max_ctx, int S) {
+paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float sl2, int max_ctx, int S) {
   using C = Chunk<HD>;
   constexpr int NS = C::NS;
   extern __shared__ __align__(1024) uint8_t chunk_smem[];
   uint8_t* const smem = chunk_smem;
   const uint32_t base = smem_u32(smem), sQ = base, sKV = base + 2 * C::TILE, b0 = base + C::BARS;
-  const uint32_t bar_q = b0, bar_kfull = b0 + 8, bar_kfree = bar_kfull + 8 * NS, bar_vfull = bar_kfree + 8 * NS, bar_vfree = bar_vfull + 8 * NS,
-                 bar_s = bar_vfree + 8 * NS, bar_p = bar_s + 16, bar_o = bar_p + 16;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::BARS + 8 * (1 + 4 * NS + 6));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (1 + 4 * NS + 6) + 4);
+  const uint32_t bar_kfull = b0, bar_kfree = bar_kfull + 8 * NS, bar_vfull = bar_kfree + 8 * NS, bar_vfree = bar_vfull + 8 * NS, bar_s = bar_vfree + 8 * NS, bar_pv = bar_s + 32;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::BARS + 8 * (4 * NS + 6));
+  volatile int* redo = abort_flag + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (4 * NS + 6) + 8);
+  uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + C::AGAIN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    mbar_init(bar_q, 8);
-    for (int s = 0; s < NS; s++) {
-      mbar_init(bar_kfull + 8 * s, 4); mbar_init(bar_kfree + 8 * s, 1);
-      mbar_init(bar_vfull + 8 * s, 4); mbar_init(bar_vfree + 8 * s, 1);
-    }
-    for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); mbar_init(bar_o + 8 * w, 1); }
-    *abort_flag = (base & 1023u) ? 6 : 0;         // swizzled tiles need the 1024-byte alignment
-    if (base & 1023u) atomicCAS(c.err, 0, 6);
-    mbar_fence_init();
-  }
-  if (warp == 12) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  if (tid < 8) s_again[tid] = 0;
+  if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
   pdl_wait();
   pdl_launch_dependents();
 
@@ -288,234 +347,296 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const Cache c, const bf16* __r
   if (ok < listed && tid == 0 && rank == 0) report(c.err);
   const int n = max(ok, 0), nq = n > 128 ? 2 : 1, ctx = p0 + n;
   const int tiles = n > 0 ? (ctx + 127) >> 7 : 0, kt0 = (int)((long)tiles * rank / S), kt1 = (int)((long)tiles * (rank + 1) / S);
-  const int lim0 = nq == 2 ? (p0 + 128 + 127) >> 7 : tiles;      // key tiles that group 0's rows see
+  const int lim0 = nq == 2 ? (p0 + 128 + 127) >> 7 : tiles;      // key tiles that group 0's rows see: all, or all but the last
   auto has = [&](int w, int j) { return nq == 2 ? w == 1 || j < lim0 : ((j - kt0) & 1) == w; };
+  if (tid == 0) {
+    // a stage is read by both groups, or by one of them: with NS = 2 and alternating tiles always by the same.  (The last tile may lack group 0:
+    // nothing is fetched over it.)
+    static_assert(NS == 2, "stages go with groups");
+    for (int s = 0; s < NS; s++) {
+      mbar_init(bar_kfull + 8 * s, 4); mbar_init(bar_kfree + 8 * s, nq);
+      mbar_init(bar_vfull + 8 * s, 4); mbar_init(bar_vfree + 8 * s, nq);
+    }
+    for (int w = 0; w < 2; w++) { mbar_init(bar_s + 16 * w, 1); mbar_init(bar_s + 16 * w + 8, 1); mbar_init(bar_pv + 8 * w, 1); }
+    *redo = 0;
+    *abort_flag = (base & 1023u) ? 6 : 0;         // swizzled tiles need the 1024-byte alignment
+    if (base & 1023u) atomicCAS(c.err, 0, 6);
+    mbar_fence_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   const bool live = *abort_flag == 0 && n > 0;
+  // After a wait that ran out the roles go through their loops without waiting, so that the named barriers match and the kernel ends.
+  bool dead = false;
+  auto wait = [&](uint32_t bar, uint32_t parity) { if (!dead && !mbar_wait(bar, parity, abort_flag, 6, c.err)) dead = true; };
 
-  if (warp >= 8 && warp < 12) {
-    // ------------------------------------------------------------------ codes -> bf16 tiles
-    constexpr int LPR = HD / 16, RPP = 128 / LPR;          // lanes per row, rows per pass; LPR passes per tile
-    const int t2 = tid - 256, l = t2 % LPR, r1 = t2 / LPR, bs = c.bs;
+  if (warp >= 8) {
+    // ------------------------------------------------------------------ codes -> f16 tiles: K by warps 8-11, V by warps 12-15
+    // A lane takes 16 codes (two 16-byte chunks of a tile) at a time; LPR lanes cover a row of a slab, so eight lanes of a store lie in rows whose
+    // numbers differ in the lowest bit, i.e. in eight bank groups.
+    constexpr int LPR = HD < 64 ? HD / 16 : 4, RPP = 128 / LPR, SLABS = HD / (16 * LPR), NP = 128 / RPP * SLABS;
+    const int vr = warp >= 12, t = tid & 127, l = t % LPR, r1 = t / LPR, bs = c.bs;
+    const uint32_t full = vr ? bar_vfull : bar_kfull, free = vr ? bar_vfree : bar_kfree;
     const int* bt = c.btab + (size_t)sl * c.max_lb;
+    uint64_t* s_addr = reinterpret_cast<uint64_t*>(smem + C::ADDR) + vr * 256;
+    uint32_t* s_fac = reinterpret_cast<uint32_t*>(smem + C::FAC) + vr * 256;
+    uint32_t* s_tmax = reinterpret_cast<uint32_t*>(smem + C::TMAX);
+    const uint32_t off0 = tile_chunk(0, r1, 2 * l);
+    uint32_t* s_wmax = reinterpret_cast<uint32_t*>(smem + C::WMAX) + vr * 8;
     bool bad = false;
-    uint4 kr[LPR], vr[LPR];
-    uint32_t er[LPR];
-    const uint8_t* ad[LPR];
-    auto rows = [&](int j) {
-#pragma unroll
-      for (int x = 0; x < LPR; x++) {
-        const int p = j * 128 + x * RPP + r1;
-        ad[x] = nullptr;
-        er[x] = 0;
-        if (p < ctx) {
-          const int lb = quot(c.div, p), at = p - lb * bs;
-          int b = __ldg(bt + lb);
-          if ((unsigned)b >= (unsigned)c.n_blocks) { bad = true; b = 0; }
-          const uint8_t* rc = record(c, b, h);
-          ad[x] = rc + at * HD + l * 16;
-          er[x] = *reinterpret_cast<const uint16_t*>(rc + 2 * bs * HD + 2 * at);
-        }
+    // A thread looks up one position of a tile (t of 128): block two tiles ahead, exponent one tile ahead, and passes address and exponent on.
+    // No loaded value is looked at before the next turn.
+    int blk = 0, blk_at = -1;
+    uint32_t e_next = 0;
+    uint64_t a_next = 0;
+    auto look = [&](int j) {                               // block of position 128 j + t
+      const int p = j * 128 + t;
+      blk_at = -1;
+      if (j < kt1 && p < ctx) {
+        const int lb = quot(c.div, p);
+        blk_at = p - lb * bs;
+        blk = ld_early_i32(bt + lb);
       }
     };
-    auto fetch = [&](uint4 (&r)[LPR], int off) {
-#pragma unroll
-      for (int x = 0; x < LPR; x++) r[x] = ad[x] ? *reinterpret_cast<const uint4*>(ad[x] + off) : make_uint4(0, 0, 0, 0);
-    };
-    auto store = [&](const uint4 (&r)[LPR], const uint32_t (&e)[LPR], int sh, uint32_t dst) {
-#pragma unroll
-      for (int x = 0; x < LPR; x++) {
-        uint4 a, b;
-        decode16(r[x], pow2_of(e[x] >> sh & 0xffu), a, b);
-        const int row = x * RPP + r1, odd = l >> 2 & 1;      // lanes 4-7 of a wide row store their halves the other way round: eight lanes, eight bank groups
-        st_shared_16(tile_chunk(dst, row, 2 * l + odd), odd ? b : a);
-        st_shared_16(tile_chunk(dst, row, 2 * l + 1 - odd), odd ? a : b);
+    auto exponent = [&]() {                                // ... its address and exponent
+      a_next = 0;
+      e_next = 0;
+      if (blk_at >= 0) {
+        if ((unsigned)blk >= (unsigned)c.n_blocks) { bad = true; blk = 0; }
+        const uint8_t* rc = record(c, blk, h);
+        e_next = ld_early_u16(rc + 2 * bs * HD + 2 * blk_at);
+        a_next = (uint64_t)(rc + (vr * bs + blk_at) * HD);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
+    };
+    uint4 x[NP];
+    auto publish = [&](int b, int it) {                    // tile -> buffer b; then its codes are on their way
+      s_addr[b * 128 + t] = a_next;
+      const uint32_t mk = __reduce_max_sync(0xffffffffu, e_next & 0xffu), mv = __reduce_max_sync(0xffffffffu, e_next >> 8);
+      if (lane == 0) s_wmax[b * 4 + (warp & 3)] = mk | mv << 16;
+      pair_barrier(4 + vr);
+#pragma unroll
+      for (int i = 0; i < NP / SLABS; i++) {
+        const uint64_t a = s_addr[b * 128 + i * RPP + r1];
+#pragma unroll
+        for (int q = 0; q < SLABS; q++) x[i * SLABS + q] = a ? *reinterpret_cast<const uint4*>(a + q * 64 + l * 16) : make_uint4(0, 0, 0, 0);
+      }
+      // the position's factor 2^(e - E + 7), E the tile's largest exponent
+      const uint32_t tops = __vmaxu2(__vmaxu2(s_wmax[b * 4], s_wmax[b * 4 + 1]), __vmaxu2(s_wmax[b * 4 + 2], s_wmax[b * 4 + 3]));
+      const int e = (int)(e_next >> 8 * vr & 0xffu), off = e - (int)(tops >> 16 * vr & 0xffffu);
+      if (vr && e > E_LO && off < -22) *redo = 1;
+      s_fac[b * 128 + t] = f16_pow2(off + 7) * 0x10001u;
+      // K's warps tell the groups both exponents: scores that are there have passed bar_kfull.  (Of four slots this one was last read for the tile
+      // four before, whose scores both groups have used: K's stage of the tile two before this one has been freed.)
+      if (t == 0 && !vr) s_tmax[it & 3] = tops;
     };
     if (live && kt0 < kt1) {
-      rows(kt0);
-      fetch(kr, 0);
-      fetch(vr, bs * HD);
+      look(kt0);
+      exponent();
+      look(kt0 + 1);
+      publish(0, 0);
+      exponent();
+      look(kt0 + 2);
       for (int j = kt0; j < kt1; j++) {
-        const int it = j - kt0, s = it % NS;
-        const uint32_t par = ((it / NS) & 1) ^ 1, sk = sKV + s * 2 * C::TILE;
-        uint32_t e[LPR];
+        const int it = j - kt0, s = it % NS, b = it & 1;
+        wait(free + 8 * s, ((it / NS) & 1) ^ 1);
+        pair_barrier(4 + vr);                              // the factors are there
+        // chunks 2 l and 2 l + 1 of rows r1, r1 + RPP ...: RPP is a multiple of 8, the swizzle is the same for all of them
+        const uint32_t dst0 = sKV + s * 2 * C::TILE + vr * C::TILE + off0, dst1 = dst0 ^ 16u;
 #pragma unroll
-        for (int x = 0; x < LPR; x++) e[x] = er[x];
-        if (!mbar_wait(bar_kfree + 8 * s, par, abort_flag, 6, c.err)) break;
-        store(kr, e, 0, sk);
-        if (lane == 0) mbar_arrive(bar_kfull + 8 * s);
-        if (j + 1 < kt1) { rows(j + 1); fetch(kr, 0); }
-        if (!mbar_wait(bar_vfree + 8 * s, par, abort_flag, 6, c.err)) break;
-        store(vr, e, 8, sk + C::TILE);
-        if (lane == 0) mbar_arrive(bar_vfull + 8 * s);
-        if (j + 1 < kt1) fetch(vr, bs * HD);
+        for (int i = 0; i < NP / SLABS; i++) {
+          const uint32_t f = s_fac[b * 128 + i * RPP + r1];
+#pragma unroll
+          for (int q = 0; q < SLABS; q++) {
+            const uint4 w = x[i * SLABS + q];
+            uint4 u, v;
+            scale4(w.x, f, u.x, u.y);
+            scale4(w.y, f, u.z, u.w);
+            scale4(w.z, f, v.x, v.y);
+            scale4(w.w, f, v.z, v.w);
+            st_shared_16(dst0 + i * RPP * 128 + q * 16384, u);
+            st_shared_16(dst1 + i * RPP * 128 + q * 16384, v);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + 8 * s);
+        if (j + 1 < kt1) {
+          publish(b ^ 1, it + 1);
+          exponent();
+          look(j + 3);
+        }
       }
     }
     if (bad) report(c.err);
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (live && elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0, 0), idesc_o = umma_idesc_bf16(128, HD, 0, 1);
-      int last[2] = {-1, -1}, np[2] = {0, 0};      // the tile whose P V is due, products P V so far
-      bool fine = mbar_wait(bar_q, 0, abort_flag, 6, c.err);
-      auto pv = [&](int w) {
-        const int it = last[w], s = it % NS, j = kt0 + it;
-        if (!mbar_wait(bar_vfull + 8 * s, (it / NS) & 1, abort_flag, 6, c.err) || !mbar_wait(bar_p + 8 * w, np[w] & 1, abort_flag, 6, c.err)) { fine = false; return; }
-        tc_fence_after();
-        const uint64_t dv = umma_desc_sw128(sKV + s * 2 * C::TILE + C::TILE, 16384, 1024);
-#pragma unroll
-        for (int kk = 0; kk < 8; kk++)
-          umma_f16_ts(tmem + 256 + w * HD, tmem + w * 128 + kk * 8, dv + (uint64_t)((kk * 2048) >> 4), idesc_o, np[w] > 0 || kk > 0);
-        np[w]++;
-        last[w] = -1;
-        if (w == 1 || !has(1, j)) umma_commit(bar_vfree + 8 * s);       // the tile's last reader
-      };
-      for (int j = kt0; fine && j < kt1; j++) {
-        const int it = j - kt0, s = it % NS;
-        for (int w = 0; fine && w < 2; w++) {
-          if (last[w] >= 0 && (nq == 2 || has(w, j))) pv(w);
-          if (!fine || !has(w, j)) continue;
-          if (!mbar_wait(bar_kfull + 8 * s, (it / NS) & 1, abort_flag, 6, c.err)) { fine = false; break; }
-          tc_fence_after();
-          const uint64_t dq = umma_desc_sw128(sQ + (nq == 2 ? w * C::TILE : 0), 16, 1024), dk = umma_desc_sw128(sKV + s * 2 * C::TILE, 16, 1024);
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; kk++) {
-            const uint64_t step = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
-            umma_f16_ss(tmem + w * 128, dq + step, dk + step, idesc_s, kk > 0);
-          }
-          umma_commit(bar_s + 8 * w);
-          if (w == 1 || !has(1, j)) umma_commit(bar_kfree + 8 * s);
-          last[w] = it;
-        }
-      }
-      for (int w = 0; fine && w < 2; w++) {
-        if (last[w] >= 0) pv(w);
-        if (fine && np[w] > 0) umma_commit(bar_o + 8 * w);
-      }
-    }
-    __syncwarp();
   } else if (live) {
     // ------------------------------------------------------------------ query rows
     const int w = warp >> 2, row = tid & 127, lrow = nq == 2 ? tid : row, qpos = p0 + lrow, wpos = qpos - lane;      // wpos: the warp's first row
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + w * 128 + lanes, tO = tmem + 256 + w * HD + lanes;
-    for (int i = tid; i < nq * 128 * (HD / 8); i += 256) {
-      const int r = i / (HD / 8), ch = i % (HD / 8);
-      const uint4 u = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + ch * 8) : make_uint4(0, 0, 0, 0);
-      st_shared_16(tile_chunk(sQ + (r >> 7) * C::TILE, r & 127, ch), u);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tO = tmem + 256 + w * HD + lanes;
+    const float* s_qe = reinterpret_cast<const float*>(smem + C::QE);
+    const uint32_t* s_tmax = reinterpret_cast<const uint32_t*>(smem + C::TMAX);
+    {
+      constexpr int LQ = HD / 8;                 // lanes per row of q
+#pragma unroll 1
+      for (int i = tid; i < nq * 128 * LQ; i += 256) {
+        const int r = i / LQ, ch = i % LQ;
+        const uint4 u = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + ch * 8) : make_uint4(0, 0, 0, 0);
+        uint32_t m = amax8(u);
+#pragma unroll
+        for (int x = LQ / 2; x > 0; x >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, x));
+        const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
+        const float f = pow2_of((uint32_t)(127 - eq));
+        const f32x2 f2 = mk2(f, f);
+        st_shared_16(tile_chunk(sQ + (r >> 7) * C::TILE, r & 127, ch),
+                     make_uint4(pack_f16(mul2(un2(u.x), f2)), pack_f16(mul2(un2(u.y), f2)), pack_f16(mul2(un2(u.z), f2)), pack_f16(mul2(un2(u.w), f2))));
+        if (ch == 0) reinterpret_cast<float*>(smem + C::QE)[r] = pow2_of((uint32_t)(127 + eq));
+      }
     }
     fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar_q);
-    float m = -INFINITY, l = 0.f;                // reference maximum (scaled, log2 units) and normaliser
-    int cnt = 0;
-    for (int j = kt0; j < kt1; j++) {
-      if (!has(w, j)) continue;
-      if (!mbar_wait(bar_s + 8 * w, cnt & 1, abort_flag, 6, c.err)) break;
+    named_barrier<1, 256>();
+    const float rq = sl2 * s_qe[lrow];
+    constexpr uint32_t idesc_s = idesc_f16(128, 64, 0), idesc_o = idesc_f16(128, HD, 1);
+    auto scores = [&](int j, int half) {         // one lane: scores of half a tile
+      const int it = j - kt0, s = it % NS;
+      if (half == 0) wait(bar_kfull + 8 * s, (it / NS) & 1);
+      if (dead) return;
       tc_fence_after();
-      const int k0 = j * 128;
-      uint32_t r[32], pk[16];
-      if (k0 > wpos + 31) {                      // every key comes after the warp's queries
+      const uint64_t dq = umma_desc_sw128(sQ + (nq == 2 ? w * C::TILE : 0), 16, 1024), dk = umma_desc_sw128(sKV + s * 2 * C::TILE + half * 8192, 16, 1024);
 #pragma unroll
-        for (int i = 0; i < 16; i++) pk[i] = 0u;
-#pragma unroll
-        for (int q = 0; q < 4; q++) tmem_st16(tS + q * 16, pk);
-      } else {
-        const bool edge = k0 + 127 > wpos;       // masks keys after the query
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          tmem_ld32(tS + q * 32, r);
-          tmem_ld_wait();
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 32; i++)
-              if (k0 + q * 32 + i > qpos) r[i] = 0xff800000u;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i++) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(r[i]));
-        }
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-        const bool grow = mt > m + 8.f;          // (from -inf too)
-        if (cnt > 0 && __any_sync(0xffffffffu, grow)) {       // S_j is there, so P V of the tile before is done: O can be rescaled in place
-          const float al = grow ? ex2(m - mt) : 1.f;
-#pragma unroll 1
-          for (int q = 0; q < HD; q += 32) {
-            tmem_ld32(tO + q, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) * al);
-            tmem_st32(tO + q, r);
-          }
-          l *= al;
-        }
-        if (grow) m = mt;
-        const float ref = m == -INFINITY ? 0.f : m;
-        const f32x2 sl = mk2(sl2, sl2), nm = mk2(-ref, -ref);
-        f32x2 rs0 = 0, rs1 = 0;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          tmem_ld32(tS + q * 32, r);
-          tmem_ld_wait();
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 32; i++)
-              if (k0 + q * 32 + i > qpos) r[i] = 0xff800000u;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const f32x2 e0 = fma2(mk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sl, nm);
-            const f32x2 e1 = fma2(mk2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), sl, nm);
-            const f32x2 x0 = mk2(ex2(lo2(e0)), ex2(hi2(e0))), x1 = mk2(ex2(lo2(e1)), ex2(hi2(e1)));
-            rs0 = add2(rs0, x0);
-            rs1 = add2(rs1, x1);
-            pk[i >> 1] = pack2(x0);
-            pk[(i >> 1) + 1] = pack2(x1);
-          }
-          tmem_st16(tS + q * 16, pk);            // over scores that have been read
-        }
-        l += (lo2(rs0) + hi2(rs0)) + (lo2(rs1) + hi2(rs1));
+      for (int kk = 0; kk < HD / 16; kk++) {
+        const uint64_t step = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+        umma_f16_ss(tmem + w * 128 + half * 64, dq + step, dk + step, idesc_s, kk > 0);
       }
-      tmem_st_wait();
-      tc_fence_before();
+      umma_commit(bar_s + 16 * w + 8 * half);
+      if (half) umma_commit(bar_kfree + 8 * s);
+    };
+    auto next = [&](int j) {                     // the group's tile after j, or kt1
+      for (j++; j < kt1 && !has(w, j);) j++;
+      return j;
+    };
+    const bool issues = (warp & 3) == 0;
+    int j = next(kt0 - 1);
+    if (issues) {
+      if (j < kt1 && elect_one()) { scores(j, 0); scores(j, 1); }
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p + 8 * w);
-      cnt++;
     }
-    if (cnt > 0) mbar_wait(bar_o + 8 * w, 0, abort_flag, 6, c.err);
+    float R = -INFINITY, l = 0.f;
+    uint32_t eb = 127;
+    int cnt = 0;                                 // tiles so far
+    while (j < kt1) {
+      const int it = j - kt0, s = it % NS, jn = next(j);
+#pragma unroll 1
+      for (int half = 0; half < 2; half++) {
+        const int k0 = j * 128 + half * 64;
+        const uint32_t tS = tmem + w * 128 + half * 64 + lanes;
+        // (never on bar_kfull here: its stage may hold the tile after next by now, and a parity that has come round again would not be seen)
+        wait(bar_s + 16 * w + 8 * half, cnt & 1);
+        tc_fence_after();
+        const uint32_t ek = s_tmax[it & 3] & 0xffffu, ev = s_tmax[it & 3] >> 16;
+        if (cnt == 0) eb = ev;
+        uint32_t pk[16];
+        if (k0 > wpos + 31) {                    // every key comes after the warp's queries
+#pragma unroll
+          for (int i = 0; i < 16; i++) pk[i] = 0u;
+          tmem_st16(tS, pk);
+          tmem_st16(tS + 16, pk);
+        } else {
+          uint32_t r[64];
+          tmem_ld32(tS, r);
+          tmem_ld32(tS + 32, r + 32);
+          tmem_ld_wait();
+          if (k0 + 63 > wpos) {                  // masks keys after the query
+#pragma unroll
+            for (int i = 0; i < 64; i++)
+              if (k0 + i > qpos) r[i] = 0xff800000u;
+          }
+          const float sl = rq * pow2_of(ek - 7), fev = (float)((int)ev - 127);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          const float mt = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl, fev);
+          const bool grow = mt > R + 8.f;        // (from -inf too)
+          if (__any_sync(0xffffffffu, grow)) {
+            const float al = grow ? ex2(R - mt) : 1.f;
+            if (cnt + half > 0) {                // O is there, once the last P V is done (the one before it is: these scores came after it)
+              wait(bar_pv + 8 * w, (half ^ 1) & 1);
+              tc_fence_after();
+              rescale<HD>(tO, al);
+            }
+            l *= al;
+            if (grow) R = mt;
+          }
+          const float c0 = fev - (R == -INFINITY ? 0.f : R);
+          const f32x2 c2 = mk2(c0, c0), slv = mk2(sl, sl);
+          f32x2 rs0 = 0, rs1 = 0;
+#pragma unroll
+          for (int q = 0; q < 2; q++) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const f32x2 e0 = fma2(mk2(__uint_as_float(r[q * 32 + i]), __uint_as_float(r[q * 32 + i + 1])), slv, c2);
+              const f32x2 e1 = fma2(mk2(__uint_as_float(r[q * 32 + i + 2]), __uint_as_float(r[q * 32 + i + 3])), slv, c2);
+              const f32x2 x0 = mk2(ex2(lo2(e0)), ex2(hi2(e0))), x1 = i % 16 == 12 ? exp2_poly(e1) : mk2(ex2(lo2(e1)), ex2(hi2(e1)));
+              rs0 = add2(rs0, x0);
+              rs1 = add2(rs1, x1);
+              pk[i >> 1] = pack_f16(x0);
+              pk[(i >> 1) + 1] = pack_f16(x1);
+            }
+            tmem_st16(tS + q * 16, pk);          // over the scores
+          }
+          l = fmaf((lo2(rs0) + hi2(rs0)) + (lo2(rs1) + hi2(rs1)), pow2_of(127 + eb - ev), l);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        pair_barrier(2 + w);
+        if (issues) {
+          const bool one = elect_one();
+          if (one && half == 0) wait(bar_vfull + 8 * s, (it / NS) & 1);
+          if (one && !dead) {
+            tc_fence_after();
+            const uint64_t dv = umma_desc_sw128(sKV + s * 2 * C::TILE + C::TILE + half * 8192, 16384, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              umma_f16_ts(tmem + 256 + w * HD, tmem + w * 128 + half * 64 + kk * 8, dv + (uint64_t)((kk * 2048) >> 4), idesc_o, cnt + half > 0 || kk > 0);
+            umma_commit(bar_pv + 8 * w);
+            if (half) umma_commit(bar_vfree + 8 * s);
+            if (jn < kt1) scores(jn, half);      // behind P V in the tensor core: these scores take P's place
+          }
+          __syncwarp();
+        }
+      }
+      cnt++;
+      j = jn;
+    }
+    if (cnt > 0) wait(bar_pv + 8 * w, 1);
     tc_fence_after();
-    const bool intact = *abort_flag == 0;
+    const float den = l * pow2_of(261u - eb);    // l 2^(7 - EB)
     // A NaN in V reaches the rows that see its position and no others.  P V multiplies it with the zeros of masked positions too, which leaves a
     // NaN in every row of the tile: such rows are done anew, one by one.
     if (S == 1 && nq == 2) {
-      const float inv = 1.f / l;
+      named_barrier<1, 256>();                   // (`redo` is written by then: all tiles have been used)
+      const bool intact = *abort_flag == 0 && lrow < n, all = *redo != 0;
+      const float inv = 1.f / den;
       bf16* dst = out + (size_t)(r0 + lrow) * ldo + h * HD;
-      uint32_t top = 0;
+      uint32_t top = __float_as_uint(inv) & 0x7fffffffu;
+      if (!(den > 0.f)) top = 0x7f800000u;
 #pragma unroll 1
       for (int q = 0; q < HD; q += 32) {
-        uint32_t r[32];
+        uint32_t r[32], o[16];
         tmem_ld32(tO + q, r);
         tmem_ld_wait();
-        uint32_t o[16];
 #pragma unroll
         for (int i = 0; i < 32; i++) top = max(top, r[i] & 0x7fffffffu);
 #pragma unroll
         for (int i = 0; i < 16; i++) o[i] = pack_bf16(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
-        if (lrow < n && intact)
+        if (intact)
 #pragma unroll
           for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(dst + q + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       }
-      uint32_t again = __ballot_sync(0xffffffffu, top >= 0x7f800000u && lrow < n && intact);
-      while (again) {
-        const int i = __ffs(again) - 1;
-        again &= again - 1;
-        const int t = r0 + lrow - lane + i;
-        __syncwarp();
-        attend_row8<HD>(c, qkv + (size_t)t * ld + h * HD, d, h, wpos + i, sl, sl2, out + (size_t)t * ldo + h * HD);
-      }
+      const uint32_t again = __ballot_sync(0xffffffffu, intact && (all || top >= 0x7f800000u));
+      if (lane == 0) s_again[warp] = again;
     } else {
-      rows_barrier();                            // no tile is read any more
+      named_barrier<1, 256>();                   // no tile is read any more
       float* part = reinterpret_cast<float*>(smem) + (w * 128 + row) * C::PITCH;
 #pragma unroll 1
       for (int q = 0; q < HD; q += 32) {
@@ -529,14 +650,20 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const Cache c, const bf16* __r
         for (int i = 0; i < 32; i += 4)
           *reinterpret_cast<uint4*>(part + q + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
-      *reinterpret_cast<float2*>(smem + C::ML + (w * 128 + row) * 8) = make_float2(m, l);
+      *reinterpret_cast<float2*>(smem + C::ML + (w * 128 + row) * 8) = make_float2(R, den);
     }
   }
   // ------------------------------------------------------------------ groups and CTAs that share rows join
   if (S > 1) { __syncwarp(); cluster_sync_all(); }
   if (live && warp < 8 && (S > 1 || nq == 1)) {
-    if (S == 1) rows_barrier();
+    if (S == 1) named_barrier<1, 256>();
     const int parts = nq == 2 ? S : 2 * S;       // of a row: part i is group i % 2 (or the row's own) of CTA i / 2 (or i)
+    bool all = false;
+    for (int i = 0; i < S; i++) {
+      float v[1];
+      ld_cluster(S > 1 ? mapa_shared(smem_u32((const void*)redo), i) : smem_u32((const void*)redo), v);
+      all |= __float_as_uint(v[0]) != 0;
+    }
 #pragma unroll 1
     for (int r = rank * 8 + warp; r < n; r += 8 * S) {
       const int row = r & 127;
@@ -547,9 +674,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const Cache c, const bf16* __r
       float pm = -INFINITY, pl = 0.f;
       if (lane < parts) {
         const uint2 at = where(lane);
-        const float2 v = ld_cluster_f32x2(at.x + C::ML + at.y * 8);
-        pm = v.x;
-        pl = v.y;
+        float v[2];
+        ld_cluster(at.x + C::ML + at.y * 8, v);
+        pm = v[0];
+        pl = v[1];
       }
       float mx = pm;
 #pragma unroll
@@ -566,28 +694,36 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const Cache c, const bf16* __r
 #pragma unroll 4
       for (int i = 0; i < parts; i++) {
         const uint2 at = where(i);
-        const uint32_t a = at.x + (at.y * C::PITCH + lane * E) * 4;
         const float fi = __shfl_sync(0xffffffffu, f, i);
-        if constexpr (E == 4) { const float4 v = ld_cluster_f32x4(a); o[0] += fi * v.x; o[1] += fi * v.y; o[2] += fi * v.z; o[3] += fi * v.w; }
-        else if constexpr (E == 2) { const float2 v = ld_cluster_f32x2(a); o[0] += fi * v.x; o[1] += fi * v.y; }
-        else o[0] += fi * ld_cluster_1(a);
-      }
-      const float inv = 1.f / __shfl_sync(0xffffffffu, den, 0);
-      bool nan = false;
+        float v[E];
+        ld_cluster(at.x + (at.y * C::PITCH + lane * E) * 4, v);
 #pragma unroll
-      for (int e = 0; e < E; e++) nan |= (__float_as_uint(o[e]) & 0x7fffffffu) >= 0x7f800000u;
+        for (int e = 0; e < E; e++) o[e] = fmaf(fi, v[e], o[e]);
+      }
+      den = __shfl_sync(0xffffffffu, den, 0);
+      const float inv = 1.f / den;
+      bool anew = all || !(den > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
+#pragma unroll
+      for (int e = 0; e < E; e++) anew |= (__float_as_uint(o[e]) & 0x7fffffffu) >= 0x7f800000u;
       if (*abort_flag) break;
       bf16* dst = out + (size_t)(r0 + r) * ldo + h * HD;
-      if (__any_sync(0xffffffffu, nan)) attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, d, h, p0 + r, sl, sl2, dst);
+      if (__any_sync(0xffffffffu, anew)) { if (lane == 0) atomicOr(s_again + (r >> 5), 1u << (r & 31)); }
       else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
       else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_bf16(o[0] * inv, o[1] * inv);
       else dst[lane] = __float2bfloat16(o[0] * inv);
     }
   }
   if (S > 1) { __syncwarp(); cluster_sync_all(); }          // the others' parts are read until here
+  if (live && warp < 8) {
+    named_barrier<1, 256>();
+#pragma unroll 1
+    for (int r = warp; r < n; r += 8)
+      if (s_again[r >> 5] >> (r & 31) & 1)
+        attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, d, h, p0 + r, sl, sl2, out + (size_t)(r0 + r) * ldo + h * HD);
+  }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+  if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 template <int HD>
