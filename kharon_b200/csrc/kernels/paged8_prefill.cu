@@ -222,7 +222,7 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ C
 //   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
 // A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
 namespace {
-constexpr int CH_ROWS = 256, CH_MAX = 1024, CH_THREADS = 512;
+constexpr int CH_ROWS = 256, CH_MAX = 1024, CH_THREADS = 640;
 struct Runs { int row0[CH_MAX]; uint16_t n[CH_MAX]; };
 
 template <int HD>
@@ -238,7 +238,7 @@ struct Chunk {
   static constexpr int WMAX = FAC + 2 * 2 * 128 * 4;            // [K, V][2 tiles][4 warps] largest exponents, of K and of V
   static constexpr int TMAX = WMAX + 2 * 2 * 4 * 4;          // [4 tiles] of the tile
   static constexpr int AGAIN = TMAX + 4 * 4;                 // rows to be done anew, as bits
-  static constexpr int BARS = AGAIN + 8 * 4, SMEM = BARS + 8 * (4 * NS + 6) + 16;
+  static constexpr int BARS = AGAIN + 8 * 4, SMEM = BARS + 8 * (4 * NS + 13) + 16;
   static_assert(2 * 128 * PITCH * 4 <= DATA, "the shared O takes the tiles' place");
 };
 __device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int row, int ch) {      // 16-byte chunk `ch` of a row of a [128 x HP] tile
@@ -315,6 +315,18 @@ __device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
   p = fma2(p, f, mk2(P0, P0));
   return mk2(__int_as_float((int)((uint32_t)t << 23) + __float_as_int(lo2(p))), __int_as_float((int)((uint32_t)(t >> 32) << 23) + __float_as_int(hi2(p))));
 }
+// The MMAs with descriptors given by their low words (the high word is the same for all tiles: groups of 8 rows 1024 bytes apart, 128-byte swizzle).
+constexpr uint32_t DESC_HI = 64u | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(DESC_HI) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(DESC_HI) : "memory");
+}
 // f16 x f16 -> fp32
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major) {
   return umma_idesc_bf16(M, N, 0, b_mn_major) & ~((1u << 7) | (1u << 10));
@@ -329,10 +341,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   extern __shared__ __align__(1024) uint8_t chunk_smem[];
   uint8_t* const smem = chunk_smem;
   const uint32_t base = smem_u32(smem), sQ = base, sKV = base + 2 * C::TILE, b0 = base + C::BARS;
-  const uint32_t bar_kfull = b0, bar_kfree = bar_kfull + 8 * NS, bar_vfull = bar_kfree + 8 * NS, bar_vfree = bar_vfull + 8 * NS, bar_s = bar_vfree + 8 * NS, bar_pv = bar_s + 32;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::BARS + 8 * (4 * NS + 6));
+  const uint32_t bar_kfull = b0, bar_kfree = bar_kfull + 8 * NS, bar_vfull = bar_kfree + 8 * NS, bar_vfree = bar_vfull + 8 * NS, bar_s = bar_vfree + 8 * NS, bar_p = bar_s + 32, bar_pv = bar_p + 32, bar_o = bar_pv + 16, bar_q = bar_o + 16;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::BARS + 8 * (4 * NS + 13));
   volatile int* redo = abort_flag + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (4 * NS + 6) + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (4 * NS + 13) + 8);
   uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + C::AGAIN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < 8) s_again[tid] = 0;
@@ -341,14 +353,18 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   pdl_launch_dependents();
 
   const int rank = (int)(blockIdx.x % S), item = (int)(blockIdx.x / S), h = item % c.H, piece = item / c.H, d = c.H * HD;
-  const int r0 = runs.row0[piece], p0 = c.pos[r0], sl = c.slot[r0], listed = runs.n[piece];
+  // (What every thread knows alike goes through a shuffle, or *tmem_slot below: the compiler keeps it in uniform registers then, which is what
+  // tcgen05 instructions take.)
+  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+  const int r0 = runs.row0[piece], p0 = uniform(c.pos[r0]), sl = uniform(c.slot[r0]), listed = runs.n[piece];
   // index guard: tokens beyond the limits are recorded (status code 8) and skipped; they are the last of the run
   const int ok = sl < 0 || sl >= c.n_slots || p0 < 0 ? 0 : (int)min((long)listed, min((long)max_ctx, (long)c.max_lb * c.bs) - p0);
   if (ok < listed && tid == 0 && rank == 0) report(c.err);
   const int n = max(ok, 0), nq = n > 128 ? 2 : 1, ctx = p0 + n;
   const int tiles = n > 0 ? (ctx + 127) >> 7 : 0, kt0 = (int)((long)tiles * rank / S), kt1 = (int)((long)tiles * (rank + 1) / S);
-  const int lim0 = nq == 2 ? (p0 + 128 + 127) >> 7 : tiles;      // key tiles that group 0's rows see: all, or all but the last
-  auto has = [&](int w, int j) { return nq == 2 ? w == 1 || j < lim0 : ((j - kt0) & 1) == w; };
+  // tiles of group w: nq = 2: all, for the first rows maybe without the last one; nq = 1: every second
+  const int lim0 = min(kt1, (p0 + 128 + 127) >> 7);
+  auto tiles_of = [&](int w) { return nq == 2 ? max(0, (w ? kt1 : lim0) - kt0) : (kt1 - kt0 + 1 - w) >> 1; };
   if (tid == 0) {
     // a stage is read by both groups, or by one of them: with NS = 2 and alternating tiles always by the same.  (The last tile may lack group 0:
     // nothing is fetched over it.)
@@ -357,7 +373,8 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       mbar_init(bar_kfull + 8 * s, 4); mbar_init(bar_kfree + 8 * s, nq);
       mbar_init(bar_vfull + 8 * s, 4); mbar_init(bar_vfree + 8 * s, nq);
     }
-    for (int w = 0; w < 2; w++) { mbar_init(bar_s + 16 * w, 1); mbar_init(bar_s + 16 * w + 8, 1); mbar_init(bar_pv + 8 * w, 1); }
+    for (int i = 0; i < 4; i++) { mbar_init(bar_s + 8 * i, 1); mbar_init(bar_p + 8 * i, 4); }      // [group][half]
+    mbar_init(bar_pv, 1); mbar_init(bar_pv + 8, 1); mbar_init(bar_o, 1); mbar_init(bar_o + 8, 1); mbar_init(bar_q, 8);
     *redo = 0;
     *abort_flag = (base & 1023u) ? 6 : 0;         // swizzled tiles need the 1024-byte alignment
     if (base & 1023u) atomicCAS(c.err, 0, 6);
@@ -366,13 +383,65 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
   const bool live = *abort_flag == 0 && n > 0;
   // After a wait that ran out the roles go through their loops without waiting, so that the named barriers match and the kernel ends.
   bool dead = false;
   auto wait = [&](uint32_t bar, uint32_t parity) { if (!dead && !mbar_wait(bar, parity, abort_flag, 6, c.err)) dead = true; };
 
-  if (warp >= 8) {
+  // 640 threads of 96 registers: 128 to the groups, 80 to the fetching warps, 64 to the rest.  What follows a role's loop stays in its branch.
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+  else if (warp < 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+
+  if (warp >= 16) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (warp == 16 && live && elect_one()) {
+      constexpr uint32_t idesc_s = idesc_f16(128, 64, 0), idesc_o = idesc_f16(128, HD, 1);
+      const int tiles_w[2] = {tiles_of(0), tiles_of(1)};
+      const uint32_t dq0 = (uint32_t)umma_desc_sw128(sQ, 16, 1024), dk0 = (uint32_t)umma_desc_sw128(sKV, 16, 1024), dv0 = (uint32_t)umma_desc_sw128(sKV + C::TILE, 16384, 1024);
+      auto scores = [&](int w, int half, int t) {          // S of half a tile, the group's t-th
+        const int it = nq == 2 ? t : 2 * t + w, s = it & 1;
+        if (half == 0) wait(bar_kfull + 8 * s, (it / NS) & 1);
+        if (dead) return;
+        tc_fence_after();
+        const uint32_t dq = dq0 + (nq == 2 && w ? C::TILE >> 4 : 0), dk = dk0 + s * (2 * C::TILE >> 4) + half * 512;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
+          const uint32_t step = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+          mma_f16_ss(tmem + w * 128 + half * 64, dq + step, dk + step, idesc_s, kk > 0);
+        }
+        umma_commit(bar_s + 16 * w + 8 * half);
+        if (half) umma_commit(bar_kfree + 8 * s);
+      };
+      wait(bar_q, 0);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (tiles_w[i & 1] > 0) scores(i & 1, i >> 1, 0);
+      const int most = max(tiles_w[0], tiles_w[1]);
+#pragma unroll 1
+      for (int t = 0; t < most; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int w = i & 1, half = i >> 1;
+          if (t >= tiles_w[w]) continue;
+          const int it = nq == 2 ? t : 2 * t + w, s = it & 1;
+          if (half == 0) wait(bar_vfull + 8 * s, (it / NS) & 1);
+          wait(bar_p + 16 * w + 8 * half, t & 1);
+          if (dead) continue;
+          tc_fence_after();
+          const uint32_t dv = dv0 + s * (2 * C::TILE >> 4) + half * 512;
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)
+            mma_f16_ts(tmem + 256 + w * HD, tmem + w * 128 + half * 64 + kk * 8, dv + (kk * 2048 >> 4), idesc_o, half > 0 || kk > 0 ? 1 : t > 0);
+          umma_commit(half && t + 1 == tiles_w[w] ? bar_o + 8 * w : bar_pv + 8 * w);
+          if (half) umma_commit(bar_vfree + 8 * s);
+          if (t + 1 < tiles_w[w]) scores(w, half, t + 1);      // behind P V in the tensor core: these scores take P's place
+        }
+    }
+    __syncwarp();
+    if (S > 1) { cluster_sync_all(); cluster_sync_all(); }
+  } else if (warp >= 8) {
     // ------------------------------------------------------------------ codes -> f16 tiles: K by warps 8-11, V by warps 12-15
     // A lane takes 16 codes (two 16-byte chunks of a tile) at a time; LPR lanes cover a row of a slab, so eight lanes of a store lie in rows whose
     // numbers differ in the lowest bit, i.e. in eight bank groups.
@@ -470,8 +539,11 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       }
     }
     if (bad) report(c.err);
-  } else if (live) {
+    __syncwarp();
+    if (S > 1) { cluster_sync_all(); cluster_sync_all(); }
+  } else {
     // ------------------------------------------------------------------ query rows
+    if (live) {
     const int w = warp >> 2, row = tid & 127, lrow = nq == 2 ? tid : row, qpos = p0 + lrow, wpos = qpos - lane;      // wpos: the warp's first row
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tO = tmem + 256 + w * HD + lanes;
     const float* s_qe = reinterpret_cast<const float*>(smem + C::QE);
@@ -495,37 +567,14 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     }
     fence_proxy_async_smem();
     named_barrier<1, 256>();
+    if (lane == 0) mbar_arrive(bar_q);
     const float rq = sl2 * s_qe[lrow];
-    constexpr uint32_t idesc_s = idesc_f16(128, 64, 0), idesc_o = idesc_f16(128, HD, 1);
-    auto scores = [&](int j, int half) {         // one lane: scores of half a tile
-      const int it = j - kt0, s = it % NS;
-      if (half == 0) wait(bar_kfull + 8 * s, (it / NS) & 1);
-      if (dead) return;
-      tc_fence_after();
-      const uint64_t dq = umma_desc_sw128(sQ + (nq == 2 ? w * C::TILE : 0), 16, 1024), dk = umma_desc_sw128(sKV + s * 2 * C::TILE + half * 8192, 16, 1024);
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; kk++) {
-        const uint64_t step = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
-        umma_f16_ss(tmem + w * 128 + half * 64, dq + step, dk + step, idesc_s, kk > 0);
-      }
-      umma_commit(bar_s + 16 * w + 8 * half);
-      if (half) umma_commit(bar_kfree + 8 * s);
-    };
-    auto next = [&](int j) {                     // the group's tile after j, or kt1
-      for (j++; j < kt1 && !has(w, j);) j++;
-      return j;
-    };
-    const bool issues = (warp & 3) == 0;
-    int j = next(kt0 - 1);
-    if (issues) {
-      if (j < kt1 && elect_one()) { scores(j, 0); scores(j, 1); }
-      __syncwarp();
-    }
     float R = -INFINITY, l = 0.f;
     uint32_t eb = 127;
-    int cnt = 0;                                 // tiles so far
-    while (j < kt1) {
-      const int it = j - kt0, s = it % NS, jn = next(j);
+    const int mine = tiles_of(w);
+#pragma unroll 1
+    for (int cnt = 0; cnt < mine; cnt++) {
+      const int it = nq == 2 ? cnt : 2 * cnt + w, j = kt0 + it;
 #pragma unroll 1
       for (int half = 0; half < 2; half++) {
         const int k0 = j * 128 + half * 64;
@@ -588,27 +637,11 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         }
         tmem_st_wait();
         tc_fence_before();
-        pair_barrier(2 + w);
-        if (issues) {
-          const bool one = elect_one();
-          if (one && half == 0) wait(bar_vfull + 8 * s, (it / NS) & 1);
-          if (one && !dead) {
-            tc_fence_after();
-            const uint64_t dv = umma_desc_sw128(sKV + s * 2 * C::TILE + C::TILE + half * 8192, 16384, 1024);
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-              umma_f16_ts(tmem + 256 + w * HD, tmem + w * 128 + half * 64 + kk * 8, dv + (uint64_t)((kk * 2048) >> 4), idesc_o, cnt + half > 0 || kk > 0);
-            umma_commit(bar_pv + 8 * w);
-            if (half) umma_commit(bar_vfree + 8 * s);
-            if (jn < kt1) scores(jn, half);      // behind P V in the tensor core: these scores take P's place
-          }
-          __syncwarp();
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p + 16 * w + 8 * half);
       }
-      cnt++;
-      j = jn;
     }
-    if (cnt > 0) wait(bar_pv + 8 * w, 1);
+    if (mine > 0) wait(bar_o + 8 * w, 0);      // (on a barrier of its own: the P V before the last may not be done, and its parity would be taken for the last one's)
     tc_fence_after();
     const float den = l * pow2_of(261u - eb);    // l 2^(7 - EB)
     // A NaN in V reaches the rows that see its position and no others.  P V multiplies it with the zeros of masked positions too, which leaves a
@@ -641,7 +674,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
 #pragma unroll 1
       for (int q = 0; q < HD; q += 32) {
         uint32_t r[32];
-        if (cnt > 0) { tmem_ld32(tO + q, r); tmem_ld_wait(); }
+        if (mine > 0) { tmem_ld32(tO + q, r); tmem_ld_wait(); }
         else {
 #pragma unroll
           for (int i = 0; i < 32; i++) r[i] = 0u;
@@ -652,10 +685,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       }
       *reinterpret_cast<float2*>(smem + C::ML + (w * 128 + row) * 8) = make_float2(R, den);
     }
-  }
+    }
   // ------------------------------------------------------------------ groups and CTAs that share rows join
   if (S > 1) { __syncwarp(); cluster_sync_all(); }
-  if (live && warp < 8 && (S > 1 || nq == 1)) {
+  if (live && (S > 1 || nq == 1)) {
     if (S == 1) named_barrier<1, 256>();
     const int parts = nq == 2 ? S : 2 * S;       // of a row: part i is group i % 2 (or the row's own) of CTA i / 2 (or i)
     bool all = false;
@@ -714,12 +747,13 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     }
   }
   if (S > 1) { __syncwarp(); cluster_sync_all(); }          // the others' parts are read until here
-  if (live && warp < 8) {
+  if (live) {
     named_barrier<1, 256>();
 #pragma unroll 1
     for (int r = warp; r < n; r += 8)
       if (s_again[r >> 5] >> (r & 31) & 1)
         attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, d, h, p0 + r, sl, sl2, out + (size_t)(r0 + r) * ldo + h * HD);
+  }
   }
   tc_fence_before();
   __syncthreads();
