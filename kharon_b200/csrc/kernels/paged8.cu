@@ -10,6 +10,7 @@
 // rounding is the one to e4m3 (half a step, 2^-4 of the value at most, or 2^-10 2^e for values below 2^-6 2^e), and the stored value is exact in bf16.  Magnitudes above 448 2^63
 // and infinities become the largest code, NaN stays NaN and does not count for the maximum.
 #include "paged8.cuh"
+#include <stdlib.h>
 
 extern "C" int kh_kv8_record_bytes(int bs, int hd) { return (2 * bs * hd + 2 * bs + 31) / 32 * 32; }
 
@@ -100,19 +101,287 @@ extern "C" int kh_read_kv8(const void* kv, int n_blocks, int rec, void* k, void*
 }
 
 // ------------------------------------------------------------------------------- single-token attention
-// o = sum_j p_j v_j / sum_j p_j, p_j = exp(q k_j / sqrt(hd) - max), over positions j = 0 .. pos of the token's sequence.
-// W warps of a CTA and the S CTAs of a cluster share a (token, head).  A position is read by HD / 16 lanes in 16-byte pieces, so a warp holds
-// KPW = 512 / HD groups of lanes; it takes chunks of U * KPW consecutive positions, chunk i goes to warp i mod (S W).  Each group keeps a running
-// fp32 softmax of its own; the groups are merged once at the end: shuffles in the warp, shared memory in warp order across warps,
-// the cluster's shared memory in rank order across CTAs (no scratch in global memory, one launch).  The next chunk's K and V replace the current
-// ones in their registers as soon as those are used.
-// With `append` != 0 the warp that owns position pos quantises the token's k and v, writes them into the cache and uses what it wrote.
+// o = sum_j 2^(s_j) v_j / sum_j 2^(s_j), s_j = q k_j log2(e) / sqrt(hd), over positions j = 0 .. pos of the token's sequence.
+//
+// A warp takes chunks of 32 consecutive positions; W warps of a CTA and the S CTAs of a cluster share a (token, head), chunk i goes to warp
+// i mod (S W).  The products run on mma.sync (f16, fp32 sums), because what bounds a plain loop is not memory but its 4.8 instructions per code (conversion to fp32,
+// multiply, reduction): 313 us for 128 sequences of 1000 to 4096 positions, 16 heads of 128.  Codes become f16 with one instruction for two:
+//   S:  A = q in every row (so each lane has the scores it needs without a shuffle), B = K: lanes 4 g + i hold 1/4 of the codes of position g of eight;
+//   O:  A = V^T, B = P: lanes 4 g + i hold 1/8 of the dims, of positions 2 i, 2 i + 1 of each eight; two positions' codes are interleaved by byte permutation.
+// What f16 cannot hold is taken out as powers of two and put back in fp32: q = q' 2^eq (largest |q'| in [2^14, 2^15)), scores times 2^ek, and
+// P' = 2^(s + ev - R + 14) with R the running maximum of s + ev, so that V's codes enter as they are.  P' goes in as two f16 terms, in the even and
+// the odd columns of B (22 bits; 2^-39 of the largest term): nothing is rounded to fewer bits than a sum of the same length in fp32.
+// The block table and the exponents of a chunk are read by one lane per position and passed on by shuffles; the next chunk's K and V replace the
+// current ones in their registers as soon as those are used.
+// With `append` != 0 the item's first warp quantises the token's k and v, writes them into the cache and starts its sums with them.
+// The warps are merged once at the end: shared memory in warp order, then the cluster's shared memory in rank order (no scratch in global
+// memory, one launch).
 namespace {
 
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// the codes of a word's lower / upper half as two f16
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& a, uint32_t& b) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
+}
+template <int WORDS>
+__device__ __forceinline__ void ld_codes(uint32_t (&r)[WORDS], const uint8_t* p) {
+  if constexpr (WORDS == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
+  else if constexpr (WORDS == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); r[0] = v.x; r[1] = v.y; }
+  else r[0] = *reinterpret_cast<const uint32_t*>(p);
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+
+// A warp's share of one token and head: R, l (the whole warp's) and o[t] = sums of dims g HD / 8 + t (in every lane of a group of four).
+template <int HD>
+__device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, int wi, int nw, int append,
+                                               float& R, float& l, float (&out)[HD / 8], bool& bad) {
+  constexpr int KS = HD == 128 ? 2 : 1, KW = HD / 16 / KS, VW = HD >= 32 ? HD / 32 : 1, NM = HD / 16;       // K: slabs of 64 codes, words per lane; V: words per lane; MMAs across hd
+  constexpr uint32_t NONE = 0xffffffffu;
+  const int lane = threadIdx.x & 31, g = lane >> 2, i4 = lane & 3, bs = c.bs;
+  const int* bt = c.btab + (size_t)sl * c.max_lb;
+  const int n = append ? p : p + 1;                // positions read from the cache
+  // lane's position of a chunk: its K row in units of 16 bytes from the cache's start (NONE: past the end), and its exponents
+  uint32_t off_n = NONE, e_n = 0;                  // of the next chunk to be fetched
+  int blk = 0, at = -1;                            // of the one after
+  auto look = [&](int j0) {
+    const int j = j0 + lane;
+    at = -1;
+    if (j < n) {
+      const int lb = quot(c.div, j);
+      at = j - lb * bs;
+      asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(blk) : "l"(bt + lb));
+    }
+  };
+  auto place = [&]() {
+    off_n = NONE;
+    e_n = 0;
+    if (at >= 0) {
+      if ((unsigned)blk >= (unsigned)c.n_blocks) { bad = true; blk = 0; }
+      const uint32_t rc = ((uint32_t)blk * c.H + h) * (uint32_t)(c.rec >> 4);
+      off_n = rc + at * (HD / 16);
+      uint16_t e;
+      asm volatile("ld.global.b16 %0, [%1];" : "=h"(e) : "l"(c.kv + (size_t)rc * 16 + 2 * bs * HD + 2 * at));
+      e_n = e;
+    }
+  };
+  uint32_t k[4][KS][KW], v[2][4][VW];              // [eight positions][slab][word]; [sixteen positions][one of a lane's four][word]
+  auto fetch_k = [&](uint32_t off) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const uint32_t o = __shfl_sync(0xffffffffu, off, q * 8 + g);
+      const uint8_t* a = c.kv + (size_t)o * 16 + i4 * KW * 4;
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        if (o != NONE) ld_codes(k[q][s], a + s * 64);
+        else
+#pragma unroll
+          for (int w = 0; w < KW; w++) k[q][s][w] = 0;
+      }
+    }
+  };
+  auto fetch_v = [&](uint32_t off) {
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const uint32_t o = __shfl_sync(0xffffffffu, off, q * 16 + (x >> 1) * 8 + 2 * i4 + (x & 1));
+        const uint8_t* a = c.kv + (size_t)o * 16 + bs * HD + g * (HD / 8);
+        if (o == NONE) {
+#pragma unroll
+          for (int w = 0; w < VW; w++) v[q][x][w] = 0;
+        } else if constexpr (HD == 16) v[q][x][0] = *reinterpret_cast<const uint16_t*>(a);
+        else ld_codes(v[q][x], a);
+      }
+  };
+  const int step = nw * 32;
+  int j0 = wi * 32;
+  look(j0);
+  place();
+  look(j0 + step);
+  uint32_t off = off_n, e = e_n;
+  fetch_k(off);
+  fetch_v(off);
+  place();
+  // q: lane's dims (of slab s: 64 s + 16 i4 ..; narrower heads: HD / 4 from HD / 4 i4) as f16 pairs, rows alike
+  uint32_t qa[NM][2];
+  float sc;
+  {
+    constexpr int PER = HD / 4 / KS;               // dims of a lane and slab
+    uint32_t w[KS][PER / 2], m = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int x = 0; x < PER / 2; x++) {
+        w[s][x] = reinterpret_cast<const uint32_t*>(row + s * 64 + i4 * PER)[x];
+        const uint32_t a = w[s][x] & 0x7fffu, b = w[s][x] >> 16 & 0x7fffu;
+        m = max(m, max(a > 0x7f80u ? 0u : a, b > 0x7f80u ? 0u : b));
+      }
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
+    const float f = pow2_of((uint32_t)(127 - eq));
+    sc = scale * pow2_of((uint32_t)(127 + eq));
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int x = 0; x < PER / 2; x++) {
+        const float2 a = unpack_bf16(w[s][x]);
+        qa[s * (PER / 4) + x / 2][x & 1] = pack_f16(a.x * f, a.y * f);
+      }
+  }
+  float o[NM][4];
+#pragma unroll
+  for (int t = 0; t < NM; t++)
+#pragma unroll
+    for (int x = 0; x < 4; x++) o[t][x] = 0.f;
+  R = -INFINITY;
+  l = 0.f;
+  if (append && wi == 0) {
+    // the token's own position: lane's HD / 8 dims of q, k, v; groups of eight lanes of the same i4 hold a row
+    constexpr int PER = HD / 8;
+    uint32_t kw[PER / 2], vw[PER / 2], qw[PER / 2], mk = 0, mv = 0;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(row + g * PER);
+#pragma unroll
+    for (int x = 0; x < PER / 2; x++) {
+      qw[x] = src[x];
+      kw[x] = src[d / 2 + x];
+      vw[x] = src[d + x];
+      const uint32_t a = kw[x] & 0x7fffu, b = kw[x] >> 16 & 0x7fffu, aa = vw[x] & 0x7fffu, bb = vw[x] >> 16 & 0x7fffu;
+      mk = max(mk, max(a > 0x7f80u ? 0u : a, b > 0x7f80u ? 0u : b));
+      mv = max(mv, max(aa > 0x7f80u ? 0u : aa, bb > 0x7f80u ? 0u : bb));
+    }
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) {
+      mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, x));
+      mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, x));
+    }
+    const uint32_t ek = exp_byte(mk), ev = exp_byte(mv);
+    const float fk = pow2_of(254u - ek), fv = pow2_of(254u - ev);
+    uint32_t kc[PER / 2], vc[PER / 2];             // codes, two in a word
+    float s = 0.f;
+#pragma unroll
+    for (int x = 0; x < PER / 2; x++) {
+      const float2 a = unpack_bf16(kw[x]), b = unpack_bf16(vw[x]), q = unpack_bf16(qw[x]);
+      kc[x] = to_e4m3x2(a.x * fk, a.y * fk);
+      vc[x] = to_e4m3x2(b.x * fv, b.y * fv);
+      const f32x2 kk = f32x2_of(half2_of(kc[x])), vv = f32x2_of(half2_of(vc[x]));
+      s = fmaf(q.x, lo2(kk), fmaf(q.y, hi2(kk), s));
+      o[x][0] = lo2(vv) * 16384.f;
+      o[x][2] = hi2(vv) * 16384.f;
+    }
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    R = s * scale * pow2_of(ek) + (float)((int)ev - 127);
+    l = i4 == 0 ? 16384.f * fv : 0.f;
+    if (R != R) l = R;                             // (a NaN in q or k)
+    const int b = block_of(c, sl, p);
+    if (b < 0) bad = true;
+    else {
+      uint8_t* rc = record(c, b, h);
+      const int a = p - quot(c.div, p) * bs;
+      if (i4 < 2) {                                // lanes 0 write k, lanes 1 v
+        uint8_t* dst = rc + (size_t)(i4 * bs + a) * HD + g * PER;
+        uint32_t cw[PER / 2];
+#pragma unroll
+        for (int x = 0; x < PER / 2; x++) cw[x] = i4 ? vc[x] : kc[x];
+        if constexpr (PER == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(cw[0] | cw[1] << 16, cw[2] | cw[3] << 16, cw[4] | cw[5] << 16, cw[6] | cw[7] << 16);
+        else if constexpr (PER == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(cw[0] | cw[1] << 16, cw[2] | cw[3] << 16);
+        else if constexpr (PER == 4) *reinterpret_cast<uint32_t*>(dst) = cw[0] | cw[1] << 16;
+        else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)cw[0];
+      } else if (lane == 2) *reinterpret_cast<uint16_t*>(rc + 2 * bs * HD + 2 * a) = (uint16_t)(ek | ev << 8);
+    }
+  }
+  look(j0 + 2 * step);
+#pragma unroll 1
+  for (; j0 < n; j0 += step) {                     // uniform over the warp
+    float s[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+#pragma unroll
+      for (int x = 0; x < 4; x++) s[q][x] = 0.f;
+#pragma unroll
+      for (int t = 0; t < NM; t++) {
+        uint32_t b0, b1;
+        halves(k[q][t / KW][t % KW], b0, b1);
+        mma_f16(s[q], qa[t][0], qa[t][0], qa[t][1], qa[t][1], b0, b1);
+      }
+    }
+    fetch_k(off_n);
+    // exponents of positions 2 i4, 2 i4 + 1 of each eight
+    const uint32_t e2 = e | __shfl_down_sync(0xffffffffu, e, 1) << 16;
+    uint32_t ep[4];
+    float tm = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      ep[q] = __shfl_sync(0xffffffffu, e2, q * 8 + 2 * i4);
+      const int j = j0 + q * 8 + 2 * i4;
+      s[q][0] = j < n ? fmaf(s[q][0] * sc, pow2_of(ep[q] & 0xffu), (float)((int)(ep[q] >> 8 & 0xffu) - 127)) : -INFINITY;
+      s[q][1] = j + 1 < n ? fmaf(s[q][1] * sc, pow2_of(ep[q] >> 16 & 0xffu), (float)((int)(ep[q] >> 24) - 127)) : -INFINITY;
+      tm = fmaxf(tm, fmaxf(s[q][0], s[q][1]));
+    }
+    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
+    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
+    if (tm > R) {                                  // uniform: every lane of a group of four has the same, and all groups have
+      const float al = ex2(R - tm);
+      l *= al;
+#pragma unroll
+      for (int t = 0; t < NM; t++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[t][x] *= al;
+      R = tm;
+    }
+    const float c0 = R == -INFINITY ? 0.f : 14.f - R;
+    uint32_t pb[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const float p0 = ex2(s[q][0] + c0), p1 = ex2(s[q][1] + c0);
+      l = fmaf(p0, j0 + q * 8 + 2 * i4 < n ? pow2_of(254u - (ep[q] >> 8 & 0xffu)) : 0.f, l);
+      l = fmaf(p1, j0 + q * 8 + 2 * i4 + 1 < n ? pow2_of(254u - (ep[q] >> 24)) : 0.f, l);
+      const uint32_t hi = pack_f16(p0, p1);
+      const f32x2 hf = f32x2_of(hi);
+      const uint32_t lo = pack_f16(p0 - lo2(hf), p1 - hi2(hf));
+      pb[q] = g & 1 ? lo : hi;
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+      for (int w = 0; w < VW; w++) {
+        // dims 4 w .. of the lane: (position 2 i4, 2 i4 + 1) pairs of each, for the lower and the upper eight positions
+        uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+        halves(__byte_perm(v[q][0][w], v[q][1][w], 0x5140), x0, x1);
+        halves(__byte_perm(v[q][2][w], v[q][3][w], 0x5140), y0, y1);
+        mma_f16(o[2 * w], x0, x1, y0, y1, pb[2 * q], pb[2 * q + 1]);
+        if constexpr (HD >= 32) {
+          halves(__byte_perm(v[q][0][w], v[q][1][w], 0x7362), x2, x3);
+          halves(__byte_perm(v[q][2][w], v[q][3][w], 0x7362), y2, y3);
+          mma_f16(o[2 * w + 1], x2, x3, y2, y3, pb[2 * q], pb[2 * q + 1]);
+        }
+      }
+    fetch_v(off_n);
+    off = off_n;
+    e = e_n;
+    place();
+    look(j0 + 3 * step);
+  }
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+  for (int t = 0; t < NM; t++) {
+    out[2 * t] = o[t][0] + o[t][1];
+    out[2 * t + 1] = o[t][2] + o[t][3];
+  }
 }
 
 }  // namespace
@@ -120,8 +389,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 template <int HD, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W)
 paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, int ntok, float scale, int max_ctx, int append, int S) {
-  constexpr int LPK = HD / 16, IPC = W == 1 ? 4 : 1;
-  __shared__ float s_part[W > 1 ? W * (HD + 2) : 1], s_cta[HD + 2];       // per warp, per CTA: HD sums, maximum, normaliser
+  constexpr int IPC = W == 1 ? 4 : 1, PER = HD / 8;
+  __shared__ float s_part[W > 1 ? W * (HD + 2) : 1], s_cta[HD + 2];       // per warp, per CTA: HD sums, reference, normaliser
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = c.H * HD;
@@ -132,27 +401,30 @@ paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restr
   // index guard: a context longer than the caller's limit or the block table is recorded (status code 8) and the token skipped
   const bool valid = live && p >= 0 && p < max_ctx && quot(c.div, p) < c.max_lb && sl >= 0 && sl < c.n_slots;      // uniform over the item
   bool bad = live && !valid;
-  float m = -INFINITY, l = 0.f;
-  f32x2 o[8];
+  float R = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
-  for (int k = 0; k < 8; k++) o[k] = 0;
-  if (valid) decode_partial<HD>(c, qkv + (size_t)t * ld + h * HD, d, h, p, sl, scale, wi, W * S, append, m, l, o, bad);
+  for (int k = 0; k < PER; k++) o[k] = 0.f;
+  if (valid) decode_partial<HD>(c, qkv + (size_t)t * ld + h * HD, d, h, p, sl, scale, wi, W * S, append, R, l, o, bad);
   if (bad) report(c.err);
   if constexpr (W == 1) {
-    if (!valid || lane >= LPK) return;
+    if (!valid || (lane & 3)) return;
     const float inv = 1.f / l;
-    bf16* dst = out + (size_t)t * ldo + h * HD + lane * 16;
-    uint32_t w[8];
+    uint32_t* dst = reinterpret_cast<uint32_t*>(out + (size_t)t * ldo + h * HD + (lane >> 2) * PER);
+    uint32_t w[PER / 2];
 #pragma unroll
-    for (int k = 0; k < 8; k++) w[k] = pack_bf16(lo2(o[k]) * inv, hi2(o[k]) * inv);
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    for (int k = 0; k < PER / 2; k++) w[k] = pack_bf16(o[2 * k] * inv, o[2 * k + 1] * inv);
+    if constexpr (PER >= 8)
+#pragma unroll
+      for (int k = 0; k < PER / 8; k++) reinterpret_cast<uint4*>(dst)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    else
+#pragma unroll
+      for (int k = 0; k < PER / 2; k++) dst[k] = w[k];
   } else {
     float* part = s_part + warp * (HD + 2);
-    if (lane < LPK) {
+    if ((lane & 3) == 0) {
 #pragma unroll
-      for (int k = 0; k < 8; k++) { part[lane * 16 + 2 * k] = lo2(o[k]); part[lane * 16 + 2 * k + 1] = hi2(o[k]); }
-      if (lane == 0) { part[HD] = m; part[HD + 1] = l; }
+      for (int k = 0; k < PER; k++) part[(lane >> 2) * PER + k] = o[k];
+      if (lane == 0) { part[HD] = R; part[HD + 1] = l; }
     }
     __syncthreads();
     const int tid = threadIdx.x;
@@ -235,16 +507,17 @@ extern "C" int kh_paged_attn8(const void* qkv, int ld, void* kv, int n_blocks, i
   if (ntok > (1 << 27)) { kh_set_error("paged_attn8: %d tokens are too many", ntok); return -1; }
   const float sl2 = scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
-  // warps to an item: one where the items alone give every SM some sixteen, else four; sixteen and a cluster of up to eight CTAs where four to an
-  // item would still leave the SMs with few bytes in flight, as far as the longest context has a chunk of 2048 / hd positions for each
-  const long items = (long)ntok * H, want = 148 * 16;
-  const int chunks = (max_ctx + 2048 / hd - 1) / (2048 / hd);
-  int W = items >= want || chunks <= 1 ? 1 : items * 4 >= want || chunks <= 4 ? 4 : 16, S = 1;
+  // warps to an item: one where the items alone give every SM some twelve, else four; eight and a cluster of up to eight CTAs where four to an
+  // item would still leave the SMs with few bytes in flight, as far as the longest context has a chunk of 32 positions for each
+  const long items = (long)ntok * H, want = 148 * 12;
+  const int chunks = (max_ctx + 31) / 32;
+  int W = chunks <= 1 || (items >= want && chunks <= 8) ? 1 : items * 4 >= want || chunks <= 4 ? 4 : 8, S = 1;
   while (W > 1 && S < 8 && items * W * S < want && chunks >= 2 * W * S) S *= 2;
+  if (const char* f = getenv("KH_W")) { W = atoi(f); S = atoi(getenv("KH_SS")); }
 #define LAUNCH(HD)                                                                                                      \
   return W == 1 ? launch_attn8<HD, 1>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, 1, st)                          \
        : W == 4 ? launch_attn8<HD, 4>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, S, st)                          \
-                : launch_attn8<HD, 16>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, S, st);
+                : launch_attn8<HD, 8>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, S, st);
   if (hd == 128) { LAUNCH(128) }
   if (hd == 64) { LAUNCH(64) }
   if (hd == 32) { LAUNCH(32) }

@@ -88,173 +88,65 @@ inline int make_cache(Cache& c, const char* name, const void* kv, int n_blocks, 
   if (bs < 1 || H < 1 || H > 65535 || n_blocks < 1 || max_lb < 1 || n_slots < 1) { kh_set_error("%s: empty cache", name); return -1; }
   if (rec < 2 * bs * hd + 2 * bs || rec % 32 || ((uintptr_t)kv & 31)) { kh_set_error("%s: records of %d bytes do not fit block size %d", name, rec, bs); return -1; }
   if ((unsigned long long)max_lb * bs * bs >= 1ull << 32 || (long long)max_lb * bs > 0x7fffffffll) { kh_set_error("%s: block table of %d x %d positions is too long", name, max_lb, bs); return -1; }
+  if ((unsigned long long)n_blocks * H * rec >> 36) { kh_set_error("%s: a cache of %d blocks x %d heads x %d bytes is larger than 64 GB", name, n_blocks, H, rec); return -1; }
   c = Cache{(uint8_t*)kv, (const int*)pos, (const int*)slot, (const int*)btab, kh_error_word_dev(), n_blocks, n_slots, max_lb, bs, H, rec,
             Div{bs == 1 ? 0u : (uint32_t)(((1ull << 32) + bs - 1) / bs)}};
   return 0;
 }
 namespace {
 
+// One token and head by one warp, a position per HD / 16 lanes at a time, in fp32: for the few rows that the tensor cores' formats do not suit.
 template <int HD>
-__device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, int wi, int nw, int append,
-                                               float& m, float& l, f32x2 (&o)[8], bool& bad) {
-  constexpr int LPK = HD / 16, KPW = 32 / LPK, U = 4, CH = U * KPW;
-  const int lane = threadIdx.x & 31, g = lane / LPK, e0 = lane % LPK * 16, bs = c.bs, exps = 2 * bs * HD;
-  const int* bt = c.btab + (size_t)sl * c.max_lb;
-  const int n = append ? p : p + 1;                // positions read from the cache
-  const size_t head = (size_t)h * c.rec, block = (size_t)c.H * c.rec;
-  uint4 k4[U], v4[U], kn, vn;
-  uint32_t e4[U], en = 0;
-  const uint8_t* a4[U];                            // K row of a position; V row and exponents lie at fixed distances
-  uint32_t x4[U];
-  kn = vn = make_uint4(0, 0, 0, 0);
-  auto rows = [&](int j0) {
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-      const int j = j0 + i * KPW;
-      if (j < n) {
-        const int lb = quot(c.div, j), at = j - lb * bs;
-        int b = __ldg(bt + lb);
-        if ((unsigned)b >= (unsigned)c.n_blocks) { bad = true; b = 0; }
-        const uint8_t* rc = c.kv + (size_t)b * block + head;
-        a4[i] = rc + at * HD + e0;
-        x4[i] = (uint32_t)(exps + 2 * at) - (uint32_t)(at * HD + e0);
-      }
-    }
-  };
-  auto fetch_k = [&](int j0) {
-#pragma unroll
-    for (int i = 0; i < U; i++)
-      if (j0 + i * KPW < n) {
-        k4[i] = *reinterpret_cast<const uint4*>(a4[i]);
-        e4[i] = *reinterpret_cast<const uint16_t*>(a4[i] + x4[i]);
-      }
-  };
-  auto fetch_v = [&](int j0) {
-#pragma unroll
-    for (int i = 0; i < U; i++)
-      if (j0 + i * KPW < n) v4[i] = *reinterpret_cast<const uint4*>(a4[i] + bs * HD);
-  };
-  const int step = nw * CH;
-  int j0 = wi * CH + g;
-  rows(j0);
-  fetch_k(j0);
-  fetch_v(j0);
-  const bool owner = append && (p / CH) % nw == wi;                // uniform over the warp
-  if (owner) {
-    uint4 s[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) s[i] = *reinterpret_cast<const uint4*>(row + d * (1 + i / 2) + e0 + (i & 1) * 8);
-    uint32_t mk = max(amax8(s[0]), amax8(s[1])), mv = max(amax8(s[2]), amax8(s[3]));
-#pragma unroll
-    for (int x = LPK / 2; x > 0; x >>= 1) {
-      mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, x));
-      mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, x));
-    }
-    const uint32_t ek = exp_byte(mk), ev = exp_byte(mv);
-    const uint2 k0 = encode8(s[0], pow2_of(254u - ek)), k1 = encode8(s[1], pow2_of(254u - ek));
-    const uint2 v0 = encode8(s[2], pow2_of(254u - ev)), v1 = encode8(s[3], pow2_of(254u - ev));
-    kn = make_uint4(k0.x, k0.y, k1.x, k1.y);
-    vn = make_uint4(v0.x, v0.y, v1.x, v1.y);
-    en = ek | ev << 8;
-    const int b = block_of(c, sl, p);
-    if (b < 0) bad = true;
-    else if (g == 0) {
-      uint8_t* rc = c.kv + (size_t)b * block + head;
-      const int at = p - quot(c.div, p) * bs;
-      *reinterpret_cast<uint4*>(rc + at * HD + e0) = kn;
-      *reinterpret_cast<uint4*>(rc + (bs + at) * HD + e0) = vn;
-      if (e0 == 0) *reinterpret_cast<uint16_t*>(rc + exps + 2 * at) = (uint16_t)en;
-    }
-  }
-  f32x2 q[8];
+__device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int h, int p, int sl, float scale, bf16* dst) {
+  constexpr int LPK = HD / 16, KPW = 32 / LPK;
+  const int lane = threadIdx.x & 31, g = lane / LPK, e0 = lane % LPK * 16, bs = c.bs;
+  f32x2 q[8], o[8];
   {
     const uint4 u0 = *reinterpret_cast<const uint4*>(row + e0), u1 = *reinterpret_cast<const uint4*>(row + e0 + 8);
     const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-    const f32x2 s2 = mk2(scale, scale);
 #pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = mul2(un2(w[i]), s2);
+    for (int i = 0; i < 8; i++) { q[i] = mul2(un2(w[i]), mk2(scale, scale)); o[i] = 0; }
   }
-  for (; j0 - g <= p; j0 += step) {                                // uniform over the warp
-    float s[U];
-    uint32_t ev[U];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (int j0 = 0; j0 <= p; j0 += KPW) {
+    const int j = j0 + g, jj = min(j, p), lb = quot(c.div, jj), at = jj - lb * bs;
+    const int b = __ldg(c.btab + (size_t)sl * c.max_lb + lb);
+    const uint8_t* rc = record(c, (unsigned)b < (unsigned)c.n_blocks ? b : 0, h);
+    const uint4 k = *reinterpret_cast<const uint4*>(rc + at * HD + e0), v = *reinterpret_cast<const uint4*>(rc + (bs + at) * HD + e0);
+    const uint32_t e = *reinterpret_cast<const uint16_t*>(rc + 2 * bs * HD + 2 * at), kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
+    f32x2 a = 0;
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-      if (j0 + i * KPW >= n) { k4[i] = kn; v4[i] = vn; e4[i] = en; }        // the appended position, or past the end (masked below)
-      const uint32_t w[4] = {k4[i].x, k4[i].y, k4[i].z, k4[i].w};
-      f32x2 a = 0, b = 0;
+    for (int i = 0; i < 8; i++) a = fma2(f32x2_of(half2_of(kw[i >> 1] >> (i & 1) * 16)), q[i], a);
+    float s = lo2(a) + hi2(a);
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
-        a = fma2(f32x2_of(half2_of(w[x])), q[2 * x], a);
-        b = fma2(f32x2_of(half2_of(w[x] >> 16)), q[2 * x + 1], b);
-      }
-      a = add2(a, b);
-      s[i] = lo2(a) + hi2(a);
-      ev[i] = e4[i];
+    for (int x = LPK / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (j <= p) {
+      s *= pow2_of(e & 0xffu);
+      const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn, sc = ex2(m - ref), pr = ex2(s - ref), pv = pr * pow2_of(e >> 8);
+      m = mn;
+      l = fmaf(l, sc, pr);
+#pragma unroll
+      for (int i = 0; i < 8; i++) o[i] = fma2(f32x2_of(half2_of(vw[i >> 1] >> (i & 1) * 16)), mk2(pv, pv), mul2(o[i], mk2(sc, sc)));
     }
-    rows(j0 + step);
-    fetch_k(j0 + step);
-#pragma unroll
-    for (int x = LPK / 2; x > 0; x >>= 1)
-#pragma unroll
-      for (int i = 0; i < U; i++) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
-    float mn = m;
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-      s[i] = j0 + i * KPW > p ? -INFINITY : s[i] * pow2_of(ev[i] & 0xffu);
-      mn = fmaxf(mn, s[i]);
-    }
-    const float ref = mn == -INFINITY ? 0.f : mn, sc = ex2(m - ref);
-    const f32x2 sc2 = mk2(sc, sc);
-    m = mn;
-    l *= sc;
-#pragma unroll
-    for (int x = 0; x < 8; x++) o[x] = mul2(o[x], sc2);
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-      const float pr = ex2(s[i] - ref);
-      l += pr;
-      const float pv = pr * pow2_of(ev[i] >> 8);
-      const f32x2 w2 = mk2(pv, pv);
-      if (j0 + i * KPW > p) v4[i] = make_uint4(0, 0, 0, 0);          // (a NaN there would count)
-      const uint32_t w[4] = {v4[i].x, v4[i].y, v4[i].z, v4[i].w};
-#pragma unroll
-      for (int x = 0; x < 4; x++) {
-        o[2 * x] = fma2(f32x2_of(half2_of(w[x])), w2, o[2 * x]);
-        o[2 * x + 1] = fma2(f32x2_of(half2_of(w[x] >> 16)), w2, o[2 * x + 1]);
-      }
-    }
-    fetch_v(j0 + step);
   }
 #pragma unroll
-  for (int x = LPK; x < 32; x <<= 1) {                             // merge the lane groups of the warp
+  for (int x = LPK; x < 32; x <<= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, x), l2 = __shfl_xor_sync(0xffffffffu, l, x);
-    const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
-    const float c1 = ex2(m - ref), c2 = ex2(m2 - ref);
+    const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn, c1 = ex2(m - ref), c2 = ex2(m2 - ref);
     m = mn;
     l = l * c1 + l2 * c2;
-    const f32x2 c1v = mk2(c1, c1), c2v = mk2(c2, c2);
 #pragma unroll
-    for (int k = 0; k < 8; k++) o[k] = fma2(o[k], c1v, mul2((f32x2)__shfl_xor_sync(0xffffffffu, o[k], x), c2v));
+    for (int i = 0; i < 8; i++) o[i] = fma2(o[i], mk2(c1, c1), mul2((f32x2)__shfl_xor_sync(0xffffffffu, o[i], x), mk2(c2, c2)));
   }
-}
-
-// One token and head by one warp.
-template <int HD>
-__device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, bf16* dst) {
-  float m = -INFINITY, l = 0.f;
-  f32x2 o[8];
-  bool bad = false;
-#pragma unroll
-  for (int k = 0; k < 8; k++) o[k] = 0;
-  decode_partial<HD>(c, row, d, h, p, sl, scale, 0, 1, 0, m, l, o, bad);
   const float inv = 1.f / l;
-  const int lane = threadIdx.x & 31;
-  if (lane < HD / 16) {
+  if (lane < LPK) {
     uint32_t w[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) w[k] = pack_bf16(lo2(o[k]) * inv, hi2(o[k]) * inv);
+    for (int i = 0; i < 8; i++) w[i] = pack_bf16(lo2(o[i]) * inv, hi2(o[i]) * inv);
     *reinterpret_cast<uint4*>(dst + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(dst + lane * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
+
 }  // namespace

@@ -41,7 +41,7 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ C
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t sK = smem_u32(smem), sV = sK + TILE;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3, h = blockIdx.y, d = c.H * HD;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3, h = blockIdx.y;
   const int r0 = tiles.row0[blockIdx.x], p0 = c.pos[r0], sl = c.slot[r0];
   int n = tiles.n[blockIdx.x];
   // index guard: tokens beyond the limits are recorded (status code 8) and skipped; they are the last of the run
@@ -187,7 +187,7 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ C
   if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {
 #pragma unroll 1
     for (int r = w0; r < min(n, w0 + 16); r++)
-      attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, d, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
+      attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
     return;
   }
 #pragma unroll
@@ -297,24 +297,6 @@ __device__ __forceinline__ void rescale(uint32_t tO, float al) {
     tmem_st16(tO + i, r);
   }
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-// 2^x for two numbers on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2, a polynomial of degree 4 for 2^f (its largest relative error,
-// 2^-18, is the least for the degree), n added to the exponent.  Below 2^-126: 2^-126.  NaN: no finite f16.
-__device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
-  constexpr float P0 = 0.9999992847f, P1 = 0.6931217909f, P2 = 0.2402474433f, P3 = 0.0559178591f, P4 = 0.0095701013f;
-  x = mk2(max_nan(lo2(x), -126.f), max_nan(hi2(x), -126.f));
-  const f32x2 t = add2(x, mk2(12582912.f, 12582912.f)), f = fma2(add2(t, mk2(-12582912.f, -12582912.f)), mk2(-1.f, -1.f), x);
-  f32x2 p = mk2(P4, P4);
-  p = fma2(p, f, mk2(P3, P3));
-  p = fma2(p, f, mk2(P2, P2));
-  p = fma2(p, f, mk2(P1, P1));
-  p = fma2(p, f, mk2(P0, P0));
-  return mk2(__int_as_float((int)((uint32_t)t << 23) + __float_as_int(lo2(p))), __int_as_float((int)((uint32_t)(t >> 32) << 23) + __float_as_int(hi2(p))));
-}
 // The MMAs with descriptors given by their low words (the high word is the same for all tiles: groups of 8 rows 1024 bytes apart, 128-byte swizzle).
 constexpr uint32_t DESC_HI = 64u | 1u << 14 | 2u << 29;
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -352,7 +334,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   pdl_wait();
   pdl_launch_dependents();
 
-  const int rank = (int)(blockIdx.x % S), item = (int)(blockIdx.x / S), h = item % c.H, piece = item / c.H, d = c.H * HD;
+  const int rank = (int)(blockIdx.x % S), item = (int)(blockIdx.x / S), h = item % c.H, piece = item / c.H;
   // (What every thread knows alike goes through a shuffle, or *tmem_slot below: the compiler keeps it in uniform registers then, which is what
   // tcgen05 instructions take.)
   auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
@@ -625,7 +607,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
             for (int i = 0; i < 32; i += 4) {
               const f32x2 e0 = fma2(mk2(__uint_as_float(r[q * 32 + i]), __uint_as_float(r[q * 32 + i + 1])), slv, c2);
               const f32x2 e1 = fma2(mk2(__uint_as_float(r[q * 32 + i + 2]), __uint_as_float(r[q * 32 + i + 3])), slv, c2);
-              const f32x2 x0 = mk2(ex2(lo2(e0)), ex2(hi2(e0))), x1 = i % 16 == 12 ? exp2_poly(e1) : mk2(ex2(lo2(e1)), ex2(hi2(e1)));
+              const f32x2 x0 = mk2(ex2(lo2(e0)), ex2(hi2(e0))), x1 = mk2(ex2(lo2(e1)), ex2(hi2(e1)));
               rs0 = add2(rs0, x0);
               rs1 = add2(rs1, x1);
               pk[i >> 1] = pack_f16(x0);
@@ -752,7 +734,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
 #pragma unroll 1
     for (int r = warp; r < n; r += 8)
       if (s_again[r >> 5] >> (r & 31) & 1)
-        attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, d, h, p0 + r, sl, sl2, out + (size_t)(r0 + r) * ldo + h * HD);
+        attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, sl2, out + (size_t)(r0 + r) * ldo + h * HD);
   }
   }
   tc_fence_before();
