@@ -10,7 +10,6 @@
 // rounding is the one to e4m3 (half a step, 2^-4 of the value at most, or 2^-10 2^e for values below 2^-6 2^e), and the stored value is exact in bf16.  Magnitudes above 448 2^63
 // and infinities become the largest code, NaN stays NaN and does not count for the maximum.
 #include "paged8.cuh"
-#include <stdlib.h>
 
 extern "C" int kh_kv8_record_bytes(int bs, int hd) { return (2 * bs * hd + 2 * bs + 31) / 32 * 32; }
 
@@ -106,7 +105,7 @@ extern "C" int kh_read_kv8(const void* kv, int n_blocks, int rec, void* k, void*
 // A warp takes chunks of 32 consecutive positions; W warps of a CTA and the S CTAs of a cluster share a (token, head), chunk i goes to warp
 // i mod (S W).  The products run on mma.sync (f16, fp32 sums), because what bounds a plain loop is not memory but its 4.8 instructions per code (conversion to fp32,
 // multiply, reduction): 313 us for 128 sequences of 1000 to 4096 positions, 16 heads of 128.  Codes become f16 with one instruction for two:
-//   S:  A = q in every row (so each lane has the scores it needs without a shuffle), B = K: lanes 4 g + i hold 1/4 of the codes of position g of eight;
+//   S:  A = K, B = q in every column: lanes 4 g + i hold 1/4 of the codes of position g of each eight, and get its score;
 //   O:  A = V^T, B = P: lanes 4 g + i hold 1/8 of the dims, of positions 2 i, 2 i + 1 of each eight; two positions' codes are interleaved by byte permutation.
 // What f16 cannot hold is taken out as powers of two and put back in fp32: q = q' 2^eq (largest |q'| in [2^14, 2^15)), scores times 2^ek, and
 // P' = 2^(s + ev - R + 14) with R the running maximum of s + ev, so that V's codes enter as they are.  P' goes in as two f16 terms, in the even and
@@ -131,11 +130,13 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 __device__ __forceinline__ void halves(uint32_t w, uint32_t& a, uint32_t& b) {
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
 }
-template <int WORDS>
+// (volatile: the compiler would move loads for the next turn down to their use)
+template <int BYTES, int WORDS>
 __device__ __forceinline__ void ld_codes(uint32_t (&r)[WORDS], const uint8_t* p) {
-  if constexpr (WORDS == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
-  else if constexpr (WORDS == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); r[0] = v.x; r[1] = v.y; }
-  else r[0] = *reinterpret_cast<const uint32_t*>(p);
+  if constexpr (BYTES == 16) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(p));
+  else if constexpr (BYTES == 8) asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+  else if constexpr (BYTES == 4) asm volatile("ld.global.b32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+  else asm volatile("{\n\t.reg .b16 h;\n\tld.global.b16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(r[0]) : "l"(p));
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
@@ -148,72 +149,66 @@ template <int HD>
 __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, int wi, int nw, int append,
                                                float& R, float& l, float (&out)[HD / 8], bool& bad) {
   constexpr int KS = HD == 128 ? 2 : 1, KW = HD / 16 / KS, VW = HD >= 32 ? HD / 32 : 1, NM = HD / 16;       // K: slabs of 64 codes, words per lane; V: words per lane; MMAs across hd
-  constexpr uint32_t NONE = 0xffffffffu;
   const int lane = threadIdx.x & 31, g = lane >> 2, i4 = lane & 3, bs = c.bs;
   const int* bt = c.btab + (size_t)sl * c.max_lb;
   const int n = append ? p : p + 1;                // positions read from the cache
-  // lane's position of a chunk: its K row in units of 16 bytes from the cache's start (NONE: past the end), and its exponents
-  uint32_t off_n = NONE, e_n = 0;                  // of the next chunk to be fetched
-  int blk = 0, at = -1;                            // of the one after
-  auto look = [&](int j0) {
-    const int j = j0 + lane;
-    at = -1;
-    if (j < n) {
-      const int lb = quot(c.div, j);
-      at = j - lb * bs;
-      asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(blk) : "l"(bt + lb));
-    }
-  };
-  auto place = [&]() {
-    off_n = NONE;
-    e_n = 0;
-    if (at >= 0) {
-      if ((unsigned)blk >= (unsigned)c.n_blocks) { bad = true; blk = 0; }
-      const uint32_t rc = ((uint32_t)blk * c.H + h) * (uint32_t)(c.rec >> 4);
-      off_n = rc + at * (HD / 16);
-      uint16_t e;
-      asm volatile("ld.global.b16 %0, [%1];" : "=h"(e) : "l"(c.kv + (size_t)rc * 16 + 2 * bs * HD + 2 * at));
-      e_n = e;
-    }
-  };
-  uint32_t k[4][KS][KW], v[2][4][VW];              // [eight positions][slab][word]; [sixteen positions][one of a lane's four][word]
-  auto fetch_k = [&](uint32_t off) {
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const uint32_t o = __shfl_sync(0xffffffffu, off, q * 8 + g);
-      const uint8_t* a = c.kv + (size_t)o * 16 + i4 * KW * 4;
-#pragma unroll
-      for (int s = 0; s < KS; s++) {
-        if (o != NONE) ld_codes(k[q][s], a + s * 64);
-        else
-#pragma unroll
-          for (int w = 0; w < KW; w++) k[q][s][w] = 0;
-      }
-    }
-  };
-  auto fetch_v = [&](uint32_t off) {
-#pragma unroll
-    for (int q = 0; q < 2; q++)
-#pragma unroll
-      for (int x = 0; x < 4; x++) {
-        const uint32_t o = __shfl_sync(0xffffffffu, off, q * 16 + (x >> 1) * 8 + 2 * i4 + (x & 1));
-        const uint8_t* a = c.kv + (size_t)o * 16 + bs * HD + g * (HD / 8);
-        if (o == NONE) {
-#pragma unroll
-          for (int w = 0; w < VW; w++) v[q][x][w] = 0;
-        } else if constexpr (HD == 16) v[q][x][0] = *reinterpret_cast<const uint16_t*>(a);
-        else ld_codes(v[q][x], a);
-      }
-  };
+  // A lane looks up one position of a chunk (lanes past the end of the context: its last position, or one of the same eight; masked below): its block, two chunks before the
+  // chunk's K is fetched; its exponents and its K row (in units of 16 bytes from the cache's start) one chunk before.  No load stands behind a condition:
+  // its registers would be copied, and waited for, at once.
   const int step = nw * 32;
   int j0 = wi * 32;
-  look(j0);
-  place();
-  look(j0 + step);
-  uint32_t off = off_n, e = e_n;
-  fetch_k(off);
-  fetch_v(off);
-  place();
+  const bool by8 = bs % 8 == 0;                    // then eight positions from a multiple of eight lie in one record
+  const int last = max(n - 1, 0);
+  struct Look { int blk, at; };
+  auto look = [&](int j0) {
+    const int j = min(j0 + lane, by8 ? (last & ~7) + (lane & 7) : last), lb = quot(c.div, j);
+    Look k;
+    k.at = j - lb * bs;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(k.blk) : "l"(bt + lb));
+    return k;
+  };
+  uint32_t e_n, ko[4], vo[8];                      // of the next chunk to be fetched: exponents, rows of the positions whose K and V the lane takes
+  auto place = [&](Look k) {
+    bad |= (unsigned)k.blk >= (unsigned)c.n_blocks;
+    const uint32_t rc = ((uint32_t)min((unsigned)k.blk, (unsigned)c.n_blocks - 1) * c.H + h) * (uint32_t)(c.rec >> 4), off = rc + k.at * (HD / 16);
+    uint16_t e;
+    asm volatile("ld.global.b16 %0, [%1];" : "=h"(e) : "l"(c.kv + (size_t)rc * 16 + 2 * bs * HD + 2 * k.at));
+    e_n = e;
+    if (by8) {
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const uint32_t first = __shfl_sync(0xffffffffu, off, q * 8);
+        ko[q] = first + g * (HD / 16);
+        vo[2 * q] = first + 2 * i4 * (HD / 16);
+        vo[2 * q + 1] = first + (2 * i4 + 1) * (HD / 16);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        ko[q] = __shfl_sync(0xffffffffu, off, q * 8 + g);
+        vo[2 * q] = __shfl_sync(0xffffffffu, off, q * 8 + 2 * i4);
+        vo[2 * q + 1] = __shfl_sync(0xffffffffu, off, q * 8 + 2 * i4 + 1);
+      }
+    }
+  };
+  uint32_t k[4][KS][KW], v[2][4][VW], e;           // [eight positions][slab][word]; [sixteen positions][one of a lane's four][word]; lane's position
+  const uint8_t* const kb = c.kv + i4 * KW * 4;
+  const uint8_t* const vb = c.kv + bs * HD + g * (HD / 8);
+  auto fetch_k = [&]() {
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int s = 0; s < KS; s++) ld_codes<KW * 4>(k[q][s], kb + (size_t)ko[q] * 16 + s * 64);
+  };
+  auto fetch_v = [&]() {
+#pragma unroll
+    for (int q = 0; q < 8; q++) ld_codes<HD / 8>(v[q >> 2][q & 3], vb + (size_t)vo[q] * 16);
+  };
+  Look n0 = look(j0), n1 = look(j0 + step), n2 = look(j0 + 2 * step);
+  place(n0);
+  fetch_k();
+  fetch_v();
+  e = e_n;
   // q: lane's dims (of slab s: 64 s + 16 i4 ..; narrower heads: HD / 4 from HD / 4 i4) as f16 pairs, rows alike
   uint32_t qa[NM][2];
   float sc;
@@ -284,7 +279,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     R = s * scale * pow2_of(ek) + (float)((int)ev - 127);
-    l = i4 == 0 ? 16384.f * fv : 0.f;
+    l = g == 0 ? 16384.f * fv : 0.f;
     if (R != R) l = R;                             // (a NaN in q or k)
     const int b = block_of(c, sl, p);
     if (b < 0) bad = true;
@@ -303,37 +298,50 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
       } else if (lane == 2) *reinterpret_cast<uint16_t*>(rc + 2 * bs * HD + 2 * a) = (uint16_t)(ek | ev << 8);
     }
   }
-  look(j0 + 2 * step);
+  const uint32_t term = g & 1 ? 0x7632 : 0x5410;   // which f16 of two (first term, second term) words the lane's column of B takes
+  place(n1);
 #pragma unroll 1
   for (; j0 < n; j0 += step) {                     // uniform over the warp
-    float s[4][4];
+    n1 = n2;
+    n2 = look(j0 + 3 * step);
+    float s[4];                                    // of positions 8 q + g
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-#pragma unroll
-      for (int x = 0; x < 4; x++) s[q][x] = 0.f;
+    for (int x = 0; x < 2; x++) {
+      float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < NM; t++) {
-        uint32_t b0, b1;
-        halves(k[q][t / KW][t % KW], b0, b1);
-        mma_f16(s[q], qa[t][0], qa[t][0], qa[t][1], qa[t][1], b0, b1);
+        uint32_t a0, a1, a2, a3;
+        halves(k[2 * x][t / KW][t % KW], a0, a2);
+        halves(k[2 * x + 1][t / KW][t % KW], a1, a3);
+        mma_f16(a, a0, a1, a2, a3, qa[t][0], qa[t][1]);
       }
+      s[2 * x] = a[0];
+      s[2 * x + 1] = a[2];
     }
-    fetch_k(off_n);
-    // exponents of positions 2 i4, 2 i4 + 1 of each eight
-    const uint32_t e2 = e | __shfl_down_sync(0xffffffffu, e, 1) << 16;
-    uint32_t ep[4];
-    float tm = -INFINITY;
+    fetch_k();
+    float nev[4], tm = -INFINITY;                  // 2^-ev
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      ep[q] = __shfl_sync(0xffffffffu, e2, q * 8 + 2 * i4);
-      const int j = j0 + q * 8 + 2 * i4;
-      s[q][0] = j < n ? fmaf(s[q][0] * sc, pow2_of(ep[q] & 0xffu), (float)((int)(ep[q] >> 8 & 0xffu) - 127)) : -INFINITY;
-      s[q][1] = j + 1 < n ? fmaf(s[q][1] * sc, pow2_of(ep[q] >> 16 & 0xffu), (float)((int)(ep[q] >> 24) - 127)) : -INFINITY;
-      tm = fmaxf(tm, fmaxf(s[q][0], s[q][1]));
+      const uint32_t x = __shfl_sync(0xffffffffu, e, q * 8 + g), ev = x >> 8;
+      s[q] = fmaf(s[q] * sc, pow2_of(x & 0xffu), (float)((int)ev - 127));
+      nev[q] = pow2_of(254u - ev);
     }
-    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
-    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
-    if (tm > R) {                                  // uniform: every lane of a group of four has the same, and all groups have
+    if (j0 + 32 > n) {                             // the last chunk: scores past the end are -inf, values zero (a NaN there would count)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        if (j0 + q * 8 + g >= n) { s[q] = -INFINITY; nev[q] = 0.f; }
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+          if (j0 + q * 8 + 2 * i4 + x >= n)
+#pragma unroll
+            for (int w = 0; w < VW; w++) v[q >> 1][(q & 1) * 2 + x][w] = 0;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) tm = fmaxf(tm, s[q]);
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, x));
+    if (tm > R) {                                  // uniform over the warp
       const float al = ex2(R - tm);
       l *= al;
 #pragma unroll
@@ -345,14 +353,14 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
     const float c0 = R == -INFINITY ? 0.f : 14.f - R;
     uint32_t pb[4];
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const float p0 = ex2(s[q][0] + c0), p1 = ex2(s[q][1] + c0);
-      l = fmaf(p0, j0 + q * 8 + 2 * i4 < n ? pow2_of(254u - (ep[q] >> 8 & 0xffu)) : 0.f, l);
-      l = fmaf(p1, j0 + q * 8 + 2 * i4 + 1 < n ? pow2_of(254u - (ep[q] >> 24)) : 0.f, l);
+    for (int x = 0; x < 2; x++) {
+      const float p0 = ex2(s[2 * x] + c0), p1 = ex2(s[2 * x + 1] + c0);
+      l = fmaf(p0, nev[2 * x], fmaf(p1, nev[2 * x + 1], l));
       const uint32_t hi = pack_f16(p0, p1);
       const f32x2 hf = f32x2_of(hi);
-      const uint32_t lo = pack_f16(p0 - lo2(hf), p1 - hi2(hf));
-      pb[q] = g & 1 ? lo : hi;
+      const uint32_t lo = pack_f16(p0 - lo2(hf), p1 - hi2(hf)), w0 = __byte_perm(hi, lo, 0x5410), w1 = __byte_perm(hi, lo, 0x7632);
+      pb[2 * x] = __byte_perm(__shfl_sync(0xffffffffu, w0, i4 * 8), __shfl_sync(0xffffffffu, w0, i4 * 8 + 4), term);
+      pb[2 * x + 1] = __byte_perm(__shfl_sync(0xffffffffu, w1, i4 * 8), __shfl_sync(0xffffffffu, w1, i4 * 8 + 4), term);
     }
 #pragma unroll
     for (int q = 0; q < 2; q++)
@@ -369,14 +377,12 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
           mma_f16(o[2 * w + 1], x2, x3, y2, y3, pb[2 * q], pb[2 * q + 1]);
         }
       }
-    fetch_v(off_n);
-    off = off_n;
+    fetch_v();
     e = e_n;
-    place();
-    look(j0 + 3 * step);
+    place(n1);
   }
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+  for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
 #pragma unroll
   for (int t = 0; t < NM; t++) {
     out[2 * t] = o[t][0] + o[t][1];
@@ -387,7 +393,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
 }  // namespace
 
 template <int HD, int W>
-__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W)
+__global__ void __launch_bounds__(W == 8 ? 256 : 128, W == 8 ? 2 : HD == 128 ? 3 : 4)
 paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, int ntok, float scale, int max_ctx, int append, int S) {
   constexpr int IPC = W == 1 ? 4 : 1, PER = HD / 8;
   __shared__ float s_part[W > 1 ? W * (HD + 2) : 1], s_cta[HD + 2];       // per warp, per CTA: HD sums, reference, normaliser
@@ -449,29 +455,20 @@ paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restr
     if (S == 1) return;
     __syncwarp();
     cluster_sync_all();
-    if (valid && tid < HD / S) {                                   // rank r joins and writes columns [r HD / S, (r + 1) HD / S)
+    if (valid && tid < HD / S) {                                  // rank r joins and writes columns [r HD / S, (r + 1) HD / S)
       const int col = rank * (HD / S) + tid;
       const uint32_t base = smem_u32(s_cta);
-      float mx = -INFINITY, num = 0.f, den = 0.f, pm[8], pl[8], po[8];
-#pragma unroll
-      for (int r = 0; r < 8; r++)
-        if (r < S) {
-          const uint32_t a = mapa_shared(base, r);
-          pm[r] = ld_cluster_f32(a + HD * 4);
-          pl[r] = ld_cluster_f32(a + (HD + 1) * 4);
-          po[r] = ld_cluster_f32(a + col * 4);
-        }
-#pragma unroll
-      for (int r = 0; r < 8; r++)
-        if (r < S) mx = fmaxf(mx, pm[r]);
+      float mx = -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll 4
+      for (int r = 0; r < S; r++) mx = fmaxf(mx, ld_cluster_f32(mapa_shared(base, r) + HD * 4));
       const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-      for (int r = 0; r < 8; r++)
-        if (r < S) {
-          const float f = ex2(pm[r] - ref);
-          den += f * pl[r];
-          num += f * po[r];
-        }
+#pragma unroll 4
+      for (int r = 0; r < S; r++) {
+        const uint32_t a = mapa_shared(base, r);
+        const float f = ex2(ld_cluster_f32(a + HD * 4) - ref);
+        den += f * ld_cluster_f32(a + (HD + 1) * 4);
+        num += f * ld_cluster_f32(a + col * 4);
+      }
       dst[col] = __float2bfloat16(num / den);
     }
     __syncwarp();
@@ -488,12 +485,19 @@ static int launch_attn8(const Cache& c, const void* qkv, int ld, void* out, int 
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
+  if (S > 8) {
+    static bool opted = false;                     // clusters of more than eight
+    if (!opted && cudaFuncSetAttribute(paged_attn8_k<HD, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      cudaGetLastError();
+      S = 8;
+    } else opted = true;
+  }
   if (S > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = S; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1;
   }
   cfg.gridDim = W == 1 ? dim3((ntok + 3) / 4, c.H) : dim3((unsigned)ntok * S, c.H);
-  cfg.blockDim = dim3(W == 1 ? 128 : 32 * W); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = n;
+  cfg.blockDim = dim3(W == 8 ? 256 : 128); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn8_k<HD, W>, c, (const bf16*)qkv, ld, (bf16*)out, ldo, ntok, scale, max_ctx, append, S);
   if (e != cudaSuccess) { cudaGetLastError(); kh_set_error("paged_attn8: %s", cudaGetErrorString(e)); return -1; }
   return 0;
@@ -507,22 +511,25 @@ extern "C" int kh_paged_attn8(const void* qkv, int ld, void* kv, int n_blocks, i
   if (ntok > (1 << 27)) { kh_set_error("paged_attn8: %d tokens are too many", ntok); return -1; }
   const float sl2 = scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
-  // warps to an item: one where the items alone give every SM some twelve, else four; eight and a cluster of up to eight CTAs where four to an
-  // item would still leave the SMs with few bytes in flight, as far as the longest context has a chunk of 32 positions for each
-  const long items = (long)ntok * H, want = 148 * 12;
+  // One warp to an item where the items fill the SMs and no context is long, else four.  Where these leave SMs idle: eight (heads of up to 64; wider ones
+  // have no registers for two such CTAs per SM), then a cluster of up to eight CTAs, as long as they fit the chip together (16 warps per SM) and the
+  // longest context has a chunk of 32 positions for each warp; sixteen CTAs of four warps for wide heads beyond 8192 positions.  us, warps x CTAs:
+  //   16 heads of 64, 16300 positions: 4 x 4 45.6, 4 x 8 21.2, 4 x 16 16.9, 8 x 8 15.8;  4000: 4 x 4 10.9, 8 x 4 7.5, 8 x 8 8.8;  200: 4 x 2 5.0, 8 x 1 3.8
+  //   512 heads of 64, 20 to 1000 positions: 4 x 1 12.7, 8 x 1 14.5;  72 at 960: 4 x 4 7.2, 8 x 2 5.7;  256 heads of 32 at 700: 4 x 2 7.5, 8 x 1 5.8
+  //   16 heads of 128, 16300: 4 x 8 28.5, 4 x 16 22.8;  64 at 4000: 4 x 8 27.9, 4 x 16 40.7
+  const long items = (long)ntok * H;
   const int chunks = (max_ctx + 31) / 32;
-  int W = chunks <= 1 || (items >= want && chunks <= 8) ? 1 : items * 4 >= want || chunks <= 4 ? 4 : 8, S = 1;
-  while (W > 1 && S < 8 && items * W * S < want && chunks >= 2 * W * S) S *= 2;
-  if (const char* f = getenv("KH_W")) { W = atoi(f); S = atoi(getenv("KH_SS")); }
-#define LAUNCH(HD)                                                                                                      \
-  return W == 1 ? launch_attn8<HD, 1>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, 1, st)                          \
-       : W == 4 ? launch_attn8<HD, 4>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, S, st)                          \
-                : launch_attn8<HD, 8>(c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append, S, st);
+  int W = chunks <= 1 || (items >= 148 * 12 && chunks <= 8) ? 1 : 4, S = 1;
+  if (W == 4 && hd <= 64 && items * 8 <= 148 * 16 && chunks >= 8) W = 8;
+  while (W > 1 && S < (W == 4 ? 16 : 8) && items * W * S * 2 <= 148 * 16 && chunks >= (S == 8 ? 256 : 2 * W * S)) S *= 2;
+#define ARGS c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append
+#define LAUNCH(HD) return W == 1 ? launch_attn8<HD, 1>(ARGS, 1, st) : W == 4 ? launch_attn8<HD, 4>(ARGS, S, st) : launch_attn8<HD, HD == 128 ? 4 : 8>(ARGS, S, st);
   if (hd == 128) { LAUNCH(128) }
   if (hd == 64) { LAUNCH(64) }
   if (hd == 32) { LAUNCH(32) }
   LAUNCH(16)
 #undef LAUNCH
+#undef ARGS
 }
 
 // ------------------------------------------------------------------------------- block copies
