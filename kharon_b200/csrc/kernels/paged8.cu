@@ -549,15 +549,19 @@ extern "C" int kh_paged_attn8(const void* qkv, int ld, void* kv, int n_blocks, i
   if (ntok > (1 << 27)) { kh_set_error("paged_attn8: %d tokens are too many", ntok); return -1; }
   const float sl2 = scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
-  // One warp to an item where the items fill the SMs and no context is long, else four.  Where these leave SMs idle: eight (heads of up to 64; wider ones
-  // have no registers for two such CTAs per SM), then a cluster of up to eight CTAs, as long as they fit the chip together (16 warps per SM) and the
-  // longest context has a chunk of 32 positions for each warp; sixteen CTAs of four warps for wide heads beyond 8192 positions.  us, warps x CTAs:
+  // One warp to an item or four: by rounds of the warps that the SMs hold (some 3 us each) and chunks of 32 positions per warp (some 1 us each) of the longest
+  // context.  us, one / four: 704 heads of 128 at 40 positions 7.0 / 9.9, 2400 of 64 at 60 9.2 / 16.1, at 200 24.8 / 28.8, 512 of 64 at 20 to 1000 34 / 13.
+  // Where four leave SMs idle: eight (heads of up to 64; wider ones have no registers for two such CTAs per SM), then a cluster of up to eight CTAs, as
+  // long as they fit the chip together (16 warps per SM) and the longest context has a chunk for each warp; sixteen CTAs of four warps for wide heads
+  // beyond 8192 positions.  us, warps x CTAs:
   //   16 heads of 64, 16300 positions: 4 x 4 45.6, 4 x 8 21.2, 4 x 16 16.9, 8 x 8 15.8;  4000: 4 x 4 10.9, 8 x 4 7.5, 8 x 8 8.8;  200: 4 x 2 5.0, 8 x 1 3.8
   //   512 heads of 64, 20 to 1000 positions: 4 x 1 12.7, 8 x 1 14.5;  72 at 960: 4 x 4 7.2, 8 x 2 5.7;  256 heads of 32 at 700: 4 x 2 7.5, 8 x 1 5.8
   //   16 heads of 128, 16300: 4 x 8 28.5, 4 x 16 22.8;  64 at 4000: 4 x 8 27.9, 4 x 16 40.7
   const long items = (long)ntok * H;
   const int chunks = (max_ctx + 31) / 32;
-  int W = chunks <= 1 || (items >= 148 * 12 && chunks <= 8) ? 1 : 4, S = 1;
+  const long held = 148 * (hd == 128 ? 12 : 16);
+  auto cost = [&](int w) { return 3 * ((items * w + held - 1) / held) + (chunks + w - 1) / w; };
+  int W = cost(1) <= cost(4) ? 1 : 4, S = 1;
   if (W == 4 && hd <= 64 && items * 8 <= 148 * 16 && chunks >= 8) W = 8;
   while (W > 1 && S < (W == 4 ? 16 : 8) && items * W * S * 2 <= 148 * 16 && chunks >= (S == 8 ? 256 : 2 * W * S)) S *= 2;
 #define ARGS c, qkv, ld, out, ldo, ntok, sl2, max_ctx, append

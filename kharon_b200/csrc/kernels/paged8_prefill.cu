@@ -1,13 +1,21 @@
 // Attention of runs of new tokens over the 8-bit paged cache (paged8.cu).
 #include "paged8.cuh"
-#include <stdlib.h>
 
-// ------------------------------------------------------------------------------- attention of pieces of prompts
-// CTA = (up to 64 consecutive tokens of a sequence, head), a warp per 16 tokens, mma.sync on K and V tiles of 64 positions that are
-// turned into bf16 (exact) on their way into shared memory; fp32 probabilities, which enter P V as three bf16 terms.
+// ------------------------------------------------------------------------------- short runs
+// CTA = (a run of up to 64 tokens, head), a warp per 16 tokens, mma.sync on K and V tiles of 64 positions that are turned into bf16 (exact) on
+// their way into shared memory; fp32 probabilities, which enter P V as three bf16 terms.  The key tiles are shared by the S CTAs of a cluster, in
+// contiguous ranges, where the runs leave SMs idle.  Bound by the trips to memory of a tile (some 1 us each): few instructions, small tiles and several
+// CTAs per SM, where the tcgen05 kernel below has 4 us more to set up (16 heads of 64, us, this / that: a fresh run of 16 3.1 / 7.1, of 64 3.6 / 7.7, thirty
+// of 64 8.2 / 30; thirty of 64 behind 200 positions 25 / 48).
 namespace {
-constexpr int P8_ROWS = 64, P8_MAX_TILES = 1024;
-struct Pieces { int row0[P8_MAX_TILES]; uint8_t n[P8_MAX_TILES]; };
+constexpr int P8_ROWS = 64, P8_MAX = 1024;
+struct Pieces { int row0[P8_MAX]; uint8_t n[P8_MAX]; };
+template <int N>
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[N]) {
+  if constexpr (N == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
+  else if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+  else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory");
+}
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -35,20 +43,22 @@ __device__ __forceinline__ void decode16(const uint4& u, float s, uint4& a, uint
 
 template <int HD>
 __global__ void __launch_bounds__(128)
-paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float scale, int max_ctx) {
+paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float scale, int max_ctx, int S) {
   constexpr int PITCH = HD * 2 + 16, TILE = P8_ROWS * PITCH, PC = HD / 16, NL = P8_ROWS * PC / 128;     // bytes per row, per tile; 16-code pieces per row, per thread
+  constexpr int OP = HD + 4, ML = P8_ROWS * OP * 4;                             // joining: floats per row of O; where (maximum, normaliser) and the rows to do anew lie
   extern __shared__ __align__(16) uint8_t smem[];                               // [K, V][64 rows]
   pdl_wait();
   pdl_launch_dependents();
+  const int rank = (int)(blockIdx.x % S), piece = (int)(blockIdx.x / S);
   const uint32_t sK = smem_u32(smem), sV = sK + TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3, h = blockIdx.y;
-  const int r0 = tiles.row0[blockIdx.x], p0 = c.pos[r0], sl = c.slot[r0];
-  int n = tiles.n[blockIdx.x];
+  const int r0 = tiles.row0[piece], p0 = c.pos[r0], sl = c.slot[r0];
+  int n = tiles.n[piece];
   // index guard: tokens beyond the limits are recorded (status code 8) and skipped; they are the last of the run
   const int ok = sl < 0 || sl >= c.n_slots || p0 < 0 ? 0 : (int)min((long)n, min((long)max_ctx, (long)c.max_lb * c.bs) - p0);
   bool bad = ok < n;
-  if (bad && tid == 0) report(c.err);
-  if (ok <= 0) return;
+  if (bad && tid == 0 && rank == 0) report(c.err);
+  if (ok <= 0) return;                                                          // (the whole cluster)
   n = ok;
   bad = false;
   const int ctx = p0 + n, bs = c.bs;
@@ -88,7 +98,8 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ C
       *reinterpret_cast<uint4*>(at + TILE + 16) = b;
     }
   };
-  fetch(0);
+  const int n_kt = (ctx + P8_ROWS - 1) / P8_ROWS, kt0 = (int)((long)n_kt * rank / S), kt1 = (int)((long)n_kt * (rank + 1) / S);
+  if (kt0 < kt1) fetch(kt0);
   const int w0 = warp * 16;                                                     // this warp's first token of the run
   uint4 q[HD / 32][2];                                                          // rows g and g + 8, piece c4 of every 32-wide block
 #pragma unroll
@@ -103,13 +114,12 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ C
   for (int t = 0; t < HD / 8; t++)
 #pragma unroll
     for (int i = 0; i < 4; i++) o[t][i] = 0.f;
-  const int n_kt = (ctx + P8_ROWS - 1) / P8_ROWS;
 #pragma unroll 1
-  for (int kt = 0; kt < n_kt; kt++) {
+  for (int kt = kt0; kt < kt1; kt++) {
     __syncthreads();                                                            // the tile before has been read
     store();
     __syncthreads();
-    if (kt + 1 < n_kt) fetch(kt + 1);
+    if (kt + 1 < kt1) fetch(kt + 1);
     const int k0 = kt * P8_ROWS;
     if (w0 < n && k0 <= p0 + w0 + 15) {                                         // uniform over the warp
       float s[8][4];
@@ -177,31 +187,86 @@ paged_prefill8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ C
     }
   }
   if (bad) report(c.err);
-  // A NaN in V reaches the rows that see its position and no others.  The products above multiply it with the zeros of masked
-  // positions too, which leaves a NaN in every row of the warp: such a warp does its rows anew.
-  uint32_t top = 0;
-#pragma unroll
-  for (int t = 0; t < HD / 8; t++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(o[t][i]) & 0x7fffffffu);
-  if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {
-#pragma unroll 1
-    for (int r = w0; r < min(n, w0 + 16); r++)
-      attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (w0 + g + 8 * i < n) {
-      const float inv = 1.f / l[i];
-      bf16* dst = out + (size_t)(r0 + w0 + g + 8 * i) * ldo + h * HD + c4 * 2;
-#pragma unroll
-      for (int t = 0; t < HD / 8; t++) *reinterpret_cast<uint32_t*>(dst + t * 8) = pack_bf16(o[t][2 * i] * inv, o[t][2 * i + 1] * inv);
-    }
   }
+  // A NaN in V reaches the rows that see its position and no others.  The products above multiply it with the zeros of masked positions
+  // too, which leaves a NaN in every row of the warp: such rows are done anew.
+  if (S == 1) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int t = 0; t < HD / 8; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(o[t][i]) & 0x7fffffffu);
+    if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {
+#pragma unroll 1
+      for (int r = w0; r < min(n, w0 + 16); r++)
+        attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      if (w0 + g + 8 * i < n) {
+        const float inv = 1.f / l[i];
+        bf16* dst = out + (size_t)(r0 + w0 + g + 8 * i) * ldo + h * HD + c4 * 2;
+#pragma unroll
+        for (int t = 0; t < HD / 8; t++) *reinterpret_cast<uint32_t*>(dst + t * 8) = pack_bf16(o[t][2 * i] * inv, o[t][2 * i + 1] * inv);
+      }
+    return;
+  }
+  __syncthreads();                                                              // no tile is read any more
+  uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + ML + P8_ROWS * 8);
+  if (tid < 2) s_again[tid] = 0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int row = w0 + g + 8 * i;
+    float* part = reinterpret_cast<float*>(smem) + row * OP + c4 * 2;
+#pragma unroll
+    for (int t = 0; t < HD / 8; t++) *reinterpret_cast<float2*>(part + t * 8) = make_float2(o[t][2 * i], o[t][2 * i + 1]);
+    if (c4 == 0) *reinterpret_cast<float2*>(smem + ML + row * 8) = make_float2(m[i], l[i]);
+  }
+  __syncwarp();
+  cluster_sync_all();
+  constexpr int TPR = HD / 4;                                                   // CTA `rank` joins rows rank, rank + S ...; a thread four columns of a row
+  const int ch = tid % TPR;
+#pragma unroll 1
+  for (int r = rank + tid / TPR * S; r < n; r += 128 / TPR * S) {
+    float mx = -INFINITY, den = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < S; i++) {
+      float v[2];
+      ld_cluster(mapa_shared(sK, i) + ML + r * 8, v);
+      mx = fmaxf(mx, v[0]);
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll 4
+    for (int i = 0; i < S; i++) {
+      const uint32_t a = mapa_shared(sK, i);
+      float v[2], x[4];
+      ld_cluster(a + ML + r * 8, v);
+      ld_cluster(a + (r * OP + ch * 4) * 4, x);
+      const float f = ex2(v[0] - ref);
+      den = fmaf(f, v[1], den);
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = fmaf(f, x[e], y[e]);
+    }
+    const float inv = 1.f / den;
+    bool anew = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) anew |= (__float_as_uint(y[e]) & 0x7fffffffu) >= 0x7f800000u;
+    if (anew) atomicOr(s_again + (r >> 5), 1u << (r & 31));
+    else *reinterpret_cast<uint2*>(out + (size_t)(r0 + r) * ldo + h * HD + ch * 4) = make_uint2(pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv));
+  }
+  __syncwarp();
+  cluster_sync_all();                                                           // the others' parts are read until here
+#pragma unroll 1
+  for (int r = warp; r < n; r += 4)
+    if (s_again[r >> 5] >> (r & 31) & 1)
+      attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
 }
+
 // ------------------------------------------------------------------------------- runs of new tokens on tcgen05
 // A work item is (up to 256 consecutive tokens of a run, head).  Warps 0-3 and 4-7 are two groups of one thread per query row; warps 8-11 fetch the
 // codes of K, 128 positions at a time, through the block table and turn them into f16 tiles in the swizzled layout that the tensor core reads,
@@ -246,12 +311,6 @@ __device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int row, int ch) {
 }
 __device__ __forceinline__ void st_shared_16(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[N]) {
-  if constexpr (N == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
-  else if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
-  else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory");
 }
 template <int ID, int N>
 __device__ __forceinline__ void named_barrier() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
@@ -440,7 +499,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     // A thread looks up one position of a tile (t of 128): block two tiles ahead, exponent one tile ahead, and passes address and exponent on.
     // No loaded value is looked at before the next turn.
     int blk = 0, blk_at = -1;
-    uint32_t e_next = 0;
+    uint32_t e_next = 0, e_now = 0;
     uint64_t a_next = 0;
     auto look = [&](int j) {                               // block of position 128 j + t
       const int p = j * 128 + t;
@@ -462,10 +521,8 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       }
     };
     uint4 x[NP];
-    auto publish = [&](int b, int it) {                    // tile -> buffer b; then its codes are on their way
+    auto publish = [&](int b) {                            // tile -> buffer b; then its codes are on their way
       s_addr[b * 128 + t] = a_next;
-      const uint32_t mk = __reduce_max_sync(0xffffffffu, e_next & 0xffu), mv = __reduce_max_sync(0xffffffffu, e_next >> 8);
-      if (lane == 0) s_wmax[b * 4 + (warp & 3)] = mk | mv << 16;
       pair_barrier(4 + vr);
 #pragma unroll
       for (int i = 0; i < NP / SLABS; i++) {
@@ -473,26 +530,32 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
 #pragma unroll
         for (int q = 0; q < SLABS; q++) x[i * SLABS + q] = a ? *reinterpret_cast<const uint4*>(a + q * 64 + l * 16) : make_uint4(0, 0, 0, 0);
       }
-      // the position's factor 2^(e - E + 7), E the tile's largest exponent
+      e_now = e_next;
+    };
+    auto factors = [&](int b, int it) {                    // 2^(e - E + 7) of its positions, E the tile's largest exponent
+      const uint32_t mk = __reduce_max_sync(0xffffffffu, e_now & 0xffu), mv = __reduce_max_sync(0xffffffffu, e_now >> 8);
+      if (lane == 0) s_wmax[b * 4 + (warp & 3)] = mk | mv << 16;
+      pair_barrier(4 + vr);
       const uint32_t tops = __vmaxu2(__vmaxu2(s_wmax[b * 4], s_wmax[b * 4 + 1]), __vmaxu2(s_wmax[b * 4 + 2], s_wmax[b * 4 + 3]));
-      const int e = (int)(e_next >> 8 * vr & 0xffu), off = e - (int)(tops >> 16 * vr & 0xffffu);
+      const int e = (int)(e_now >> 8 * vr & 0xffu), off = e - (int)(tops >> 16 * vr & 0xffffu);
       if (vr && e > E_LO && off < -22) *redo = 1;
       s_fac[b * 128 + t] = f16_pow2(off + 7) * 0x10001u;
       // K's warps tell the groups both exponents: scores that are there have passed bar_kfull.  (Of four slots this one was last read for the tile
       // four before, whose scores both groups have used: K's stage of the tile two before this one has been freed.)
       if (t == 0 && !vr) s_tmax[it & 3] = tops;
+      pair_barrier(4 + vr);
     };
     if (live && kt0 < kt1) {
       look(kt0);
       exponent();
       look(kt0 + 1);
-      publish(0, 0);
+      publish(0);
       exponent();
       look(kt0 + 2);
       for (int j = kt0; j < kt1; j++) {
         const int it = j - kt0, s = it % NS, b = it & 1;
         wait(free + 8 * s, ((it / NS) & 1) ^ 1);
-        pair_barrier(4 + vr);                              // the factors are there
+        factors(b, it);
         // chunks 2 l and 2 l + 1 of rows r1, r1 + RPP ...: RPP is a multiple of 8, the swizzle is the same for all of them
         const uint32_t dst0 = sKV + s * 2 * C::TILE + vr * C::TILE + off0, dst1 = dst0 ^ 16u;
 #pragma unroll
@@ -514,7 +577,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         __syncwarp();
         if (lane == 0) mbar_arrive(full + 8 * s);
         if (j + 1 < kt1) {
-          publish(b ^ 1, it + 1);
+          publish(b ^ 1);
           exponent();
           look(j + 3);
         }
@@ -531,20 +594,28 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     const float* s_qe = reinterpret_cast<const float*>(smem + C::QE);
     const uint32_t* s_tmax = reinterpret_cast<const uint32_t*>(smem + C::TMAX);
     {
-      constexpr int LQ = HD / 8;                 // lanes per row of q
+      constexpr int LQ = HD / 8, NQ = LQ / 2;    // lanes per row of q; loads of a thread for 128 rows, all on their way together
 #pragma unroll 1
-      for (int i = tid; i < nq * 128 * LQ; i += 256) {
-        const int r = i / LQ, ch = i % LQ;
-        const uint4 u = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + ch * 8) : make_uint4(0, 0, 0, 0);
-        uint32_t m = amax8(u);
+      for (int x = 0; x < nq; x++) {
+        uint4 u[NQ];
 #pragma unroll
-        for (int x = LQ / 2; x > 0; x >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, x));
-        const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
-        const float f = pow2_of((uint32_t)(127 - eq));
-        const f32x2 f2 = mk2(f, f);
-        st_shared_16(tile_chunk(sQ + (r >> 7) * C::TILE, r & 127, ch),
-                     make_uint4(pack_f16(mul2(un2(u.x), f2)), pack_f16(mul2(un2(u.y), f2)), pack_f16(mul2(un2(u.z), f2)), pack_f16(mul2(un2(u.w), f2))));
-        if (ch == 0) reinterpret_cast<float*>(smem + C::QE)[r] = pow2_of((uint32_t)(127 + eq));
+        for (int i = 0; i < NQ; i++) {
+          const int r = x * 128 + (tid + i * 256) / LQ;
+          u[i] = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + tid % LQ * 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+          const int r = (tid + i * 256) / LQ, ch = tid % LQ;
+          uint32_t m = amax8(u[i]);
+#pragma unroll
+          for (int y = LQ / 2; y > 0; y >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
+          const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
+          const float f = pow2_of((uint32_t)(127 - eq));
+          const f32x2 f2 = mk2(f, f);
+          st_shared_16(tile_chunk(sQ + x * C::TILE, r, ch),
+                       make_uint4(pack_f16(mul2(un2(u[i].x), f2)), pack_f16(mul2(un2(u[i].y), f2)), pack_f16(mul2(un2(u[i].z), f2)), pack_f16(mul2(un2(u[i].w), f2))));
+          if (ch == 0) reinterpret_cast<float*>(smem + C::QE)[x * 128 + r] = pow2_of((uint32_t)(127 + eq));
+        }
       }
     }
     fence_proxy_async_smem();
@@ -628,31 +699,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     const float den = l * pow2_of(261u - eb);    // l 2^(7 - EB)
     // A NaN in V reaches the rows that see its position and no others.  P V multiplies it with the zeros of masked positions too, which leaves a
     // NaN in every row of the tile: such rows are done anew, one by one.
-    if (S == 1 && nq == 2) {
-      named_barrier<1, 256>();                   // (`redo` is written by then: all tiles have been used)
-      const bool intact = *abort_flag == 0 && lrow < n, all = *redo != 0;
-      const float inv = 1.f / den;
-      bf16* dst = out + (size_t)(r0 + lrow) * ldo + h * HD;
-      uint32_t top = __float_as_uint(inv) & 0x7fffffffu;
-      if (!(den > 0.f)) top = 0x7f800000u;
-#pragma unroll 1
-      for (int q = 0; q < HD; q += 32) {
-        uint32_t r[32], o[16];
-        tmem_ld32(tO + q, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; i++) top = max(top, r[i] & 0x7fffffffu);
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[i] = pack_bf16(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
-        if (intact)
-#pragma unroll
-          for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(dst + q + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-      }
-      const uint32_t again = __ballot_sync(0xffffffffu, intact && (all || top >= 0x7f800000u));
-      if (lane == 0) s_again[warp] = again;
-    } else {
-      named_barrier<1, 256>();                   // no tile is read any more
+    auto leave = [&]() {                         // (R, normaliser, O) of the group's rows in shared memory, over the tiles
       float* part = reinterpret_cast<float*>(smem) + (w * 128 + row) * C::PITCH;
+      *reinterpret_cast<float2*>(smem + C::ML + (w * 128 + row) * 8) = make_float2(R, den);
+      if (lrow - lane >= n) return;              // (a warp without rows)
 #pragma unroll 1
       for (int q = 0; q < HD; q += 32) {
         uint32_t r[32];
@@ -665,71 +715,104 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         for (int i = 0; i < 32; i += 4)
           *reinterpret_cast<uint4*>(part + q + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
-      *reinterpret_cast<float2*>(smem + C::ML + (w * 128 + row) * 8) = make_float2(R, den);
+    };
+    named_barrier<1, 256>();                     // no tile is read any more, and `redo` is written
+    if (S > 1) leave();
+    else {
+      float own = 1.f, other = 0.f, sum = den;   // weights of the group's sums and of the second group's for the same rows
+      if (nq == 1) {
+        if (w == 1) leave();
+        named_barrier<1, 256>();
+        if (w == 0) {
+          const float2 v = *reinterpret_cast<const float2*>(smem + C::ML + (128 + row) * 8);
+          const float mx = fmaxf(R, v.x), ref = mx == -INFINITY ? 0.f : mx;
+          own = ex2(R - ref);
+          other = ex2(v.x - ref);
+          sum = fmaf(own, den, other * v.y);
+        }
+      }
+      if (nq == 2 || w == 0) {
+        const bool intact = *abort_flag == 0 && lrow < n, all = *redo != 0;
+        const float inv = 1.f / sum;
+        const float* part = reinterpret_cast<const float*>(smem) + (128 + row) * C::PITCH;
+        bf16* dst = out + (size_t)(r0 + lrow) * ldo + h * HD;
+        uint32_t top = sum > 0.f ? __float_as_uint(inv) & 0x7fffffffu : 0x7f800000u;
+        if (lrow - lane < n)
+#pragma unroll 1
+          for (int q = 0; q < HD; q += 32) {
+            uint32_t r[32], o[16];
+            tmem_ld32(tO + q, r);
+            tmem_ld_wait();
+            if (nq == 1)
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(part + q + i);
+                r[i] = __float_as_uint(fmaf(other, v.x, own * __uint_as_float(r[i])));
+                r[i + 1] = __float_as_uint(fmaf(other, v.y, own * __uint_as_float(r[i + 1])));
+                r[i + 2] = __float_as_uint(fmaf(other, v.z, own * __uint_as_float(r[i + 2])));
+                r[i + 3] = __float_as_uint(fmaf(other, v.w, own * __uint_as_float(r[i + 3])));
+              }
+#pragma unroll
+            for (int i = 0; i < 32; i++) top = max(top, r[i] & 0x7fffffffu);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = pack_bf16(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
+            if (intact)
+#pragma unroll
+              for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(dst + q + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        const uint32_t again = __ballot_sync(0xffffffffu, intact && (all || top >= 0x7f800000u));
+        if (lane == 0) s_again[warp] = again;
+      }
     }
     }
-  // ------------------------------------------------------------------ groups and CTAs that share rows join
+  // ------------------------------------------------------------------ the cluster's CTAs join
   if (S > 1) { __syncwarp(); cluster_sync_all(); }
-  if (live && (S > 1 || nq == 1)) {
-    if (S == 1) named_barrier<1, 256>();
+  if (live && S > 1) {
     const int parts = nq == 2 ? S : 2 * S;       // of a row: part i is group i % 2 (or the row's own) of CTA i / 2 (or i)
     bool all = false;
     for (int i = 0; i < S; i++) {
       float v[1];
-      ld_cluster(S > 1 ? mapa_shared(smem_u32((const void*)redo), i) : smem_u32((const void*)redo), v);
+      ld_cluster(mapa_shared(smem_u32((const void*)redo), i), v);
       all |= __float_as_uint(v[0]) != 0;
     }
+    // CTA `rank` joins rows rank, rank + S ...; a thread four columns of a row
+    constexpr int TPR = HD / 4;
+    const int ch = tid % TPR;
 #pragma unroll 1
-    for (int r = rank * 8 + warp; r < n; r += 8 * S) {
-      const int row = r & 127;
-      auto where = [&](int i) {                  // (CTA, group row) of part i
-        const uint32_t off = nq == 2 ? (uint32_t)(r >> 7) * 128 + row : (uint32_t)(i & 1) * 128 + row;
-        return make_uint2(S > 1 ? mapa_shared(base, nq == 2 ? i : i >> 1) : base, off);
-      };
-      float pm = -INFINITY, pl = 0.f;
-      if (lane < parts) {
-        const uint2 at = where(lane);
-        float v[2];
-        ld_cluster(at.x + C::ML + at.y * 8, v);
-        pm = v[0];
-        pl = v[1];
-      }
-      float mx = pm;
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      const float f = ex2(pm - ref);
-      float den = f * pl;
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
-      constexpr int E = HD / 32;
-      float o[E];
-#pragma unroll
-      for (int e = 0; e < E; e++) o[e] = 0.f;
+    for (int r = rank + tid / TPR * S; r < n; r += 256 / TPR * S) {
+      const int own = nq == 2 ? r : 0, row = r & 127;          // (nq = 2: the group's rows are r itself)
+      auto where = [&](int i) { return mapa_shared(base, nq == 2 ? i : i >> 1); };
+      auto line = [&](int i) { return nq == 2 ? own : (i & 1) * 128 + row; };
+      float mx = -INFINITY, den = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
       for (int i = 0; i < parts; i++) {
-        const uint2 at = where(i);
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        float v[E];
-        ld_cluster(at.x + (at.y * C::PITCH + lane * E) * 4, v);
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(fi, v[e], o[e]);
+        float v[2];
+        ld_cluster(where(i) + C::ML + line(i) * 8, v);
+        mx = fmaxf(mx, v[0]);
       }
-      den = __shfl_sync(0xffffffffu, den, 0);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll 4
+      for (int i = 0; i < parts; i++) {
+        const uint32_t a = where(i);
+        float v[2], y[4];
+        ld_cluster(a + C::ML + line(i) * 8, v);
+        ld_cluster(a + (line(i) * C::PITCH + ch * 4) * 4, y);
+        const float f = ex2(v[0] - ref);
+        den = fmaf(f, v[1], den);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
+      }
       const float inv = 1.f / den;
       bool anew = all || !(den > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
 #pragma unroll
-      for (int e = 0; e < E; e++) anew |= (__float_as_uint(o[e]) & 0x7fffffffu) >= 0x7f800000u;
+      for (int e = 0; e < 4; e++) anew |= (__float_as_uint(o[e]) & 0x7fffffffu) >= 0x7f800000u;
       if (*abort_flag) break;
-      bf16* dst = out + (size_t)(r0 + r) * ldo + h * HD;
-      if (__any_sync(0xffffffffu, anew)) { if (lane == 0) atomicOr(s_again + (r >> 5), 1u << (r & 31)); }
-      else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-      else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_bf16(o[0] * inv, o[1] * inv);
-      else dst[lane] = __float2bfloat16(o[0] * inv);
+      if (anew) atomicOr(s_again + (r >> 5), 1u << (r & 31));
+      else *reinterpret_cast<uint2*>(out + (size_t)(r0 + r) * ldo + h * HD + ch * 4) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
     }
   }
   if (S > 1) { __syncwarp(); cluster_sync_all(); }          // the others' parts are read until here
-  if (live) {
+  if (live) {                                    // (after the join: a row's other columns may have been stored)
     named_barrier<1, 256>();
 #pragma unroll 1
     for (int r = warp; r < n; r += 8)
@@ -742,10 +825,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-template <int HD>
-static int launch_chunks(const Runs& runs, int n_runs, const Cache& c, const bf16* qkv, int ld, bf16* out, int ldo, float sl2, int max_ctx, int S, cudaStream_t st) {
-  using C = Chunk<HD>;
-  if (cudaFuncSetAttribute(paged_chunk8_k<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+// Launch in clusters of S CTAs along x.
+template <typename... P, typename... A>
+static int launch_clusters(void (*kernel)(P...), dim3 grid, int threads, int smem, int S, cudaStream_t st, A... args) {
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     kh_set_error("paged_prefill8: shared memory opt-in failed");
     return -1;
@@ -761,10 +844,79 @@ static int launch_chunks(const Runs& runs, int n_runs, const Cache& c, const bf1
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = S; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1;
   }
-  cfg.gridDim = dim3((unsigned)n_runs * c.H * S); cfg.blockDim = dim3(CH_THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_chunk8_k<HD>, runs, c, qkv, ld, out, ldo, sl2, max_ctx, S);
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
   if (e != cudaSuccess) { cudaGetLastError(); kh_set_error("paged_prefill8: %s", cudaGetErrorString(e)); return -1; }
   return 0;
+}
+// Clusters of S = 2, 4, 8 CTAs of the tcgen05 kernel (one per SM) that the chip holds at once: a cluster lies in one group of SMs.
+template <int HD>
+static int chunk_clusters(int S) {
+  static int known[4] = {0, 0, 0, 0};
+  int& n = known[S == 2 ? 1 : S == 4 ? 2 : 3];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = S; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(S * 148); cfg.blockDim = dim3(CH_THREADS); cfg.dynamicSmemBytes = Chunk<HD>::SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaFuncSetAttribute(paged_chunk8_k<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<HD>::SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&got, paged_chunk8_k<HD>, &cfg) != cudaSuccess || got < 1) {
+      cudaGetLastError();
+      got = -1;                                      // not available
+    }
+    n = got;
+  }
+  return n;
+}
+template <int HD>
+static int launch_runs(const Cache& c, const bf16* qkv, int ld, bf16* out, int ldo, float sl2, int max_ctx, const int* row0, const int* len, int n_runs, cudaStream_t st) {
+  // Runs of up to 64 tokens take the kernel of short runs, unless they are few and may lie behind long contexts, whose tiles of 64 positions are too many
+  // trips for it (16 heads of 64, one run of 32 behind 2000 positions, us: 46 / 13 in clusters of four; eight runs 52 / 39; at 500 14 / 10).
+  int n_short = 0, most = 0;
+  for (int i = 0; i < n_runs; i++) {
+    if (row0[i] < 0 || len[i] < 1) { kh_set_error("paged_prefill8: run %d is empty", i); return -1; }
+    n_short += len[i] <= P8_ROWS;
+    most = len[i] > most ? len[i] : most;
+  }
+  const bool split_short = max_ctx <= 1024 || (long)n_short * c.H > 2 * 148;
+  int nt = 0;
+  if (split_short && n_short) {
+    Pieces tiles;
+    auto flush = [&]() -> int {
+      const int n = nt;
+      nt = 0;
+      int S = 1;                                     // two CTAs per SM, two tiles of the longest context for each
+      while (S < 8 && (long)n * c.H * S * 2 <= 2 * 148 && (max_ctx + P8_ROWS - 1) / P8_ROWS >= 4 * S) S *= 2;
+      return n ? launch_clusters(paged_short8_k<HD>, dim3((unsigned)n * S, c.H), 128, 2 * P8_ROWS * (HD * 2 + 16) + P8_ROWS * 8 + 16, S, st, tiles, c, qkv, ld, out, ldo, sl2, max_ctx, S) : 0;
+    };
+    for (int i = 0; i < n_runs; i++)
+      if (len[i] <= P8_ROWS) {
+        tiles.row0[nt] = row0[i];
+        tiles.n[nt] = (uint8_t)len[i];
+        if (++nt == P8_MAX && flush()) return -1;
+      }
+    if (flush()) return -1;
+  }
+  Runs runs;
+  auto flush = [&]() -> int {
+    const int n = nt;
+    nt = 0;
+    // the largest cluster with which all items are on the chip at once and each CTA has two tiles of the longest context
+    int S = 8;
+    while (S > 1 && ((long)n * c.H > chunk_clusters<HD>(S) || (max_ctx + 127) / 128 < 2 * S)) S /= 2;
+    return n ? launch_clusters(paged_chunk8_k<HD>, dim3((unsigned)n * c.H * S), CH_THREADS, Chunk<HD>::SMEM, S, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, S) : 0;
+  };
+  // the pieces that see the most keys first (as far as the lengths tell)
+  for (int at = (most - 1) / CH_ROWS * CH_ROWS; at >= 0; at -= CH_ROWS)
+    for (int i = 0; i < n_runs; i++) {
+      if (len[i] <= at || (split_short && len[i] <= P8_ROWS)) continue;
+      runs.row0[nt] = row0[i] + at;
+      runs.n[nt] = (uint16_t)(len[i] - at < CH_ROWS ? len[i] - at : CH_ROWS);
+      if (++nt == CH_MAX && flush()) return -1;
+    }
+  return flush();
 }
 
 // Runs of tokens: `row0`, `len` (host arrays) give each run's first row in qkv / pos / slot / out and its length; the positions of a run
@@ -777,52 +929,9 @@ extern "C" int kh_paged_prefill8(const void* qkv, int ld, const void* kv, int n_
   if (hd == 16) { kh_set_error("paged_prefill8: head dim %d is not supported", hd); return -1; }
   if (((uintptr_t)qkv & 15) || ld % 8 || ld < 3 * H * hd || ((uintptr_t)out & 15) || ldo % 8 || ldo < H * hd) { kh_set_error("paged_prefill8: rows must be 16-byte aligned"); return -1; }
   const float sl2 = scale * 1.4426950408889634f;
-  static const int force = getenv("KH_CHUNK") ? atoi(getenv("KH_CHUNK")) : 1;
-  if (force) {
-    Runs runs;
-    int nt = 0;
-    const int S = getenv("KH_S") ? atoi(getenv("KH_S")) : 1;
-    auto flush = [&]() -> int {
-      if (nt == 0) return 0;
-      const int n = nt;
-      nt = 0;
-#define LAUNCH(HD) return launch_chunks<HD>(runs, n, c, (const bf16*)qkv, ld, (bf16*)out, ldo, sl2, max_ctx, S, (cudaStream_t)stream);
-      if (hd == 128) { LAUNCH(128) }
-      if (hd == 64) { LAUNCH(64) }
-      LAUNCH(32)
+#define LAUNCH(HD) return launch_runs<HD>(c, (const bf16*)qkv, ld, (bf16*)out, ldo, sl2, max_ctx, (const int*)row0, (const int*)len, n_runs, (cudaStream_t)stream);
+  if (hd == 128) { LAUNCH(128) }
+  if (hd == 64) { LAUNCH(64) }
+  LAUNCH(32)
 #undef LAUNCH
-    };
-    for (int i = 0; i < n_runs; i++) {
-      const int r = ((const int*)row0)[i], n = ((const int*)len)[i];
-      if (r < 0 || n < 1) { kh_set_error("paged_prefill8: run %d is empty", i); return -1; }
-      for (int at = (n - 1) / CH_ROWS * CH_ROWS; at >= 0; at -= CH_ROWS) {
-        runs.row0[nt] = r + at;
-        runs.n[nt] = (uint16_t)(n - at < CH_ROWS ? n - at : CH_ROWS);
-        if (++nt == CH_MAX && flush()) return -1;
-      }
-    }
-    return flush();
-  }
-  const int smem = 2 * P8_ROWS * (hd * 2 + 16);
-  Pieces tiles;
-  int nt = 0;
-  auto flush = [&]() -> int {
-    if (nt == 0) return 0;
-#define LAUNCH(HD) KH_LAUNCH(paged_prefill8_k<HD>, dim3(nt, H), 128, smem, stream, tiles, c, (const bf16*)qkv, ld, (bf16*)out, ldo, sl2, max_ctx)
-    if (hd == 128) LAUNCH(128); else if (hd == 64) LAUNCH(64); else LAUNCH(32);
-#undef LAUNCH
-    KH_LAUNCH_CHECK("paged_prefill8");
-    nt = 0;
-    return 0;
-  };
-  for (int i = 0; i < n_runs; i++) {
-    const int r = ((const int*)row0)[i], n = ((const int*)len)[i];
-    if (r < 0 || n < 1) { kh_set_error("paged_prefill8: run %d is empty", i); return -1; }
-    for (int at = (n - 1) / P8_ROWS * P8_ROWS; at >= 0; at -= P8_ROWS) {          // the pieces that see the most keys first
-      tiles.row0[nt] = r + at;
-      tiles.n[nt] = (uint8_t)(n - at < P8_ROWS ? n - at : P8_ROWS);
-      if (++nt == P8_MAX_TILES && flush()) return -1;
-    }
-  }
-  return flush();
 }
