@@ -331,6 +331,11 @@ __device__ __forceinline__ uint32_t ld_early_u16(const uint8_t* p) {
   asm volatile("ld.global.b16 %0, [%1];" : "=h"(r) : "l"(p));
   return r;
 }
+__device__ __forceinline__ uint4 ld_early_16(uint64_t p) {
+  uint4 r;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
 // four codes times f (twice in a word), as f16
 __device__ __forceinline__ void scale4(uint32_t codes, uint32_t f, uint32_t& a, uint32_t& b) {
   asm("{\n\t.reg .b16 l, h;\n\t.reg .b32 x, y;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 x, l;\n\tcvt.rn.f16x2.e4m3x2 y, h;\n\t"
@@ -496,29 +501,22 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     const uint32_t off0 = tile_chunk(0, r1, 2 * l);
     uint32_t* s_wmax = reinterpret_cast<uint32_t*>(smem + C::WMAX) + vr * 8;
     bool bad = false;
-    // A thread looks up one position of a tile (t of 128): block two tiles ahead, exponent one tile ahead, and passes address and exponent on.
-    // No loaded value is looked at before the next turn.
-    int blk = 0, blk_at = -1;
+    // A thread looks up one position of a tile (t of 128; past the end of the context: its last position, with a factor of zero): block two tiles ahead,
+    // exponents one tile ahead, and passes address and exponent on.  No loaded value is looked at before the next turn, and no load stands
+    // behind a condition: its registers would be copied, and waited for, at once.
+    int blk, blk_at;
     uint32_t e_next = 0, e_now = 0;
     uint64_t a_next = 0;
     auto look = [&](int j) {                               // block of position 128 j + t
-      const int p = j * 128 + t;
-      blk_at = -1;
-      if (j < kt1 && p < ctx) {
-        const int lb = quot(c.div, p);
-        blk_at = p - lb * bs;
-        blk = ld_early_i32(bt + lb);
-      }
+      const int p = min(j * 128 + t, ctx - 1), lb = quot(c.div, p);
+      blk_at = p - lb * bs;
+      blk = ld_early_i32(bt + lb);
     };
-    auto exponent = [&]() {                                // ... its address and exponent
-      a_next = 0;
-      e_next = 0;
-      if (blk_at >= 0) {
-        if ((unsigned)blk >= (unsigned)c.n_blocks) { bad = true; blk = 0; }
-        const uint8_t* rc = record(c, blk, h);
-        e_next = ld_early_u16(rc + 2 * bs * HD + 2 * blk_at);
-        a_next = (uint64_t)(rc + (vr * bs + blk_at) * HD);
-      }
+    auto exponent = [&]() {                                // ... its address and exponents
+      bad |= (unsigned)blk >= (unsigned)c.n_blocks;
+      const uint8_t* rc = record(c, (int)min((unsigned)blk, (unsigned)c.n_blocks - 1), h);
+      e_next = ld_early_u16(rc + 2 * bs * HD + 2 * blk_at);
+      a_next = (uint64_t)(rc + (vr * bs + blk_at) * HD);
     };
     uint4 x[NP];
     auto publish = [&](int b) {                            // tile -> buffer b; then its codes are on their way
@@ -526,13 +524,14 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       pair_barrier(4 + vr);
 #pragma unroll
       for (int i = 0; i < NP / SLABS; i++) {
-        const uint64_t a = s_addr[b * 128 + i * RPP + r1];
+        const uint64_t a = s_addr[b * 128 + i * RPP + r1] + l * 16;
 #pragma unroll
-        for (int q = 0; q < SLABS; q++) x[i * SLABS + q] = a ? *reinterpret_cast<const uint4*>(a + q * 64 + l * 16) : make_uint4(0, 0, 0, 0);
+        for (int q = 0; q < SLABS; q++) x[i * SLABS + q] = ld_early_16(a + q * 64);
       }
       e_now = e_next;
     };
     auto factors = [&](int b, int it) {                    // 2^(e - E + 7) of its positions, E the tile's largest exponent
+      if ((kt0 + it) * 128 + t >= ctx) e_now = 0;
       const uint32_t mk = __reduce_max_sync(0xffffffffu, e_now & 0xffu), mv = __reduce_max_sync(0xffffffffu, e_now >> 8);
       if (lane == 0) s_wmax[b * 4 + (warp & 3)] = mk | mv << 16;
       pair_barrier(4 + vr);
@@ -576,11 +575,9 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(full + 8 * s);
-        if (j + 1 < kt1) {
-          publish(b ^ 1);
-          exponent();
-          look(j + 3);
-        }
+        publish(b ^ 1);                                    // (once more than there are tiles)
+        exponent();
+        look(j + 3);
       }
     }
     if (bad) report(c.err);
