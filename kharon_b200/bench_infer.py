@@ -31,6 +31,7 @@ def run(argv=None):
     tp_flag = f.int("tp", 0, "tensor-parallel degree (0 = world size under torchrun)")
     fused = not f.has("no-fused-comm")
     graphs = not f.has("no-graphs")
+    kv8 = f.has("kv8", "keep keys and values in 8 bits")
     f.maybe_help()
     cfg = Config(L, d, H, V, seq, 1)
     import torch.distributed as dist
@@ -55,12 +56,12 @@ def run(argv=None):
     else:
         m.init_weights(1234)
     say("infer bench: L=%d d=%d H=%d V=%d seq=%d  prompt=%d new=%d block=%d %s" %
-          (L, d, H, V, seq, plen, n_new, bs, "bf16" if bf16 else "fp32"))
+          (L, d, H, V, seq, plen, n_new, bs, ("bf16" if bf16 else "fp32") + (", 8-bit cache" if kv8 else "")))
     prompt = [(i * 131 + 7) % V for i in range(plen)]
     max_lb = (seq + bs - 1) // bs
     results = {"decode": [], "prefix": []}
     for G in Gs:
-        eng = InferEngine(m, bs, G * max_lb + 16, max(G, plen) * 1 + G * plen + 64, G + 1, use_graphs=graphs)
+        eng = InferEngine(m, bs, G * max_lb + 16, max(G, plen) * 1 + G * plen + 64, G + 1, use_graphs=graphs, kv8=kv8)
         best = None
         for _ in range(max(1, reps)):
             outs, st, ms = eng.generate([prompt] * G, n_new, max_active=G)
@@ -77,7 +78,7 @@ def run(argv=None):
                                       ratio=naive / paged))
         eng.close()
     for G in [g for g in Gs if g > 1]:
-        eng = InferEngine(m, bs, G * max_lb + 16, plen + 64 + G, G + 1)
+        eng = InferEngine(m, bs, G * max_lb + 16, plen + 64 + G, G + 1, kv8=kv8)
         best = None
         for _ in range(max(1, reps)):
             outs, st, ms = eng.generate_group(prompt, G, n_new)

@@ -36,7 +36,10 @@ class InferStats(dict):
 
 class InferEngine:
     def __init__(self, model: GPT, block_size=16, n_blocks=None, max_tokens=None, max_seqs=33, use_graphs=True,
-                 persistent_decode=None, attn_splits=None, flash_prefill=True):
+                 persistent_decode=None, attn_splits=None, flash_prefill=True, kv8=False):
+        """``kv8``: keys and values are kept in 8 bits (``ops.append_kv8``): half the cache and half the bytes that attention over long contexts
+        reads, for values that are off by up to 2^-4.  Every token, prompts' too, attends to the cache as it is kept, so results do not
+        depend on how steps are composed.  Decode steps take the kernel chain (the persistent kernel reads a bf16 cache)."""
         cfg = model.cfg
         self.model, self.cfg = model, cfg
         self.dev, self.dt = model.device, model.dtype
@@ -53,8 +56,14 @@ class InferEngine:
             raise _native.NativeError(lib.kh_last_error().decode())
         L, d, dl, fo = cfg.n_layer, cfg.d_model, cfg.d_model // self.tp, 4 * cfg.d_model // self.tp
         z = dict(device=self.dev)
-        self.kc = torch.zeros(L, self.n_blocks, self.bs, self.Hl, self.hd, dtype=self.dt, **z)
-        self.vc = torch.zeros_like(self.kc)
+        self.kc = self.vc = self.kv8 = None
+        if kv8:
+            if self.hd not in ops.KV8_HEAD_DIMS:
+                raise ValueError("kv8: head width %d is not one of %s" % (self.hd, ops.KV8_HEAD_DIMS))
+            self.kv8 = torch.zeros(L, self.n_blocks, self.Hl, ops.kv8_record_bytes(self.bs, self.hd), dtype=torch.uint8, **z)
+        else:
+            self.kc = torch.zeros(L, self.n_blocks, self.bs, self.Hl, self.hd, dtype=self.dt, **z)
+            self.vc = torch.zeros_like(self.kc)
         # packed step metadata: tok | pos | slot | rows | btab | pairs
         mt, ms_ = self.max_tokens, max_seqs
         self._o_tok, self._o_pos, self._o_slot = 0, mt, 2 * mt
@@ -108,7 +117,7 @@ class InferEngine:
         #   L24 d2048, context 300: G = 16 1537 / 3459, 17 2478 / 1832 (two launches), 32 3080 / 1933.
         if persistent_decode is None:
             persistent_decode = os.environ.get("KHARON_PERSISTENT_DECODE", "1") != "0"
-        self.persistent = bool(persistent_decode and self.skinny is not None and self.tp == 1 and self.dt == torch.bfloat16
+        self.persistent = bool(persistent_decode and not kv8 and self.skinny is not None and self.tp == 1 and self.dt == torch.bfloat16
                                and ops.decode_layers_ok(1, d, cfg.n_head, cfg.head_dim, cfg.seq))
         self.persistent_max, self.skinny_rows = 0, ops.SKINNY_BEST_ROWS
         if self.persistent:
@@ -123,7 +132,7 @@ class InferEngine:
                                             dtype=torch.int64, device=self.dev)
             self.decode_work = ops.decode_layers_work(d, self.dev)
         # Contexts beyond 2048 positions: the keys of a token are cut into ranges with a CTA each (split-KV) and merged
-        self.attn_splits = int(attn_splits) if attn_splits else (1 if cfg.seq <= 2048 else min(16, (cfg.seq + 2047) // 2048))
+        self.attn_splits = 1 if kv8 else int(attn_splits) if attn_splits else (1 if cfg.seq <= 2048 else min(16, (cfg.seq + 2047) // 2048))
         self.attn_scratch = None
         if self.attn_splits > 1 and self.dev.type == "cuda":
             self.attn_scratch = torch.zeros(self.max_tokens * self.Hl * self.attn_splits * (self.hd + 1), dtype=torch.float32, **z)
@@ -131,7 +140,7 @@ class InferEngine:
         # step) run their attention on the tensor cores with the training forward kernel, all prompts in one launch;
         # prompts beside decoding sequences, short and chunked ones go through the paged tile kernel (fp32 probabilities),
         # everything else through the paged kernel.
-        self.flash_prefill = bool(flash_prefill and self.dev.type == "cuda" and self.dt == torch.bfloat16
+        self.flash_prefill = bool(flash_prefill and not kv8 and self.dev.type == "cuda" and self.dt == torch.bfloat16
                                   and self.hd in (64, 128))
         self._fresh = self._runs = None
         self._fused = False
@@ -182,22 +191,25 @@ class InferEngine:
             return
         ln, qkv, att, xmid = self.ln[:ntok], self.qkv[:ntok], self.att[:ntok], self.xmid[:ntok]
         decode = ntok == nseq            # one new token per sequence: the attention kernel appends k, v itself
-        if self._runs:
+        if self._runs and self.kv8 is None:
             runs = self._runs[0]
             rest = [(qkv[a:b], att[a:b], pos[a:b], slot[a:b]) for a, b in self._runs[1]]
         for l in range(cfg.n_layer):
             self._ln_lin(xs, m.L(l, "ln1_w"), m.L(l, "ln1_b"), ln, m.L(l, "qkv_w"), qkv, ops.EPI_BIAS, m.L(l, "qkv_b"))
-            if not decode:
-                ops.append_kv(qkv, self.kc[l], self.vc[l], pos, slot, self.d_btab, self.bs, self.Hl, self.hd, ntok)
-            if not decode and self._fresh:
-                ops.flash_fwd_varlen(qkv, att, self._fresh, self.Hl, self.hd)
-            elif not decode and self._runs:
-                ops.paged_prefill(qkv, self.kc[l], self.vc[l], att, pos, slot, self.d_btab, self.bs, self.Hl, self.hd, runs, cfg.seq)
-                for q, o, p, s in rest:
-                    ops.paged_attn(q, self.kc[l], self.vc[l], o, p, s, self.d_btab, self.bs, self.Hl, self.hd, q.shape[0], cfg.seq)
+            if self.kv8 is not None:
+                self._attend8(l, qkv, att, pos, slot, ntok, decode)
             else:
-                ops.paged_attn(qkv, self.kc[l], self.vc[l], att, pos, slot, self.d_btab, self.bs, self.Hl, self.hd, ntok,
-                               cfg.seq, append=decode, n_split=self.attn_splits, scratch=self.attn_scratch)
+                if not decode:
+                    ops.append_kv(qkv, self.kc[l], self.vc[l], pos, slot, self.d_btab, self.bs, self.Hl, self.hd, ntok)
+                if not decode and self._fresh:
+                    ops.flash_fwd_varlen(qkv, att, self._fresh, self.Hl, self.hd)
+                elif not decode and self._runs:
+                    ops.paged_prefill(qkv, self.kc[l], self.vc[l], att, pos, slot, self.d_btab, self.bs, self.Hl, self.hd, runs, cfg.seq)
+                    for q, o, p, s in rest:
+                        ops.paged_attn(q, self.kc[l], self.vc[l], o, p, s, self.d_btab, self.bs, self.Hl, self.hd, q.shape[0], cfg.seq)
+                else:
+                    ops.paged_attn(qkv, self.kc[l], self.vc[l], att, pos, slot, self.d_btab, self.bs, self.Hl, self.hd, ntok,
+                                   cfg.seq, append=decode, n_split=self.attn_splits, scratch=self.attn_scratch)
             # row-parallel products: one GEMM, or under TP the fused GEMM + all-reduce kernel / NCCL seam
             self._row(att, m.L(l, "proj_w"), xmid, m.L(l, "proj_b"), xs)
             self._ln_lin(xmid, m.L(l, "ln2_w"), m.L(l, "ln2_b"), ln, m.L(l, "fc_w"), self.act[:ntok], ops.EPI_GELU, m.L(l, "fc_b"))
@@ -210,6 +222,20 @@ class InferEngine:
                      self.logits[:nseq, :cfg.vocab])
         ops.sample(self.logits, cfg.vocab, self.temperature, self.seed, self.step_no, rep, self.h_out if nseq * rep <= self._direct else self.d_out, nseq,
                        step_dev=self.d_stepno)
+
+    def _attend8(self, l, qkv, att, pos, slot, ntok, decode):
+        """Attention of one layer over the 8-bit cache: decode steps append and attend in one kernel; steps with several tokens of a sequence append first,
+        then ``_runs`` go to the run kernels and what lies between them to the single-token kernel."""
+        kv, tail = self.kv8[l], (self.d_btab, self.bs, self.Hl, self.hd)
+        if decode:
+            ops.paged_attn8(qkv, kv, att, pos, slot, *tail, ntok, self.cfg.seq, append=True)
+            return
+        ops.append_kv8(qkv, kv, pos, slot, *tail, ntok)
+        runs, rest = self._runs
+        if runs:
+            ops.paged_prefill8(qkv, kv, att, pos, slot, *tail, runs, self.cfg.seq)
+        for a, b in rest:
+            ops.paged_attn8(qkv[a:b], kv, att[a:b], pos[a:b], slot[a:b], *tail, b - a, self.cfg.seq)
 
     def _lin(self, x, w, out, epi=ops.EPI_NONE, bias=None, aux=None):
         """Column-parallel / replicated linear layer: skinny kernel for decode-sized inputs."""
@@ -279,6 +305,25 @@ class InferEngine:
         least = {32: 1280, 64: 896, 128: 1100}[self.hd] if rest else 600 if self.hd == 128 else 1
         return (runs, rest) if runs and ntok * self.Hl >= least else None
 
+    def _runs8(self, ntok, nseq):
+        """(runs, rest) of a step over the 8-bit cache: runs = [(first row, length)] of several consecutive positions of a sequence, rest = [(a, b)] the
+        row ranges between them."""
+        if ntok == nseq or self.hd == 16:              # (the run kernels take heads of 32 and more)
+            return [], [(0, ntok)]
+        pos = self.np_meta[self._o_pos:self._o_pos + ntok]
+        slot = self.np_meta[self._o_slot:self._o_slot + ntok]
+        cuts = (np.flatnonzero((slot[1:] != slot[:-1]) | (pos[1:] != pos[:-1] + 1)) + 1).tolist()
+        runs, rest, at = [], [], 0
+        for a, b in zip([0] + cuts, cuts + [ntok]):
+            if b - a > 1:
+                if at < a:
+                    rest.append((at, a))
+                runs.append((a, b - a))
+                at = b
+        if at < ntok:
+            rest.append((at, ntok))
+        return runs, rest
+
     def _one_kernel(self, ntok, nseq):
         """Whether this step runs in the persistent kernel.  Over long contexts its W warps per (sequence, head) lose to the chain's
         attention (split-KV where the model has more than 2048 positions) once the sequences fill the SMs.  L4 d1024, 4200 positions, us a step, persistent / chain:
@@ -293,7 +338,7 @@ class InferEngine:
         """Metadata is already in ``h_meta``; runs one step and returns the sampled ids (host)."""
         self._fused = self._one_kernel(ntok, nseq)
         self._fresh = self._fresh_prompts(ntok, nseq)
-        self._runs = None if self._fresh else self._prompt_runs(ntok, nseq)
+        self._runs = self._runs8(ntok, nseq) if self.kv8 is not None else None if self._fresh else self._prompt_runs(ntok, nseq)
         sd = self.seed & 0xFFFFFFFFFFFFFFFF
         to_i32 = lambda u: u - (1 << 32) if u >= (1 << 31) else u
         self.np_meta[self._o_step:self._o_step + 3] = (self.step_no & 0x7FFFFFFF, to_i32(sd & 0xFFFFFFFF), to_i32(sd >> 32))
@@ -339,7 +384,10 @@ class InferEngine:
             return False
         if npairs:
             self.d_meta.copy_(self.h_meta, non_blocking=True)
-            ops.copy_blocks(self.kc, self.vc, self.d_pairs, npairs)
+            if self.kv8 is not None:
+                ops.copy_blocks8(self.kv8, self.d_pairs, npairs)
+            else:
+                ops.copy_blocks(self.kc, self.vc, self.d_pairs, npairs)
         out = self._run(ntok, nseq)
         _native.rt_check(_native.rt().kh_eng_commit(self._h, out.data_ptr(), nseq))
         return True
@@ -459,6 +507,8 @@ class InferEngine:
         return outs, self._stats(), ms
 
     def kv_bytes_per_position(self):
+        if self.kv8 is not None:
+            return self.cfg.n_layer * self.Hl * self.kv8.shape[-1] / self.bs
         return 2 * self.cfg.n_layer * self.Hl * self.hd * self.kc.element_size()
 
 
@@ -484,3 +534,9 @@ def smoke_decode():
     assert eng.persistent and all(len(o) == 32 for o in outs) and all(o == outs[0] for o in outs)
     ops.check_device_status()
     print("smoke: persistent decode kernel, 4 x 12 tokens")
+    # the 8-bit cache: quantised as it is written, attended to by prompts and single tokens
+    eng = InferEngine(m, block_size=16, max_seqs=5, kv8=True)
+    outs, st, ms = eng.generate_group(prompt, 4, 12)
+    assert all(len(o) == 32 for o in outs) and all(o == outs[0] for o in outs)
+    ops.check_device_status()
+    print("smoke: 8-bit cache, 4 x 12 tokens")

@@ -62,3 +62,33 @@ def attend(q, k, v, p_half_step=0.0):
     top = torch.einsum("he,jhe->hj", q.abs(), k.abs()).amax(-1) / math.sqrt(hd)
     c = 2 * ((hd + 4) * 2.0 ** -24 * top + 2.0 ** -21) + 2 * (ctx + 8) * 2.0 ** -24 + p_half_step
     return o, 2.0 ** -8 * o.abs() + (1 + 2.0 ** -8) * c[:, None] * mag + 1e-30
+
+
+def quantising_oracle(cfg, model):
+    """The PyTorch statement of the architecture, with keys and values replaced by what the 8-bit cache keeps of them (a row is a token and head)."""
+    from kharon_b200.models.oracle import OracleGPT
+    o = OracleGPT(cfg)
+    o.load_from(model)
+    g, hd = grid()[:127].float(), cfg.d_model // cfg.n_head
+
+    def kept(x):
+        rows = x.reshape(-1, hd)
+        a = rows.abs().amax(-1)
+        e = torch.zeros_like(a)
+        for k in range(-40, 41):
+            e = torch.where(a > 448.0 * 2.0 ** k, torch.full_like(a, 2.0 ** (k + 1)), e)
+        e = e.clamp(min=2.0 ** -40)
+        y = rows.abs() / e[:, None]
+        up = torch.searchsorted(g, y.contiguous()).clamp(max=126)
+        dn = (up - 1).clamp(min=0)
+        lo, hi = y - g[dn], g[up] - y
+        i = torch.where((lo < hi) | ((lo == hi) & (dn % 2 == 0)), dn, up)
+        return (torch.sign(rows) * g[i] * e[:, None]).reshape(x.shape)
+
+    def hook(module, args, out):
+        q, k, v = out.split(cfg.d_model, dim=-1)
+        return torch.cat([q, kept(k), kept(v)], -1)
+
+    for b in o.blocks:
+        b.qkv.register_forward_hook(hook)
+    return o

@@ -5,7 +5,10 @@ import pytest
 import torch
 
 from kharon_b200 import ops
-from kv8_exact import attend, quantise, rows_of
+from kharon_b200 import bench_infer
+from kharon_b200.infer import InferEngine
+from kharon_b200.models import GPT, Config
+from kv8_exact import attend, quantise, quantising_oracle, rows_of
 
 
 def make(seed, lens, H, hd, bs, extra=2):
@@ -132,3 +135,60 @@ def test_refused_arguments():
     ops.paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, 0, 64, append=True)
     ops.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, [], 64)
     assert torch.equal(kv, before) and float(out.abs().max()) == 0.0
+
+
+CFG = Config(2, 64, 4, 97, 48, 1)
+PROMPTS = [[5, 17, 3], [9, 1, 44, 23, 8, 61, 2], [70], [11, 12, 13, 14, 15, 16, 17, 18, 19, 20, 21]]
+NEW = [12, 7, 20, 9]
+
+
+@pytest.fixture(scope="module")
+def pair():
+    m = GPT(CFG, "cpu", torch.float32)
+    m.init_weights(1234)
+    m.params.w.mul_(8.0)
+    m.params.p["lnf_w"].fill_(1.0)
+    for l in range(CFG.n_layer):
+        m.params.p["l%d.ln1_w" % l].fill_(1.0)
+        m.params.p["l%d.ln2_w" % l].fill_(1.0)
+    return m, quantising_oracle(CFG, m)
+
+
+def greedy(o, prompt, n_new):
+    toks = list(prompt)
+    with torch.no_grad():
+        for _ in range(n_new):
+            toks.append(int(o(torch.tensor([toks]))[0][0, -1].argmax()))
+    return toks
+
+
+@pytest.mark.parametrize("bs,active", [(4, 2), (64, 4), (8, 4), (3, 1)])
+def test_engine_over_the_8bit_cache_is_token_exact(pair, bs, active):
+    """Greedy decoding with the quantised keys and values, whatever the block size and however prompts and decoding sequences share steps."""
+    m, o = pair
+    eng = InferEngine(m, block_size=bs, max_seqs=4, kv8=True)
+    assert eng.kc is None and eng.kv8.dtype == torch.uint8
+    outs, st, _ = eng.generate(PROMPTS, NEW, max_active=active)
+    for p, n, got in zip(PROMPTS, NEW, outs):
+        assert got == greedy(o, p, n)
+    assert st["tokens_decoded"] == sum(NEW)
+
+
+def test_shared_prefix_over_the_8bit_cache(pair):
+    m, o = pair
+    eng = InferEngine(m, block_size=4, max_seqs=9, kv8=True)
+    outs, st, _ = eng.generate_group(PROMPTS[3][:10], 8, 9)
+    assert all(x == greedy(o, PROMPTS[3][:10], 9) for x in outs) and st["prefix_blocks_saved"] == 7 * (10 // 4)
+    # per layer, head and block of 4 positions: 2 * 4 * 16 codes and 8 exponents, padded to 160 bytes; fp32 keeps 2 * 16 * 4 bytes a position
+    assert eng.kv_bytes_per_position() == 2 * 4 * 160 / 4 and InferEngine(m, block_size=4, max_seqs=9).kv_bytes_per_position() == 2 * 4 * 128
+
+
+def test_engine_refuses_head_widths_without_an_8bit_cache():
+    with pytest.raises(ValueError):
+        InferEngine(GPT(Config(1, 48, 2, 50, 16, 1), "cpu", torch.float32), block_size=4, max_seqs=2, kv8=True)
+
+
+def test_bench_command_with_the_8bit_cache():
+    r = bench_infer.run(["--layers", "1", "--d", "64", "--heads", "4", "--vocab", "50", "--seq", "32", "--prompt", "6", "--new", "4", "--block", "4", "--bf16", "0",
+                         "--G", "1,2", "--device", "cpu", "--reps", "1", "--kv8"])
+    assert len(r["decode"]) == 2 and r["decode"][0]["kv_paged_mb"] > 0

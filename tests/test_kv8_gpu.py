@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from kharon_b200 import ops
+from kharon_b200.infer import InferEngine
+from kharon_b200.models import GPT, Config
 from kv8_exact import attend, grid, quantise, rows_of
 from test_kv8_cpu import awkward
 
@@ -368,3 +370,100 @@ def test_fp32_rows_on_a_gpu_take_the_plain_evaluation():
     ops.paged_attn8(qkv.float(), kv, out, pos, slot, btab, bs, H, hd, 9, 16)
     ops.paged_attn8(qkv, kv, out2, pos, slot, btab, bs, H, hd, 9, 16)
     assert float((out - out2.float()).abs().max()) <= 2.0 ** -7 * float(out.abs().max())
+
+
+@pytest.mark.parametrize("L,d,heads,bs", [(2, 128, 4, 8), (2, 256, 4, 16), (2, 256, 2, 5), (1, 64, 4, 2)])
+def test_engine_over_the_8bit_cache(L, d, heads, bs, monkeypatch):
+    """Prompts that join a step beside decoding sequences (runs of many and of few tokens, single ones), captured and eager decode steps, a shared prefix;
+    and the logits of a prefill and of a mixed step against the same engine with the plain evaluation of the cache's operators.  Both round at the
+    same points; what differs is a bf16 step of some attention outputs, and codes that this moves: the bound of the engine's other tests, 3e-2."""
+    cfg = Config(L, d, heads, 300, 200, 1)
+    m = GPT(cfg, DEV, torch.bfloat16)
+    m.init_weights(1234)
+    m.sync_bf16()
+    g = torch.Generator().manual_seed(d + bs)
+    prompts = [torch.randint(0, 300, (n,), generator=g).tolist() for n in (5, 130, 1, 70, 17, 2, 40)]
+    new = [20, 12, 25, 9, 14, 30, 8]
+    outs = {}
+    for graphs in (True, False):
+        e = InferEngine(m, block_size=bs, max_seqs=4, max_tokens=264, use_graphs=graphs, kv8=True)
+        assert e.kc is None and not e.persistent
+        a, _, _ = e.generate(prompts, new, max_active=3)
+        b, _, _ = e.generate(prompts, new, max_active=3)
+        assert a == b and (len(e.graphs) > 0) == graphs
+        outs[graphs] = a
+    assert outs[True] == outs[False]
+    e = InferEngine(m, block_size=bs, max_seqs=6, kv8=True)
+    grp, st, _ = e.generate_group(prompts[4], 5, 12)
+    assert all(x == grp[0] for x in grp) and st["prefix_blocks_saved"] == 4 * (17 // bs)
+
+    def logits():
+        e = InferEngine(m, block_size=bs, max_seqs=8, max_tokens=512, use_graphs=False, kv8=True)
+        got = []
+        run = e._run
+
+        def spy(ntok, nseq, rep=1):
+            r = run(ntok, nseq, rep).clone()
+            got.append((ntok, e.logits[:nseq, :300].float().clone()))
+            return r
+        e._run = spy
+        e.generate(prompts, 1)                                     # one step: every prompt
+        e.generate([prompts[1], prompts[6]], [4, 1], max_active=2)
+        return got
+    native = logits()
+    from kharon_b200.ops import reference as ref
+
+    def attn(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=False):
+        if append:
+            ref.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+        ref.paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx)
+
+    def prefill(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
+        for r, n in runs:
+            ref.paged_attn8(qkv[r:r + n], kv, out[r:r + n], pos[r:r + n], slot[r:r + n], btab, bs, H, hd, n, max_ctx)
+    monkeypatch.setattr(ops, "append_kv8", ref.append_kv8)
+    monkeypatch.setattr(ops, "paged_attn8", attn)
+    monkeypatch.setattr(ops, "paged_prefill8", prefill)
+    plain = logits()
+    assert [n for n, _ in native] == [n for n, _ in plain]
+    for (_, x), (_, y) in zip(native[:2], plain[:2]):              # (later steps follow from the tokens chosen)
+        assert ((x - y).norm() / y.norm()).item() < 3e-2
+    assert ops.error_word() == 0
+
+
+def test_long_runs_leave_no_status_code():
+    """Many key tiles and more items than SMs, so that every role of the kernel for long runs waits for every other."""
+    for hd, H, runs in ((128, 16, [(2000, 256), (1500, 700), (0, 300), (60, 129)]), (64, 16, [(0, 1000), (0, 511), (3000, 65)]), (32, 8, [(5000, 300), (100, 100)])):
+        lens = [p + n for p, n in runs]
+        kv, btab, pos, slot, qkv = make(hd, lens, H, hd, 16)
+        ops.append_kv8(qkv, kv, pos, slot, btab, 16, H, hd, len(pos))
+        new = torch.cat([torch.arange(n) >= p for (p, _), n in zip(runs, lens)]).to(DEV)
+        q, p, s = qkv[new], pos[new].contiguous(), slot[new].contiguous()
+        out, one = (torch.zeros(len(p), H * hd, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+        starts, at = [], 0
+        for _, k in runs:
+            starts.append((at, k))
+            at += k
+        for _ in range(20):
+            ops.paged_prefill8(q, kv, out, p, s, btab, 16, H, hd, starts, max(lens))
+        first = out.clone()
+        ops.paged_prefill8(q, kv, out, p, s, btab, 16, H, hd, starts, max(lens))
+        ops.paged_attn8(q, kv, one, p, s, btab, 16, H, hd, len(p), max(lens))
+        torch.cuda.synchronize()
+        assert ops.error_word() == 0 and torch.equal(first, out)
+        assert ((one.float() - out.float()).norm() / one.float().norm()).item() < 2 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("where", [22, 45, 63, 64, 127])
+def test_nan_keys_at_every_place_of_a_tile(where):
+    """A NaN in a key makes the score of its position, and with it every row that sees it, NaN."""
+    H, hd, bs, n = 2, 64, 16, 300
+    kv, btab, pos, slot, qkv = make(where, [n], H, hd, bs)
+    qkv[where, H * hd + 5] = math.nan
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    for runs in ([(0, n)], [(0, 100), (100, 64), (164, 136)]):
+        out = torch.zeros(n, H * hd, device=DEV, dtype=torch.bfloat16)
+        ops.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, n)
+        torch.cuda.synchronize()
+        assert bool(out[where:, :hd].isnan().all()) and not bool(out[:where].isnan().any()) and not bool(out[:, hd:].isnan().any())
+    assert ops.error_word() == 0
