@@ -11,8 +11,6 @@
 // and infinities become the largest code, NaN stays NaN and does not count for the maximum.
 #include "paged8.cuh"
 
-extern "C" int kh_kv8_record_bytes(int bs, int hd) { return (2 * bs * hd + 2 * bs + 31) / 32 * 32; }
-
 // ------------------------------------------------------------------------------- append and read back
 // A lane takes sixteen elements of a k row and of the v row beside it: HD / 16 lanes of a warp hold both and find their largest magnitudes with
 // shuffles; the exponents leave as one pair.  The lanes of a token (H HD / 16 of them) lie side by side; a CTA covers 256 of them, of several tokens
@@ -249,7 +247,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
   e = e_n;
   // q: lane's dims (of slab s: 64 s + 16 i4 ..; narrower heads: HD / 4 from HD / 4 i4) as f16 pairs, rows alike
   uint32_t qa[NM][2];
-  float sc;
+  float sc, qf;
   {
     constexpr int PER = HD / 4 / KS;               // dims of a lane and slab
     uint32_t w[KS][PER / 2], m = 0;
@@ -264,14 +262,14 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
-    const float f = pow2_of((uint32_t)(127 - eq));
+    qf = pow2_of((uint32_t)(127 - eq));
     sc = scale * pow2_of((uint32_t)(127 + eq));
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int x = 0; x < PER / 2; x++) {
         const float2 a = unpack_bf16(w[s][x]);
-        qa[s * (PER / 4) + x / 2][x & 1] = pack_f16(a.x * f, a.y * f);
+        qa[s * (PER / 4) + x / 2][x & 1] = pack_f16(a.x * qf, a.y * qf);
       }
   }
   float o[NM][4];
@@ -310,15 +308,19 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
       kc[x] = to_e4m3x2(a.x * fk, a.y * fk);
       vc[x] = to_e4m3x2(b.x * fv, b.y * fv);
       const f32x2 kk = f32x2_of(half2_of(kc[x])), vv = f32x2_of(half2_of(vc[x]));
-      s = fmaf(q.x, lo2(kk), fmaf(q.y, hi2(kk), s));
+      s = fmaf(q.x * qf, lo2(kk), fmaf(q.y * qf, hi2(kk), s));
       o[x][0] = lo2(vv) * 16384.f;
       o[x][2] = hi2(vv) * 16384.f;
     }
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    R = s * scale * pow2_of(ek) + (float)((int)ev - 127);
+    R = fmaf(s * sc, pow2_of(ek), (float)((int)ev - 127));
     l = g == 0 ? 16384.f * fv : 0.f;
-    if (R != R) l = R;                             // (a NaN in q or k)
+    if (R == -INFINITY) {                          // (an infinity in q: the position has no weight ..
+      l = 0.f;
+#pragma unroll
+      for (int x = 0; x < PER / 2; x++) o[x][0] = o[x][2] = 0.f;
+    } else if (!(R < INFINITY)) l = __int_as_float(0x7fffffff);      // .. or all of it, inf - inf; or a NaN in q or k)
     const int b = block_of(c, sl, p);
     if (b < 0) bad = true;
     else {
@@ -523,12 +525,9 @@ static int launch_attn8(const Cache& c, const void* qkv, int ld, void* out, int 
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (S > 8) {
-    static bool opted = false;                     // clusters of more than eight
-    if (!opted && cudaFuncSetAttribute(paged_attn8_k<HD, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-      cudaGetLastError();
-      S = 8;
-    } else opted = true;
+  if (S > 8 && cudaFuncSetAttribute(paged_attn8_k<HD, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    S = 8;
   }
   if (S > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
@@ -546,6 +545,7 @@ extern "C" int kh_paged_attn8(const void* qkv, int ld, void* kv, int n_blocks, i
   if (make_cache(c, "paged_attn8", kv, n_blocks, rec, pos, slot, btab, n_slots, max_lb, bs, H, hd)) return -1;
   if (((uintptr_t)qkv & 15) || ld % 8 || ld < 3 * H * hd || ((uintptr_t)out & 15) || ldo % 8 || ldo < H * hd) { kh_set_error("paged_attn8: rows must be 16-byte aligned"); return -1; }
   if (ntok <= 0) return 0;
+  max_ctx = max_ctx < max_lb * bs ? max_ctx : max_lb * bs;
   if (ntok > (1 << 27)) { kh_set_error("paged_attn8: %d tokens are too many", ntok); return -1; }
   const float sl2 = scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;

@@ -87,7 +87,7 @@ inline int make_cache(Cache& c, const char* name, const void* kv, int n_blocks, 
   if (hd != 16 && hd != 32 && hd != 64 && hd != 128) { kh_set_error("%s: head dim %d is not supported", name, hd); return -1; }
   if (bs < 1 || H < 1 || H > 65535 || n_blocks < 1 || max_lb < 1 || n_slots < 1) { kh_set_error("%s: empty cache", name); return -1; }
   if (rec < 2 * bs * hd + 2 * bs || rec % 32 || ((uintptr_t)kv & 31)) { kh_set_error("%s: records of %d bytes do not fit block size %d", name, rec, bs); return -1; }
-  if ((unsigned long long)max_lb * bs * bs >= 1ull << 32 || (long long)max_lb * bs > 0x7fffffffll) { kh_set_error("%s: block table of %d x %d positions is too long", name, max_lb, bs); return -1; }
+  if ((unsigned long long)max_lb * bs * bs >= 1ull << 32 || (long long)max_lb * bs > 1ll << 30) { kh_set_error("%s: block table of %d x %d positions is too long", name, max_lb, bs); return -1; }
   if ((unsigned long long)n_blocks * H * rec >> 36) { kh_set_error("%s: a cache of %d blocks x %d heads x %d bytes is larger than 64 GB", name, n_blocks, H, rec); return -1; }
   c = Cache{(uint8_t*)kv, (const int*)pos, (const int*)slot, (const int*)btab, kh_error_word_dev(), n_blocks, n_slots, max_lb, bs, H, rec,
             Div{bs == 1 ? 0u : (uint32_t)(((1ull << 32) + bs - 1) / bs)}};

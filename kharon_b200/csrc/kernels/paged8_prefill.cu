@@ -925,6 +925,7 @@ extern "C" int kh_paged_prefill8(const void* qkv, int ld, const void* kv, int n_
   if (make_cache(c, "paged_prefill8", kv, n_blocks, rec, pos, slot, btab, n_slots, max_lb, bs, H, hd)) return -1;
   if (hd == 16) { kh_set_error("paged_prefill8: head dim %d is not supported", hd); return -1; }
   if (((uintptr_t)qkv & 15) || ld % 8 || ld < 3 * H * hd || ((uintptr_t)out & 15) || ldo % 8 || ldo < H * hd) { kh_set_error("paged_prefill8: rows must be 16-byte aligned"); return -1; }
+  max_ctx = max_ctx < max_lb * bs ? max_ctx : max_lb * bs;
   const float sl2 = scale * 1.4426950408889634f;
 #define LAUNCH(HD) return launch_runs<HD>(c, (const bf16*)qkv, ld, (bf16*)out, ldo, sl2, max_ctx, (const int*)row0, (const int*)len, n_runs, (cudaStream_t)stream);
   if (hd == 128) { LAUNCH(128) }

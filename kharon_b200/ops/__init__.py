@@ -605,7 +605,8 @@ def kv8_record_bytes(bs, hd):
     """Bytes of one (block, head) record of the 8-bit cache: ``bs * hd`` e4m3 codes of k, as many of v, ``bs`` pairs of exponent
     bytes, padded to a multiple of 32.  A layer's cache is uint8 ``[n_blocks, H, kv8_record_bytes(bs, hd)]``, zeroed once.  A row of
     ``hd`` numbers is kept as code * 2^(byte - 127) with the smallest exponent in [-63, 63] for which no magnitude exceeds 448;
-    what lies above 448 * 2^63 (infinities too) becomes the largest code, NaN stays NaN."""
+    what lies above 448 * 2^63 (infinities too) becomes the largest code, NaN stays NaN.  A layer's cache takes up to 64 GB, a block table up
+    to 2^30 positions a sequence.  Outputs of the operators below must not overlap their inputs."""
     return (2 * bs * hd + 2 * bs + 31) // 32 * 32
 
 
@@ -670,8 +671,8 @@ def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=
     if out.shape[0] < ntok or out.device != qkv.device:
         raise ValueError("paged_attn8: %d rows of output for %d tokens" % (out.shape[0], ntok))
     _call(_lib().kh_paged_attn8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2], out.data_ptr(), out.stride(0),
-          pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, 1.0 / math.sqrt(hd), ntok, max_ctx,
-          int(append), _stream())
+          pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, 1.0 / math.sqrt(hd), ntok,
+          min(max_ctx, 0x7fffffff), int(append), _stream())
 
 
 def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
@@ -694,7 +695,7 @@ def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
     rows, lens = _row_lists(runs, limit)
     _call_keeping((rows, lens), _lib().kh_paged_prefill8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2],
                   out.data_ptr(), out.stride(0), pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd,
-                  1.0 / math.sqrt(hd), max_ctx, C.addressof(rows), C.addressof(lens), len(runs), _stream())
+                  1.0 / math.sqrt(hd), min(max_ctx, 0x7fffffff), C.addressof(rows), C.addressof(lens), len(runs), _stream())
 
 
 def copy_blocks8(kv, pairs, npairs):
@@ -707,6 +708,8 @@ def copy_blocks8(kv, pairs, npairs):
         for i in range(npairs):
             kv[:, int(pairs[2 * i + 1])].copy_(kv[:, int(pairs[2 * i])])
         return
+    if kv.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("copy_blocks8: the tensors must be on the current device")
     _call(_lib().kh_copy_blocks8, 1, kv.data_ptr(), pairs.data_ptr(), npairs, kv.shape[0], kv.shape[1], kv.stride(1), kv.stride(0), _stream())
 
 

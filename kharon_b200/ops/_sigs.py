@@ -66,7 +66,6 @@ _OPTIONAL = {
     "kh_paged_attn_split": (i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, i32, i32, i32, vp),
     "kh_paged_attn": (i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, i32, i32, vp),
     "kh_paged_prefill": (i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp, vp, i32, vp),
-    "kh_kv8_record_bytes": (i32, i32, i32),
     "kh_append_kv8": (i32, vp, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp),
     "kh_read_kv8": (i32, vp, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp),
     "kh_paged_attn8": (i32, vp, i32, vp, i32, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, i32, i32, vp),

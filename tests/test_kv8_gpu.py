@@ -336,6 +336,62 @@ def test_prompt_then_decode_steps_eager_captured_and_on_another_stream(hd, H, bs
     assert ops.error_word() == 0
 
 
+@pytest.mark.parametrize("hd,bs", [(16, 3), (32, 16), (64, 5), (128, 16)])
+def test_infinite_queries_and_queries_near_the_types_ends(hd, bs):
+    """An infinity in q leaves no finite row, be the scores +inf or -inf, at the first position too and with the token's own k taken from its registers;
+    magnitudes of 1e19 beside keys of 1e-19, and of 1e-30, are ordinary."""
+    H, lens = 6, [1, 2, 9, 70, 300]
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, 0] = float("inf")                       # head 0; what the others take comes after it
+    qkv[:, hd + 1] = float("-inf")
+    qkv[:, 2 * hd + 2] = float("nan")
+    qkv[:, 3 * hd:4 * hd] *= 1e19
+    qkv[:, d + 3 * hd:d + 4 * hd] *= 1e-19
+    qkv[:, 4 * hd:5 * hd] *= 1e-30
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    last = torch.tensor([sum(lens[:i + 1]) - 1 for i in range(len(lens))], device=DEV)
+    q, p, s = qkv[last], pos[last].contiguous(), slot[last].contiguous()
+    outs = []
+    for append in (False, True):
+        out = torch.zeros(len(lens), d, device=DEV, dtype=torch.bfloat16)
+        ops.paged_attn8(q, kv, out, p, s, btab, bs, H, hd, len(lens), max(lens), append=append)
+        check_rows(out, q, kv, btab, bs, H, hd, p, s, range(len(lens)))
+        outs.append(out)
+    assert bool(outs[0][:, :3 * hd].isnan().all()) and not bool(outs[0][:, 3 * hd:].isnan().any())
+    if hd > 16:
+        out, at, runs = torch.zeros(n, d, device=DEV, dtype=torch.bfloat16), 0, []
+        for k in lens:
+            runs.append((at, k))
+            at += k
+        ops.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max(lens))
+        check_rows(out, qkv, kv, btab, bs, H, hd, pos, slot, [0, 2, 11, 12, 40, 81, 82, 200, n - 1], p_half_step=2.0 ** -8)
+    assert ops.error_word() == 0
+
+
+def test_limits_beyond_the_table_and_calls_without_work():
+    H, hd, bs = 2, 64, 16
+    kv, btab, pos, slot, qkv = make(3, [40], H, hd, bs)
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, 40)
+    a, b = torch.zeros(2, 40, H * hd, device=DEV, dtype=torch.bfloat16)
+    ops.paged_attn8(qkv, kv, a, pos, slot, btab, bs, H, hd, 40, 40)
+    ops.paged_attn8(qkv, kv, b, pos, slot, btab, bs, H, hd, 40, 1 << 40)
+    assert torch.equal(a, b)
+    ops.paged_prefill8(qkv, kv, a, pos, slot, btab, bs, H, hd, [(0, 40)], 40)
+    ops.paged_prefill8(qkv, kv, b, pos, slot, btab, bs, H, hd, [(0, 40)], 1 << 40)
+    assert torch.equal(a, b)
+    before = kv.clone()
+    ops.paged_prefill8(qkv, kv, b, pos, slot, btab, bs, H, hd, [], 40)
+    ops.paged_attn8(qkv, kv, b, pos, slot, btab, bs, H, hd, 0, 40, append=True)
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, 0)
+    ops.read_kv8(kv, a, a, pos, slot, btab, bs, H, hd, 0)
+    ops.copy_blocks8(kv.unsqueeze(0), torch.zeros(0, dtype=torch.int32, device=DEV), 0)
+    assert torch.equal(a, b) and torch.equal(kv, before) and ops.error_word() == 0
+    long = torch.zeros(1, (1 << 26) + 1, dtype=torch.int32, device=DEV)      # 2^30 positions and sixteen
+    with pytest.raises(ops.KernelError):
+        ops.append_kv8(qkv, kv, pos, slot, long, bs, H, hd, 40)
+
+
 def test_refused_on_a_gpu():
     H, hd, bs = 2, 64, 16
     kv, btab, pos, slot, qkv = make(1, [20], H, hd, bs)
