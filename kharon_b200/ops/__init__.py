@@ -8,8 +8,10 @@ numerical oracle of the GPU tests and what the CPU test tier exercises.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
+import operator
 
 import torch
 
@@ -30,9 +32,12 @@ def _lib():
     return _native.cuda()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None)         # (absent from builds of torch for the CPU alone)
+
+
 def _stream():
     """Handle of the current device's current stream (without the Stream object of torch.cuda.current_stream())."""
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return torch._C._cuda_getCurrentRawStream(_current_device())
 
 
 #: when a list, every native call is also appended as (function, args, launches) -- see ``LaunchPlan``
@@ -611,49 +616,54 @@ def kv8_record_bytes(bs, hd):
 
 
 def _kv8_check(name, x, kv, pos, slot, btab, bs, H, hd, ntok):
-    """Argument checks of the 8-bit cache's operators; positions, sequences and blocks are checked in the kernels (status code 8)."""
+    """Argument checks of the 8-bit cache's operators; positions, sequences and blocks are checked in the kernels (status code 8).  Every attribute of a
+    tensor is asked for once: these checks are most of what a small call costs.  Returns the cache's and the table's part of a native call's arguments:
+    (cache, blocks, bytes of a record), (positions, sequences, table, its rows and columns, bs, H, hd)."""
     if hd not in KV8_HEAD_DIMS or bs < 1:
         raise ValueError("%s: head width %d (of %s) or block size %d is not supported" % (name, hd, KV8_HEAD_DIMS, bs))
-    if kv.dtype != torch.uint8 or kv.dim() != 3 or kv.shape[1:] != (H, (2 * bs * hd + 2 * bs + 31) // 32 * 32) or not kv.is_contiguous():
+    sk, i32 = kv.shape, torch.int32
+    if len(sk) != 3 or sk[2] != (2 * bs * hd + 2 * bs + 31) // 32 * 32 or sk[1] != H or kv.dtype is not torch.uint8 or not kv.is_contiguous():
         raise ValueError("%s: the cache must be contiguous uint8 [blocks, %d, %d]" % (name, H, kv8_record_bytes(bs, hd)))
-    i32 = torch.int32
-    if pos.dtype != i32 or slot.dtype != i32 or btab.dtype != i32 or btab.dim() != 2 or not btab.is_contiguous():
+    sb = btab.shape
+    if len(sb) != 2 or pos.dtype is not i32 or slot.dtype is not i32 or btab.dtype is not i32 or not btab.is_contiguous():
         raise ValueError("%s: positions, sequences and the block table must be int32, the table contiguous" % name)
-    if not 0 <= ntok <= len(x) or pos.numel() < ntok or slot.numel() < ntok or not (pos.is_contiguous() and slot.is_contiguous()):
+    if not 0 <= ntok <= x.shape[0] or pos.numel() < ntok or slot.numel() < ntok or not (pos.is_contiguous() and slot.is_contiguous()):
         raise ValueError("%s: %d tokens of rows %s, positions %s, sequences %s" % (name, ntok, tuple(x.shape), tuple(pos.shape), tuple(slot.shape)))
     dev = kv.get_device()                          # -1: the CPU
-    if x.get_device() != dev or pos.get_device() != dev or slot.get_device() != dev or btab.get_device() != dev or (dev >= 0 and dev != torch._C._cuda_getDevice()):
+    if x.get_device() != dev or pos.get_device() != dev or slot.get_device() != dev or btab.get_device() != dev or (dev >= 0 and dev != _current_device()):
         raise ValueError("%s: the tensors must be on one device, the current one" % name)
+    return (kv.data_ptr(), sk[0], sk[2]), (pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), sb[0], sb[1], bs, H, hd)
 
 
 def _kv8_rows(name, x, width, dtype):
-    if x.dtype != dtype or x.dim() != 2 or x.shape[1] < width or x.stride(1) != 1:
+    """Checks rows of a matrix; returns its address and pitch."""
+    st = x.stride()
+    if x.dtype is not dtype or len(st) != 2 or st[1] != 1 or x.shape[1] < width:
         raise ValueError("%s: rows of %d contiguous %s are needed, not %s %s" % (name, width, dtype, tuple(x.shape), x.dtype))
+    return x.data_ptr(), st[0]
 
 
 def append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok):
     """``append_kv`` into the 8-bit cache: quantises k and v of each listed token (``qkv`` rows q | k | v) and stores them at their positions.
     Two tokens of one call must not share a position of a block."""
-    _kv8_check("append_kv8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+    cache, table = _kv8_check("append_kv8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
     if _use_reference(qkv):
         return ref.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)
-    _kv8_rows("append_kv8", qkv, 3 * H * hd, torch.bfloat16)
-    _call(_lib().kh_append_kv8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2], pos.data_ptr(),
-          slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, ntok, _stream())
+    _call(_lib().kh_append_kv8, 1, *_kv8_rows("append_kv8", qkv, 3 * H * hd, torch.bfloat16), *cache, *table, ntok, _stream())
 
 
 def read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok):
     """The inverse of ``append_kv8``: rows ``k``, ``v`` [ntok, H * hd] (bf16, which holds the stored values exactly, or fp32) of the listed
     positions, for handing a cached sequence on (another engine, another block size, a bf16 cache)."""
-    _kv8_check("read_kv8", k, kv, pos, slot, btab, bs, H, hd, ntok)
-    if k.dtype not in (torch.bfloat16, torch.float32) or v.device != k.device or v.shape[0] < ntok or v.stride(0) != k.stride(0):
+    cache, table = _kv8_check("read_kv8", k, kv, pos, slot, btab, bs, H, hd, ntok)
+    dt = k.dtype
+    if dt not in (torch.bfloat16, torch.float32) or v.get_device() != k.get_device() or v.shape[0] < ntok or v.stride() != k.stride():
         raise ValueError("read_kv8: k and v must be bf16 or fp32 rows of one pitch, not %s %s and %s %s" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
-    _kv8_rows("read_kv8", k, H * hd, k.dtype)
-    _kv8_rows("read_kv8", v, H * hd, k.dtype)
+    k_at, pitch = _kv8_rows("read_kv8", k, H * hd, dt)
+    v_at, _ = _kv8_rows("read_kv8", v, H * hd, dt)
     if not kv.is_cuda:
         return ref.read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok)
-    _call(_lib().kh_read_kv8, 1, kv.data_ptr(), kv.shape[0], kv.shape[2], k.data_ptr(), v.data_ptr(), k.stride(0), int(k.dtype == torch.float32),
-          pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, ntok, _stream())
+    _call(_lib().kh_read_kv8, 1, *cache, k_at, v_at, pitch, int(dt is torch.float32), *table, ntok, _stream())
 
 
 def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=False):
@@ -661,41 +671,38 @@ def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=
     holds them.  ``append``: the kernel first quantises and stores each token's own k, v (valid when no two listed tokens belong to
     one sequence, i.e. decode steps); otherwise ``append_kv8`` must have run.  Few tokens over long contexts: the keys of a
     token are shared out to the thread blocks of a cluster; no workspace."""
-    _kv8_check("paged_attn8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
+    cache, table = _kv8_check("paged_attn8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
     if _use_reference(qkv):
         if append:
             ref.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)
         return ref.paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx)
-    _kv8_rows("paged_attn8", qkv, 3 * H * hd, torch.bfloat16)
-    _kv8_rows("paged_attn8", out, H * hd, torch.bfloat16)
-    if out.shape[0] < ntok or out.device != qkv.device:
+    x = _kv8_rows("paged_attn8", qkv, 3 * H * hd, torch.bfloat16)
+    y = _kv8_rows("paged_attn8", out, H * hd, torch.bfloat16)
+    if out.shape[0] < ntok or out.get_device() != qkv.get_device():
         raise ValueError("paged_attn8: %d rows of output for %d tokens" % (out.shape[0], ntok))
-    _call(_lib().kh_paged_attn8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2], out.data_ptr(), out.stride(0),
-          pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd, 1.0 / math.sqrt(hd), ntok,
-          min(max_ctx, 0x7fffffff), int(append), _stream())
+    _call(_lib().kh_paged_attn8, 1, *x, *cache, *y, *table, hd ** -0.5, ntok, min(max_ctx, 0x7fffffff), int(append), _stream())
 
 
 def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
     """``paged_prefill`` over the 8-bit cache: ``paged_attn8`` for runs of consecutive positions of one sequence each,
     ``runs = [(first row, length), ...]``, whose K/V are in the cache already (``append_kv8``).  Head widths 32, 64 and 128."""
-    _kv8_check("paged_prefill8", qkv, kv, pos, slot, btab, bs, H, hd, 0)
+    cache, table = _kv8_check("paged_prefill8", qkv, kv, pos, slot, btab, bs, H, hd, 0)
     if hd == 16:
         raise ValueError("paged_prefill8: head width 16 is not supported")
-    limit = min(qkv.shape[0], out.shape[0], pos.numel(), slot.numel())
-    if any(r < 0 or n < 1 or r + n > limit for r, n in runs):
+    limit, rows, lens = min(qkv.shape[0], out.shape[0], pos.numel(), slot.numel()), [r for r, _ in runs], [n for _, n in runs]
+    if rows and (min(rows) < 0 or min(lens) < 1 or max(map(operator.add, rows, lens)) > limit):
         raise ValueError("paged_prefill8: runs %s within %d rows" % (list(runs)[:8], limit))
     if _use_reference(qkv):
         for r, n in runs:
             ref.paged_attn8(qkv[r:r + n], kv, out[r:r + n], pos[r:r + n], slot[r:r + n], btab, bs, H, hd, n, max_ctx)
         return
-    _kv8_rows("paged_prefill8", qkv, 3 * H * hd, torch.bfloat16)
-    _kv8_rows("paged_prefill8", out, H * hd, torch.bfloat16)
-    if out.device != qkv.device:
+    x = _kv8_rows("paged_prefill8", qkv, 3 * H * hd, torch.bfloat16)
+    y = _kv8_rows("paged_prefill8", out, H * hd, torch.bfloat16)
+    if out.get_device() != qkv.get_device():
         raise ValueError("paged_prefill8: the tensors must be on one device, the current one")
-    rows, lens = _row_lists(runs, limit)
-    _call_keeping((rows, lens), _lib().kh_paged_prefill8, 1, qkv.data_ptr(), qkv.stride(0), kv.data_ptr(), kv.shape[0], kv.shape[2],
-                  out.data_ptr(), out.stride(0), pos.data_ptr(), slot.data_ptr(), btab.data_ptr(), btab.shape[0], btab.shape[1], bs, H, hd,
-                  1.0 / math.sqrt(hd), min(max_ctx, 0x7fffffff), C.addressof(rows), C.addressof(lens), len(runs), _stream())
+    n, keep = len(runs), array.array("i", rows + lens)
+    at = keep.buffer_info()[0]
+    _call_keeping(keep, _lib().kh_paged_prefill8, 1, *x, *cache, *y, *table, hd ** -0.5, min(max_ctx, 0x7fffffff), at, at + 4 * n, n, _stream())
 
 
 def copy_blocks8(kv, pairs, npairs):
@@ -708,7 +715,7 @@ def copy_blocks8(kv, pairs, npairs):
         for i in range(npairs):
             kv[:, int(pairs[2 * i + 1])].copy_(kv[:, int(pairs[2 * i])])
         return
-    if kv.get_device() != torch._C._cuda_getDevice():
+    if kv.get_device() != _current_device():
         raise ValueError("copy_blocks8: the tensors must be on the current device")
     _call(_lib().kh_copy_blocks8, 1, kv.data_ptr(), pairs.data_ptr(), npairs, kv.shape[0], kv.shape[1], kv.stride(1), kv.stride(0), _stream())
 
