@@ -262,9 +262,10 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
   __syncwarp();
   cluster_sync_all();                                                           // the others' parts are read until here
 #pragma unroll 1
-  for (int r = warp; r < n; r += 4)
-    if (s_again[r >> 5] >> (r & 31) & 1)
-      attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
+  for (uint32_t m = s_again[warp >> 1] >> (warp & 1) * 16 & 0xffffu; m; m &= m - 1) {
+    const int r = w0 + __ffs(m) - 1;
+    attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, scale, out + (size_t)(r0 + r) * ldo + h * HD);
+  }
 }
 
 // ------------------------------------------------------------------------------- runs of new tokens on tcgen05
@@ -287,24 +288,25 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 //   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
 // A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
 namespace {
-constexpr int CH_ROWS = 256, CH_MAX = 1024, CH_THREADS = 640;
+constexpr int CH_MAX = 1024;
 struct Runs { int row0[CH_MAX]; uint16_t n[CH_MAX]; };
 
-template <int HD>
+template <int HD, int G>
 struct Chunk {
+  static constexpr int GW = 4 * G, ROWS = 128 * G, THREADS = ROWS + 384;      // warps of the groups; query rows
   static constexpr int HP = HD < 64 ? 64 : HD;               // columns of a tile in shared memory (slabs of 64)
   static constexpr int TILE = 128 * HP * 2, NS = 2;
-  static constexpr int DATA = 2 * TILE + NS * 2 * TILE;      // Q of both groups, NS stages of K and V
+  static constexpr int DATA = G * TILE + NS * 2 * TILE;      // Q of the groups, NS stages of K and V
   static constexpr int PITCH = HD + 4;                       // floats per row of a group's O when it is shared
-  static constexpr int ML = DATA;                            // (R, normaliser) of 256 group rows
-  static constexpr int QE = ML + 256 * 8;                    // 2^eq of 256 rows
-  static constexpr int ADDR = QE + 256 * 4;                  // [K, V][2 tiles][128] addresses, then as many factors
+  static constexpr int ML = DATA;                            // (R, normaliser) of the groups' rows
+  static constexpr int QE = ML + ROWS * 8;                   // 2^eq of the rows
+  static constexpr int ADDR = QE + ROWS * 4;                 // [K, V][2 tiles][128] addresses, then as many factors
   static constexpr int FAC = ADDR + 2 * 2 * 128 * 8;
   static constexpr int WMAX = FAC + 2 * 2 * 128 * 4;            // [K, V][2 tiles][4 warps] largest exponents, of K and of V
   static constexpr int TMAX = WMAX + 2 * 2 * 4 * 4;          // [4 tiles] of the tile
   static constexpr int AGAIN = TMAX + 4 * 4;                 // rows to be done anew, as bits
   static constexpr int BARS = AGAIN + 8 * 4, SMEM = BARS + 8 * (4 * NS + 13) + 16;
-  static_assert(2 * 128 * PITCH * 4 <= DATA, "the shared O takes the tiles' place");
+  static_assert(G == 1 || ROWS * PITCH * 4 <= DATA, "the shared O takes the tiles' place");
 };
 __device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int row, int ch) {      // 16-byte chunk `ch` of a row of a [128 x HP] tile
   return base + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
@@ -379,14 +381,14 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int b_mn_major) {
 }
 }  // namespace
 
-template <int HD>
-__global__ void __launch_bounds__(CH_THREADS, 1)
+template <int HD, int G>
+__global__ void __launch_bounds__(Chunk<HD, G>::THREADS, G == 1 ? 2 : 1)
 paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restrict__ out, int ldo, float sl2, int max_ctx, int S) {
-  using C = Chunk<HD>;
-  constexpr int NS = C::NS;
+  using C = Chunk<HD, G>;
+  constexpr int NS = C::NS, GW = C::GW, COLS = G == 1 ? 256 : 512;     // TMEM: 128 columns of scores and HD of O a group
   extern __shared__ __align__(1024) uint8_t chunk_smem[];
   uint8_t* const smem = chunk_smem;
-  const uint32_t base = smem_u32(smem), sQ = base, sKV = base + 2 * C::TILE, b0 = base + C::BARS;
+  const uint32_t base = smem_u32(smem), sQ = base, sKV = base + G * C::TILE, b0 = base + C::BARS;
   const uint32_t bar_kfull = b0, bar_kfree = bar_kfull + 8 * NS, bar_vfull = bar_kfree + 8 * NS, bar_vfree = bar_vfull + 8 * NS, bar_s = bar_vfree + 8 * NS, bar_p = bar_s + 32, bar_pv = bar_p + 32, bar_o = bar_pv + 16, bar_q = bar_o + 16;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::BARS + 8 * (4 * NS + 13));
   volatile int* redo = abort_flag + 1;
@@ -394,7 +396,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + C::AGAIN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < 8) s_again[tid] = 0;
-  if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
+  if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), COLS); tmem_relinquish(); }
   pdl_wait();
   pdl_launch_dependents();
 
@@ -406,11 +408,12 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   // index guard: tokens beyond the limits are recorded (status code 8) and skipped; they are the last of the run
   const int ok = sl < 0 || sl >= c.n_slots || p0 < 0 ? 0 : (int)min((long)listed, min((long)max_ctx, (long)c.max_lb * c.bs) - p0);
   if (ok < listed && tid == 0 && rank == 0) report(c.err);
-  const int n = max(ok, 0), nq = n > 128 ? 2 : 1, ctx = p0 + n;
+  const int n = max(ok, 0), nq = G == 2 && n > 128 ? 2 : 1, ctx = p0 + n;
+  const bool apart = G == 1 || nq == 2;          // every group has rows of its own
   const int tiles = n > 0 ? (ctx + 127) >> 7 : 0, kt0 = (int)((long)tiles * rank / S), kt1 = (int)((long)tiles * (rank + 1) / S);
-  // tiles of group w: nq = 2: all, for the first rows maybe without the last one; nq = 1: every second
+  // tiles of group w: all, where it has its own rows (the first of two groups maybe without the last one); every second, where both have the same
   const int lim0 = min(kt1, (p0 + 128 + 127) >> 7);
-  auto tiles_of = [&](int w) { return nq == 2 ? max(0, (w ? kt1 : lim0) - kt0) : (kt1 - kt0 + 1 - w) >> 1; };
+  auto tiles_of = [&](int w) { return w >= G ? 0 : apart ? max(0, (w ? kt1 : lim0) - kt0) : (kt1 - kt0 + 1 - w) >> 1; };
   if (tid == 0) {
     // a stage is read by both groups, or by one of them: with NS = 2 and alternating tiles always by the same.  (The last tile may lack group 0:
     // nothing is fetched over it.)
@@ -420,7 +423,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       mbar_init(bar_vfull + 8 * s, 4); mbar_init(bar_vfree + 8 * s, nq);
     }
     for (int i = 0; i < 4; i++) { mbar_init(bar_s + 8 * i, 1); mbar_init(bar_p + 8 * i, 4); }      // [group][half]
-    mbar_init(bar_pv, 1); mbar_init(bar_pv + 8, 1); mbar_init(bar_o, 1); mbar_init(bar_o + 8, 1); mbar_init(bar_q, 8);
+    mbar_init(bar_pv, 1); mbar_init(bar_pv + 8, 1); mbar_init(bar_o, 1); mbar_init(bar_o + 8, 1); mbar_init(bar_q, GW);
     *redo = 0;
     *abort_flag = (base & 1023u) ? 6 : 0;         // swizzled tiles need the 1024-byte alignment
     if (base & 1023u) atomicCAS(c.err, 0, 6);
@@ -435,19 +438,20 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   bool dead = false;
   auto wait = [&](uint32_t bar, uint32_t parity) { if (!dead && !mbar_wait(bar, parity, abort_flag, 6, c.err)) dead = true; };
 
-  // 640 threads of 96 registers: 128 to the groups, 80 to the fetching warps, 64 to the rest.  What follows a role's loop stays in its branch.
-  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-  else if (warp < 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  // 640 threads of 96 registers: 128 to the groups, 80 to the fetching warps, 64 to the rest; 512 of 64: 128, 48 and 32.  What follows a role's loop
+  // stays in its branch.
+  if (warp < GW) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+  else if (warp < GW + 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G == 1 ? 48 : 80));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G == 1 ? 32 : 64));
 
-  if (warp >= 16) {
+  if (warp >= GW + 8) {
     // ------------------------------------------------------------------ MMA issuer
-    if (warp == 16 && live && elect_one()) {
+    if (warp == GW + 8 && live && elect_one()) {
       constexpr uint32_t idesc_s = idesc_f16(128, 64, 0), idesc_o = idesc_f16(128, HD, 1);
       const int tiles_w[2] = {tiles_of(0), tiles_of(1)};
       const uint32_t dq0 = (uint32_t)umma_desc_sw128(sQ, 16, 1024), dk0 = (uint32_t)umma_desc_sw128(sKV, 16, 1024), dv0 = (uint32_t)umma_desc_sw128(sKV + C::TILE, 16384, 1024);
       auto scores = [&](int w, int half, int t) {          // S of half a tile, the group's t-th
-        const int it = nq == 2 ? t : 2 * t + w, s = it & 1;
+        const int it = apart ? t : 2 * t + w, s = it & 1;
         if (half == 0) wait(bar_kfull + 8 * s, (it / NS) & 1);
         if (dead) return;
         tc_fence_after();
@@ -471,7 +475,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         for (int i = 0; i < 4; i++) {
           const int w = i & 1, half = i >> 1;
           if (t >= tiles_w[w]) continue;
-          const int it = nq == 2 ? t : 2 * t + w, s = it & 1;
+          const int it = apart ? t : 2 * t + w, s = it & 1;
           if (half == 0) wait(bar_vfull + 8 * s, (it / NS) & 1);
           wait(bar_p + 16 * w + 8 * half, t & 1);
           if (dead) continue;
@@ -479,20 +483,20 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
           const uint32_t dv = dv0 + s * (2 * C::TILE >> 4) + half * 512;
 #pragma unroll
           for (int kk = 0; kk < 4; kk++)
-            mma_f16_ts(tmem + 256 + w * HD, tmem + w * 128 + half * 64 + kk * 8, dv + (kk * 2048 >> 4), idesc_o, half > 0 || kk > 0 ? 1 : t > 0);
+            mma_f16_ts(tmem + 128 * G + w * HD, tmem + w * 128 + half * 64 + kk * 8, dv + (kk * 2048 >> 4), idesc_o, half > 0 || kk > 0 ? 1 : t > 0);
           umma_commit(half && t + 1 == tiles_w[w] ? bar_o + 8 * w : bar_pv + 8 * w);
           if (half) umma_commit(bar_vfree + 8 * s);
           if (t + 1 < tiles_w[w]) scores(w, half, t + 1);      // behind P V in the tensor core: these scores take P's place
         }
     }
     __syncwarp();
-    if (S > 1) { cluster_sync_all(); cluster_sync_all(); }
-  } else if (warp >= 8) {
-    // ------------------------------------------------------------------ codes -> f16 tiles: K by warps 8-11, V by warps 12-15
+    if (G == 2 && S > 1) { cluster_sync_all(); cluster_sync_all(); }
+  } else if (warp >= GW) {
+    // ------------------------------------------------------------------ codes -> f16 tiles: K by four warps, V by four
     // A lane takes 16 codes (two 16-byte chunks of a tile) at a time; LPR lanes cover a row of a slab, so eight lanes of a store lie in rows whose
     // numbers differ in the lowest bit, i.e. in eight bank groups.
     constexpr int LPR = HD < 64 ? HD / 16 : 4, RPP = 128 / LPR, SLABS = HD / (16 * LPR), NP = 128 / RPP * SLABS;
-    const int vr = warp >= 12, t = tid & 127, l = t % LPR, r1 = t / LPR, bs = c.bs;
+    const int vr = warp >= GW + 4, t = tid & 127, l = t % LPR, r1 = t / LPR, bs = c.bs;
     const uint32_t full = vr ? bar_vfull : bar_kfull, free = vr ? bar_vfree : bar_kfree;
     const int* bt = c.btab + (size_t)sl * c.max_lb;
     uint64_t* s_addr = reinterpret_cast<uint64_t*>(smem + C::ADDR) + vr * 256;
@@ -582,27 +586,27 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     }
     if (bad) report(c.err);
     __syncwarp();
-    if (S > 1) { cluster_sync_all(); cluster_sync_all(); }
+    if (G == 2 && S > 1) { cluster_sync_all(); cluster_sync_all(); }
   } else {
     // ------------------------------------------------------------------ query rows
     if (live) {
     const int w = warp >> 2, row = tid & 127, lrow = nq == 2 ? tid : row, qpos = p0 + lrow, wpos = qpos - lane;      // wpos: the warp's first row
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tO = tmem + 256 + w * HD + lanes;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tO = tmem + 128 * G + w * HD + lanes;
     const float* s_qe = reinterpret_cast<const float*>(smem + C::QE);
     const uint32_t* s_tmax = reinterpret_cast<const uint32_t*>(smem + C::TMAX);
     {
-      constexpr int LQ = HD / 8, NQ = LQ / 2;    // lanes per row of q; loads of a thread for 128 rows, all on their way together
+      constexpr int LQ = HD / 8, NQ = LQ / G;    // lanes per row of q; loads of a thread for 128 rows, all on their way together
 #pragma unroll 1
       for (int x = 0; x < nq; x++) {
         uint4 u[NQ];
 #pragma unroll
         for (int i = 0; i < NQ; i++) {
-          const int r = x * 128 + (tid + i * 256) / LQ;
+          const int r = x * 128 + (tid + i * C::ROWS) / LQ;
           u[i] = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + tid % LQ * 8) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < NQ; i++) {
-          const int r = (tid + i * 256) / LQ, ch = tid % LQ;
+          const int r = (tid + i * C::ROWS) / LQ, ch = tid % LQ;
           uint32_t m = amax8(u[i]);
 #pragma unroll
           for (int y = LQ / 2; y > 0; y >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
@@ -616,7 +620,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       }
     }
     fence_proxy_async_smem();
-    named_barrier<1, 256>();
+    named_barrier<1, C::ROWS>();
     if (lane == 0) mbar_arrive(bar_q);
     const float rq = sl2 * s_qe[lrow];
     float R = -INFINITY, l = 0.f;
@@ -624,7 +628,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     const int mine = tiles_of(w);
 #pragma unroll 1
     for (int cnt = 0; cnt < mine; cnt++) {
-      const int it = nq == 2 ? cnt : 2 * cnt + w, j = kt0 + it;
+      const int it = apart ? cnt : 2 * cnt + w, j = kt0 + it;
 #pragma unroll 1
       for (int half = 0; half < 2; half++) {
         const int k0 = j * 128 + half * 64;
@@ -713,13 +717,13 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
           *reinterpret_cast<uint4*>(part + q + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
     };
-    named_barrier<1, 256>();                     // no tile is read any more, and `redo` is written
-    if (S > 1) leave();
+    named_barrier<1, C::ROWS>();                     // no tile is read any more, and `redo` is written
+    if (G == 2 && S > 1) leave();
     else {
       float own = 1.f, other = 0.f, sum = den;   // weights of the group's sums and of the second group's for the same rows
-      if (nq == 1) {
+      if (!apart) {
         if (w == 1) leave();
-        named_barrier<1, 256>();
+        named_barrier<1, C::ROWS>();
         if (w == 0) {
           const float2 v = *reinterpret_cast<const float2*>(smem + C::ML + (128 + row) * 8);
           const float mx = fmaxf(R, v.x), ref = mx == -INFINITY ? 0.f : mx;
@@ -728,7 +732,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
           sum = fmaf(own, den, other * v.y);
         }
       }
-      if (nq == 2 || w == 0) {
+      if (apart || w == 0) {
         const bool intact = *abort_flag == 0 && lrow < n, all = *redo != 0;
         const float inv = 1.f / sum;
         const float* part = reinterpret_cast<const float*>(smem) + (128 + row) * C::PITCH;
@@ -740,7 +744,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
             uint32_t r[32], o[16];
             tmem_ld32(tO + q, r);
             tmem_ld_wait();
-            if (nq == 1)
+            if (!apart)
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float4 v = *reinterpret_cast<const float4*>(part + q + i);
@@ -763,8 +767,8 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     }
     }
   // ------------------------------------------------------------------ the cluster's CTAs join
-  if (S > 1) { __syncwarp(); cluster_sync_all(); }
-  if (live && S > 1) {
+  if (G == 2 && S > 1) { __syncwarp(); cluster_sync_all(); }
+  if (G == 2 && live && S > 1) {
     const int parts = nq == 2 ? S : 2 * S;       // of a row: part i is group i % 2 (or the row's own) of CTA i / 2 (or i)
     bool all = false;
     for (int i = 0; i < S; i++) {
@@ -808,18 +812,19 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       else *reinterpret_cast<uint2*>(out + (size_t)(r0 + r) * ldo + h * HD + ch * 4) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
     }
   }
-  if (S > 1) { __syncwarp(); cluster_sync_all(); }          // the others' parts are read until here
+  if (G == 2 && S > 1) { __syncwarp(); cluster_sync_all(); }          // the others' parts are read until here
   if (live) {                                    // (after the join: a row's other columns may have been stored)
-    named_barrier<1, 256>();
+    named_barrier<1, C::ROWS>();
 #pragma unroll 1
-    for (int r = warp; r < n; r += 8)
-      if (s_again[r >> 5] >> (r & 31) & 1)
-        attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, sl2, out + (size_t)(r0 + r) * ldo + h * HD);
+    for (uint32_t m = s_again[warp]; m; m &= m - 1) {      // (over the set bits: a turn costs some 140 cycles even where it does nothing)
+      const int r = warp * 32 + __ffs(m) - 1;
+      attend_row8<HD>(c, qkv + (size_t)(r0 + r) * ld + h * HD, h, p0 + r, sl, sl2, out + (size_t)(r0 + r) * ldo + h * HD);
+    }
   }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+  if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem, COLS); }
 }
 
 // Launch in clusters of S CTAs along x.
@@ -856,10 +861,10 @@ static int chunk_clusters(int S) {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = S; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(S * 148); cfg.blockDim = dim3(CH_THREADS); cfg.dynamicSmemBytes = Chunk<HD>::SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(S * 148); cfg.blockDim = dim3(Chunk<HD, 2>::THREADS); cfg.dynamicSmemBytes = Chunk<HD, 2>::SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
     int got = 0;
-    if (cudaFuncSetAttribute(paged_chunk8_k<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<HD>::SMEM) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&got, paged_chunk8_k<HD>, &cfg) != cudaSuccess || got < 1) {
+    if (cudaFuncSetAttribute(paged_chunk8_k<HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<HD, 2>::SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&got, paged_chunk8_k<HD, 2>, &cfg) != cudaSuccess || got < 1) {
       cudaGetLastError();
       got = -1;                                      // not available
     }
@@ -896,21 +901,29 @@ static int launch_runs(const Cache& c, const bf16* qkv, int ld, bf16* out, int l
       }
     if (flush()) return -1;
   }
+  // the largest cluster with which all items are on the chip at once and each CTA has two tiles of the longest context
+  long items = 0;
+  for (int i = 0; i < n_runs; i++) items += split_short && len[i] <= P8_ROWS ? 0 : (len[i] + 255) / 256;
+  items *= c.H;
+  int S = 8;
+  while (S > 1 && (items > chunk_clusters<HD>(S) || (max_ctx + 127) / 128 < 2 * S)) S /= 2;
+  const bool one = HD <= 64 && S == 1;
+  const int rows = one ? 128 : 256;
   Runs runs;
   auto flush = [&]() -> int {
     const int n = nt;
     nt = 0;
-    // the largest cluster with which all items are on the chip at once and each CTA has two tiles of the longest context
-    int S = 8;
-    while (S > 1 && ((long)n * c.H > chunk_clusters<HD>(S) || (max_ctx + 127) / 128 < 2 * S)) S /= 2;
-    return n ? launch_clusters(paged_chunk8_k<HD>, dim3((unsigned)n * c.H * S), CH_THREADS, Chunk<HD>::SMEM, S, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, S) : 0;
+    if (n == 0) return 0;
+    if constexpr (HD <= 64)
+      if (one) return launch_clusters(paged_chunk8_k<HD, 1>, dim3((unsigned)n * c.H), Chunk<HD, 1>::THREADS, Chunk<HD, 1>::SMEM, 1, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, 1);
+    return launch_clusters(paged_chunk8_k<HD, 2>, dim3((unsigned)n * c.H * S), Chunk<HD, 2>::THREADS, Chunk<HD, 2>::SMEM, S, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, S);
   };
   // the pieces that see the most keys first (as far as the lengths tell)
-  for (int at = (most - 1) / CH_ROWS * CH_ROWS; at >= 0; at -= CH_ROWS)
+  for (int at = (most - 1) / rows * rows; at >= 0; at -= rows)
     for (int i = 0; i < n_runs; i++) {
       if (len[i] <= at || (split_short && len[i] <= P8_ROWS)) continue;
       runs.row0[nt] = row0[i] + at;
-      runs.n[nt] = (uint16_t)(len[i] - at < CH_ROWS ? len[i] - at : CH_ROWS);
+      runs.n[nt] = (uint16_t)(len[i] - at < rows ? len[i] - at : rows);
       if (++nt == CH_MAX && flush()) return -1;
     }
   return flush();
