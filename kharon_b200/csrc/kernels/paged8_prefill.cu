@@ -17,6 +17,48 @@ __device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[N]) {
   else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory");
 }
 
+// Joins `parts` partial results of NR rows: (reference, normaliser) at ml, four columns of the sums at data, in the cluster's shared memory.  Four parts
+// of all rows are on their way together: a trip takes some 300 cycles.
+template <int NR, typename A>
+__device__ __forceinline__ void join_parts(int parts, A place, float (&den)[NR], float (&o)[NR][4]) {
+  float mx[NR];
+#pragma unroll
+  for (int k = 0; k < NR; k++) {
+    mx[k] = -INFINITY;
+    den[k] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[k][e] = 0.f;
+  }
+#pragma unroll 1
+  for (int i0 = 0; i0 < parts; i0 += 4) {
+    float v[NR][4][2], y[NR][4][4];
+#pragma unroll
+    for (int k = 0; k < NR; k++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t ml, data;
+        place(k, min(i0 + i, parts - 1), ml, data);
+        ld_cluster(ml, v[k][i]);
+        ld_cluster(data, y[k][i]);
+      }
+#pragma unroll
+    for (int k = 0; k < NR; k++) {
+      const float m = fmaxf(fmaxf(fmaxf(v[k][0][0], v[k][1][0]), fmaxf(v[k][2][0], v[k][3][0])), mx[k]), ref = m == -INFINITY ? 0.f : m, al = ex2(mx[k] - ref);
+      mx[k] = m;
+      den[k] *= al;
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[k][e] *= al;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float f = i0 + i < parts ? ex2(v[k][i][0] - ref) : 0.f;
+        den[k] = fmaf(f, v[k][i][1], den[k]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[k][e] = fmaf(f, y[k][i][e], o[k][e]);
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -233,25 +275,13 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
   const int ch = tid % TPR;
 #pragma unroll 1
   for (int r = rank + tid / TPR * S; r < n; r += 128 / TPR * S) {
-    float mx = -INFINITY, den = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = 0; i < S; i++) {
-      float v[2];
-      ld_cluster(mapa_shared(sK, i) + ML + r * 8, v);
-      mx = fmaxf(mx, v[0]);
-    }
-    const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll 4
-    for (int i = 0; i < S; i++) {
+    float dens[1], sums[1][4];
+    join_parts<1>(S, [&](int, int i, uint32_t& ml, uint32_t& data) {
       const uint32_t a = mapa_shared(sK, i);
-      float v[2], x[4];
-      ld_cluster(a + ML + r * 8, v);
-      ld_cluster(a + (r * OP + ch * 4) * 4, x);
-      const float f = ex2(v[0] - ref);
-      den = fmaf(f, v[1], den);
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = fmaf(f, x[e], y[e]);
-    }
+      ml = a + ML + r * 8;
+      data = a + (r * OP + ch * 4) * 4;
+    }, dens, sums);
+    const float den = dens[0], (&y)[4] = sums[0];
     const float inv = 1.f / den;
     bool anew = false;
 #pragma unroll
@@ -779,37 +809,28 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     // CTA `rank` joins rows rank, rank + S ...; a thread four columns of a row
     constexpr int TPR = HD / 4;
     const int ch = tid % TPR;
+    constexpr int NR = 2, STEP = 256 / TPR;
 #pragma unroll 1
-    for (int r = rank + tid / TPR * S; r < n; r += 256 / TPR * S) {
-      const int own = nq == 2 ? r : 0, row = r & 127;          // (nq = 2: the group's rows are r itself)
-      auto where = [&](int i) { return mapa_shared(base, nq == 2 ? i : i >> 1); };
-      auto line = [&](int i) { return nq == 2 ? own : (i & 1) * 128 + row; };
-      float mx = -INFINITY, den = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int i = 0; i < parts; i++) {
-        float v[2];
-        ld_cluster(where(i) + C::ML + line(i) * 8, v);
-        mx = fmaxf(mx, v[0]);
-      }
-      const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll 4
-      for (int i = 0; i < parts; i++) {
-        const uint32_t a = where(i);
-        float v[2], y[4];
-        ld_cluster(a + C::ML + line(i) * 8, v);
-        ld_cluster(a + (line(i) * C::PITCH + ch * 4) * 4, y);
-        const float f = ex2(v[0] - ref);
-        den = fmaf(f, v[1], den);
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = fmaf(f, y[e], o[e]);
-      }
-      const float inv = 1.f / den;
-      bool anew = all || !(den > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
-#pragma unroll
-      for (int e = 0; e < 4; e++) anew |= (__float_as_uint(o[e]) & 0x7fffffffu) >= 0x7f800000u;
+    for (int r1 = rank + tid / TPR * S; r1 < n; r1 += NR * STEP * S) {
+      float den[NR], o[NR][4];
+      join_parts<NR>(parts, [&](int k, int i, uint32_t& ml, uint32_t& data) {
+        const int r = min(r1 + k * STEP * S, n - 1), line = nq == 2 ? r : (i & 1) * 128 + (r & 127);
+        const uint32_t a = mapa_shared(base, nq == 2 ? i : i >> 1);
+        ml = a + C::ML + line * 8;
+        data = a + (line * C::PITCH + ch * 4) * 4;
+      }, den, o);
       if (*abort_flag) break;
-      if (anew) atomicOr(s_again + (r >> 5), 1u << (r & 31));
-      else *reinterpret_cast<uint2*>(out + (size_t)(r0 + r) * ldo + h * HD + ch * 4) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+#pragma unroll
+      for (int k = 0; k < NR; k++) {
+        const int r = r1 + k * STEP * S;
+        if (r >= n) break;
+        const float inv = 1.f / den[k];
+        bool anew = all || !(den[k] > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
+#pragma unroll
+        for (int e = 0; e < 4; e++) anew |= (__float_as_uint(o[k][e]) & 0x7fffffffu) >= 0x7f800000u;
+        if (anew) atomicOr(s_again + (r >> 5), 1u << (r & 31));
+        else *reinterpret_cast<uint2*>(out + (size_t)(r0 + r) * ldo + h * HD + ch * 4) = make_uint2(pack_bf16(o[k][0] * inv, o[k][1] * inv), pack_bf16(o[k][2] * inv, o[k][3] * inv));
+      }
     }
   }
   if (G == 2 && S > 1) { __syncwarp(); cluster_sync_all(); }          // the others' parts are read until here
