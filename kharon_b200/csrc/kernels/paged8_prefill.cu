@@ -922,13 +922,22 @@ static int launch_runs(const Cache& c, const bf16* qkv, int ld, bf16* out, int l
       }
     if (flush()) return -1;
   }
-  // the largest cluster with which all items are on the chip at once and each CTA has two tiles of the longest context
-  long items = 0;
-  for (int i = 0; i < n_runs; i++) items += split_short && len[i] <= P8_ROWS ? 0 : (len[i] + 255) / 256;
+  // Clusters where all their CTAs are on the chip at once: of eight from 24 key tiles, of four from 4, of two from 8 (8 heads, us in clusters of 1 / 2 / 4 / 8.
+  // Of 64: 384 fresh tokens 10.2 / 12.3 / 11.3 / -, 700 14.7 / 15.7 / 13.1 / -, 2048 31.7 / 27.0 / 29.6 / -, 100 behind 2000 24.7 / 18.0 / 14.6 / 15.0, behind
+  // 4000 42.6 / 26.8 / 18.7 / 16.8.  Of 128: 512 fresh 18.5 / 20.5 / 15.6 / -, 200 behind 14000 256 / 142 / 77 / 48).
+  long items = 0, halves = 0;                        // pieces of 256 and of 128 tokens
+  for (int i = 0; i < n_runs; i++)
+    if (!split_short || len[i] > P8_ROWS) { items += (len[i] + 255) / 256; halves += (len[i] + 127) / 128; }
   items *= c.H;
+  halves *= c.H;
+  const int kt = (max_ctx + 127) / 128;
   int S = 8;
-  while (S > 1 && (items > chunk_clusters<HD>(S) || (max_ctx + 127) / 128 < 2 * S)) S /= 2;
-  const bool one = HD <= 64 && S == 1;
+  while (S > 1 && (items > chunk_clusters<HD>(S) || kt < (S == 8 ? 24 : S == 4 ? 4 : 8))) S /= 2;
+  // Without a cluster, heads of up to 64: items of 128 tokens, two CTAs per SM, unless items of 256 fill the SMs in whole rounds (three quarters at least)
+  // and see more than three tiles: those fetch the keys once for twice the rows.  us, items of 128 / of 256, heads of 64: 1024 runs of 128 fresh tokens and heads 35.7 / 56.2,
+  // 320 of 300 20.9 / 28.6, 192 of 200 behind 500 positions 32.5 / 36.8, 128 of 150 behind 1000 29.1 / 25.6, 192 of 500 behind 4000 256 / 230.
+  const long rounds = (items + 147) / 148;
+  const bool one = HD <= 64 && S == 1 && (kt <= 3 || halves * 2 < 3 * 148 * rounds);
   const int rows = one ? 128 : 256;
   Runs runs;
   auto flush = [&]() -> int {
