@@ -1,4 +1,6 @@
 // Attention of runs of new tokens over the 8-bit paged cache (paged8.cu).
+#include <type_traits>
+
 #include "paged8.cuh"
 
 // ------------------------------------------------------------------------------- short runs
@@ -668,27 +670,83 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         tc_fence_after();
         const uint32_t ek = s_tmax[it & 3] & 0xffffu, ev = s_tmax[it & 3] >> 16;
         if (cnt == 0) eb = ev;
-        uint32_t pk[16];
-        if (k0 > wpos + 31) {                    // every key comes after the warp's queries
+        const float sl = rq * pow2_of(ek - 7), fev = (float)((int)ev - 127);
+        const f32x2 slv = mk2(sl, sl);
+        bool done = false;
+        // Optimistic: exponentials with the reference R as it stands, the next scores on their way; the largest score beside them.  Where that would have
+        // moved R (seldom after the first tile) what follows does it again.
+        auto optimistic = [&](auto masked) {
+          constexpr int W = 16;
+          const float c0 = fev - R;
+          const f32x2 c2 = mk2(c0, c0);
+          f32x2 rs0 = 0, rs1 = 0;
+          uint32_t r[2][W], pk[32];
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_ld16(tS, r[0]);
+#pragma unroll
+          for (int q = 0; q < 64 / W; q++) {
+            uint32_t (&x)[W] = r[q & 1];
+            tmem_ld_wait();
+            if (q + 1 < 64 / W) tmem_ld16(tS + (q + 1) * W, r[(q + 1) & 1]);
+            if constexpr (decltype(masked)::value) {
+#pragma unroll
+              for (int i = 0; i < W; i++)
+                if (k0 + q * W + i > qpos) x[i] = 0xff800000u;
+            }
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+              const f32x2 e0 = fma2(mk2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), slv, c2);
+              const f32x2 e1 = fma2(mk2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), slv, c2);
+              const f32x2 y0 = mk2(ex2(lo2(e0)), ex2(hi2(e0))), y1 = mk2(ex2(lo2(e1)), ex2(hi2(e1)));
+              mx[i & 4 ? 2 : 0] = max3(mx[i & 4 ? 2 : 0], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+              mx[i & 4 ? 3 : 1] = max3(mx[i & 4 ? 3 : 1], __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+              rs0 = add2(rs0, y0);
+              rs1 = add2(rs1, y1);
+              pk[(q * W + i) >> 1] = pack_f16(y0);
+              pk[((q * W + i) >> 1) + 1] = pack_f16(y1);
+            }
+          }
+          const float mt = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl, fev);
+          done = !__any_sync(0xffffffffu, mt > R + 8.f);
+          if (done) {
+            tmem_st16(tS, pk);                   // over the scores
+            tmem_st16(tS + 16, pk + 16);
+            l = fmaf((lo2(rs0) + hi2(rs0)) + (lo2(rs1) + hi2(rs1)), pow2_of(127 + eb - ev), l);
+          }
+        };
+        if (k0 <= wpos + 31 && !__any_sync(0xffffffffu, R == -INFINITY)) {
+          if (k0 + 63 <= wpos) optimistic(std::false_type{}); else optimistic(std::true_type{});
+        }
+        if (done) {
+        } else if (k0 > wpos + 31) {             // every key comes after the warp's queries
+          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) pk[i] = 0u;
           tmem_st16(tS, pk);
           tmem_st16(tS + 16, pk);
         } else {
-          uint32_t r[64];
-          tmem_ld32(tS, r);
-          tmem_ld32(tS + 32, r + 32);
-          tmem_ld_wait();
-          if (k0 + 63 > wpos) {                  // masks keys after the query
+          float mx = -INFINITY;
+          auto half_of = [&](int q, uint32_t (&r)[32]) {       // 32 scores, masked
+            tmem_ld32(tS + q * 32, r);
+            tmem_ld_wait();
+            if (k0 + q * 32 + 31 > wpos)         // masks keys after the query
 #pragma unroll
-            for (int i = 0; i < 64; i++)
-              if (k0 + i > qpos) r[i] = 0xff800000u;
+              for (int i = 0; i < 32; i++)
+                if (k0 + q * 32 + i > qpos) r[i] = 0xff800000u;
+          };
+#pragma unroll 1
+          for (int q = 0; q < 2; q++) {
+            uint32_t r[32];
+            half_of(q, r);
+            float m0 = mx, m1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              m0 = max3(m0, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+              m1 = max3(m1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+            }
+            mx = fmaxf(m0, m1);
           }
-          const float sl = rq * pow2_of(ek - 7), fev = (float)((int)ev - 127);
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-          const float mt = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl, fev);
+          const float mt = fmaf(mx, sl, fev);
           const bool grow = mt > R + 8.f;        // (from -inf too)
           if (__any_sync(0xffffffffu, grow)) {
             const float al = grow ? ex2(R - mt) : 1.f;
@@ -701,21 +759,23 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
             if (grow) R = mt;
           }
           const float c0 = fev - (R == -INFINITY ? 0.f : R);
-          const f32x2 c2 = mk2(c0, c0), slv = mk2(sl, sl);
+          const f32x2 c2 = mk2(c0, c0);
           f32x2 rs0 = 0, rs1 = 0;
-#pragma unroll
+#pragma unroll 1
           for (int q = 0; q < 2; q++) {
+            uint32_t r[32], pk[16];
+            half_of(q, r);
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const f32x2 e0 = fma2(mk2(__uint_as_float(r[q * 32 + i]), __uint_as_float(r[q * 32 + i + 1])), slv, c2);
-              const f32x2 e1 = fma2(mk2(__uint_as_float(r[q * 32 + i + 2]), __uint_as_float(r[q * 32 + i + 3])), slv, c2);
+              const f32x2 e0 = fma2(mk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), slv, c2);
+              const f32x2 e1 = fma2(mk2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), slv, c2);
               const f32x2 x0 = mk2(ex2(lo2(e0)), ex2(hi2(e0))), x1 = mk2(ex2(lo2(e1)), ex2(hi2(e1)));
               rs0 = add2(rs0, x0);
               rs1 = add2(rs1, x1);
               pk[i >> 1] = pack_f16(x0);
               pk[(i >> 1) + 1] = pack_f16(x1);
             }
-            tmem_st16(tS + q * 16, pk);          // over the scores
+            tmem_st16(tS + q * 16, pk);          // over scores that have been used
           }
           l = fmaf((lo2(rs0) + hi2(rs0)) + (lo2(rs1) + hi2(rs1)), pow2_of(127 + eb - ev), l);
         }
