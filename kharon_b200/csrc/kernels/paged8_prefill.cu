@@ -429,23 +429,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < 8) s_again[tid] = 0;
   if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), COLS); tmem_relinquish(); }
-  pdl_wait();
-  pdl_launch_dependents();
-
-  const int rank = (int)(blockIdx.x % S), item = (int)(blockIdx.x / S), h = item % c.H, piece = item / c.H;
-  // (What every thread knows alike goes through a shuffle, or *tmem_slot below: the compiler keeps it in uniform registers then, which is what
-  // tcgen05 instructions take.)
-  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
-  const int r0 = runs.row0[piece], p0 = uniform(c.pos[r0]), sl = uniform(c.slot[r0]), listed = runs.n[piece];
-  // index guard: tokens beyond the limits are recorded (status code 8) and skipped; they are the last of the run
-  const int ok = sl < 0 || sl >= c.n_slots || p0 < 0 ? 0 : (int)min((long)listed, min((long)max_ctx, (long)c.max_lb * c.bs) - p0);
-  if (ok < listed && tid == 0 && rank == 0) report(c.err);
-  const int n = max(ok, 0), nq = G == 2 && n > 128 ? 2 : 1, ctx = p0 + n;
+  // What needs no other kernel's results comes first: barriers, TMEM, the roles' registers.  (Grid: heads times S, pieces; S is a power of two.)
+  const int ls = 31 - __clz(S), rank = (int)blockIdx.x & (S - 1), h = (int)blockIdx.x >> ls, piece = (int)blockIdx.y;
+  const int r0 = runs.row0[piece], listed = runs.n[piece], nq = G == 2 && listed > 128 ? 2 : 1;
   const bool apart = G == 1 || nq == 2;          // every group has rows of its own
-  const int tiles = n > 0 ? (ctx + 127) >> 7 : 0, kt0 = (int)((long)tiles * rank / S), kt1 = (int)((long)tiles * (rank + 1) / S);
-  // tiles of group w: all, where it has its own rows (the first of two groups maybe without the last one); every second, where both have the same
-  const int lim0 = min(kt1, (p0 + 128 + 127) >> 7);
-  auto tiles_of = [&](int w) { return w >= G ? 0 : apart ? max(0, (w ? kt1 : lim0) - kt0) : (kt1 - kt0 + 1 - w) >> 1; };
   if (tid == 0) {
     // a stage is read by both groups, or by one of them: with NS = 2 and alternating tiles always by the same.  (The last tile may lack group 0:
     // nothing is fetched over it.)
@@ -464,8 +451,22 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // (What every thread knows alike goes through a shuffle: the compiler keeps it in uniform registers then, which is what tcgen05 instructions take.)
+  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
   const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
-  const bool live = *abort_flag == 0 && n > 0;
+  const bool aligned = *abort_flag == 0;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int p0 = uniform(c.pos[r0]), sl = uniform(c.slot[r0]);
+  // index guard: tokens beyond the limits are recorded (status code 8) and skipped; they are the last of the run
+  const int n = sl < 0 || sl >= c.n_slots || p0 < 0 ? 0 : max(0, min(listed, max_ctx - p0)), ctx = p0 + n;
+  if (n < listed && tid == 0 && rank == 0) report(c.err);
+  const int tiles = n > 0 ? (ctx + 127) >> 7 : 0, kt0 = tiles * rank >> ls, kt1 = tiles * (rank + 1) >> ls;
+  // tiles of group w: all, where it has its own rows (the first of two groups maybe without the last one); every second, where both have the same
+  const int lim0 = min(kt1, (p0 + 128 + 127) >> 7);
+  auto tiles_of = [&](int w) { return w >= G ? 0 : apart ? max(0, (w ? kt1 : lim0) - kt0) : (kt1 - kt0 + 1 - w) >> 1; };
+  const bool live = aligned && n > 0;
   // After a wait that ran out the roles go through their loops without waiting, so that the named barriers match and the kernel ends.
   bool dead = false;
   auto wait = [&](uint32_t bar, uint32_t parity) { if (!dead && !mbar_wait(bar, parity, abort_flag, 6, c.err)) dead = true; };
@@ -1005,8 +1006,8 @@ static int launch_runs(const Cache& c, const bf16* qkv, int ld, bf16* out, int l
     nt = 0;
     if (n == 0) return 0;
     if constexpr (HD <= 64)
-      if (one) return launch_clusters(paged_chunk8_k<HD, 1>, dim3((unsigned)n * c.H), Chunk<HD, 1>::THREADS, Chunk<HD, 1>::SMEM, 1, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, 1);
-    return launch_clusters(paged_chunk8_k<HD, 2>, dim3((unsigned)n * c.H * S), Chunk<HD, 2>::THREADS, Chunk<HD, 2>::SMEM, S, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, S);
+      if (one) return launch_clusters(paged_chunk8_k<HD, 1>, dim3((unsigned)c.H, n), Chunk<HD, 1>::THREADS, Chunk<HD, 1>::SMEM, 1, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, 1);
+    return launch_clusters(paged_chunk8_k<HD, 2>, dim3((unsigned)c.H * S, n), Chunk<HD, 2>::THREADS, Chunk<HD, 2>::SMEM, S, st, runs, c, qkv, ld, out, ldo, sl2, max_ctx, S);
   };
   // the pieces that see the most keys first (as far as the lengths tell)
   for (int at = (most - 1) / rows * rows; at >= 0; at -= rows)
