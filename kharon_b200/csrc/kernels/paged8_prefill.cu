@@ -430,7 +430,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   if (tid < 8) s_again[tid] = 0;
   if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), COLS); tmem_relinquish(); }
   // What needs no other kernel's results comes first: barriers, TMEM, the roles' registers.  (Grid: heads times S, pieces; S is a power of two.)
-  const int ls = 31 - __clz(S), rank = (int)blockIdx.x & (S - 1), h = (int)blockIdx.x >> ls, piece = (int)blockIdx.y;
+  // What every thread knows alike goes through a shuffle where the compiler is to keep it in uniform registers, which is what tcgen05 instructions take;
+  // h for the opposite reason: as a uniform value it made the inner loops spill (heads of 128: 276 us for 271).
+  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+  const int ls = 31 - __clz(S), rank = (int)blockIdx.x & (S - 1), h = uniform((int)blockIdx.x >> ls), piece = (int)blockIdx.y;
   const int r0 = runs.row0[piece], listed = runs.n[piece], nq = G == 2 && listed > 128 ? 2 : 1;
   const bool apart = G == 1 || nq == 2;          // every group has rows of its own
   if (tid == 0) {
@@ -451,10 +454,6 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // (What every thread knows alike goes through a shuffle: the compiler keeps it in uniform registers then, which is what tcgen05 instructions take.)
-  auto uniform = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
-  const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
-  const bool aligned = *abort_flag == 0;
   pdl_wait();
   pdl_launch_dependents();
 
@@ -466,7 +465,8 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   // tiles of group w: all, where it has its own rows (the first of two groups maybe without the last one); every second, where both have the same
   const int lim0 = min(kt1, (p0 + 128 + 127) >> 7);
   auto tiles_of = [&](int w) { return w >= G ? 0 : apart ? max(0, (w ? kt1 : lim0) - kt0) : (kt1 - kt0 + 1 - w) >> 1; };
-  const bool live = aligned && n > 0;
+  const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
+  const bool live = *abort_flag == 0 && n > 0;
   // After a wait that ran out the roles go through their loops without waiting, so that the named barriers match and the kernel ends.
   bool dead = false;
   auto wait = [&](uint32_t bar, uint32_t parity) { if (!dead && !mbar_wait(bar, parity, abort_flag, 6, c.err)) dead = true; };
