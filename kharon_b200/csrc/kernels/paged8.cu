@@ -14,7 +14,7 @@
 // ------------------------------------------------------------------------------- append and read back
 // A lane takes sixteen elements of a k row and of the v row beside it: HD / 16 lanes of a warp hold both and find their largest magnitudes with
 // shuffles; the exponents leave as one pair.  The lanes of a token (H HD / 16 of them) lie side by side; a CTA covers 256 of them, of several tokens
-// where one has fewer.  Bound by memory: 6018 tokens of 16 heads of 128 appended in 16.7 us (3.9 TB/s), 39800 positions read back in 74 us (5.8 TB/s).
+// where one has fewer.  Bound by memory: 6018 tokens of 16 heads of 128 appended in 17.0 us (3.9 TB/s), 39800 positions read back in 74.7 us (5.8 TB/s).
 // With k and v in different lanes (two byte stores for the exponents of a row) 23.6 and 132 us; two or four tokens a lane, fetched together: 16.7 and 80, 21.0 and 81.
 namespace {
 
@@ -150,7 +150,9 @@ extern "C" int kh_read_kv8(const void* kv, int n_blocks, int rec, void* k, void*
 // current ones in their registers as soon as those are used.
 // With `append` != 0 the item's first warp quantises the token's k and v, writes them into the cache and starts its sums with them.
 // The warps are merged once at the end: shared memory in warp order, then the cluster's shared memory in rank order (no scratch in global
-// memory, one launch).
+// memory, one launch).  Bound by memory for wide heads: 128 sequences of 1000 to 4096 positions, 16 heads of 128, 225 us (5.8 TB/s); by
+// issue slots and latency for narrower ones (128 sequences of 3000, 16 heads of 64: 148 us, 5.4 TB/s; of 32: 103 us, 3.9 TB/s); few items by three dependent trips to memory and
+// the join (16 heads of 64 at 16300 positions: 16 us, 2.1 TB/s).
 namespace {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

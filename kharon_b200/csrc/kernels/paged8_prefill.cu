@@ -7,8 +7,8 @@
 // CTA = (a run of up to 64 tokens, head), a warp per 16 tokens, mma.sync on K and V tiles of 64 positions that are turned into bf16 (exact) on
 // their way into shared memory; fp32 probabilities, which enter P V as three bf16 terms.  The key tiles are shared by the S CTAs of a cluster, in
 // contiguous ranges, where the runs leave SMs idle.  Bound by the trips to memory of a tile (some 1 us each): few instructions, small tiles and several
-// CTAs per SM, where the tcgen05 kernel below has 4 us more to set up (16 heads of 64, us, this / that: a fresh run of 16 3.1 / 7.1, of 64 3.6 / 7.7, thirty
-// of 64 8.2 / 30; thirty of 64 behind 200 positions 25 / 48).
+// CTAs per SM, where the tcgen05 kernel below has 2 us more to set up (16 heads of 64, us, this / that: a fresh run of 16 3.6 / 6.0, of 64 4.1 / 6.0, thirty of
+// 64 9.4 / 14.0).
 namespace {
 constexpr int P8_ROWS = 64, P8_MAX = 1024;
 struct Pieces { int row0[P8_MAX]; uint8_t n[P8_MAX]; };
@@ -301,12 +301,12 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 }
 
 // ------------------------------------------------------------------------------- runs of new tokens on tcgen05
-// A work item is (up to 256 consecutive tokens of a run, head).  Warps 0-3 and 4-7 are two groups of one thread per query row; warps 8-11 fetch the
-// codes of K, 128 positions at a time, through the block table and turn them into f16 tiles in the swizzled layout that the tensor core reads,
-// warps 12-15 those of V.  One lane of each group issues the group's products:
+// A work item is (up to 128 G consecutive tokens of a run, head): G = 2 groups of four warps, one thread per query row, or one group (heads of up to 64,
+// two CTAs per SM).  Four more warps fetch the codes of K, 128 positions at a time, through the block table and turn them into f16 tiles in the swizzled
+// layout that the tensor core reads, four those of V.  One lane issues the products, half a tile (64 positions) at a time:
 //   S_w = Q_w K_j^T -> TMEM;  group w: online softmax, P_w -> TMEM over S_w as f16;  O_w += P_w V_j in TMEM.
-// Items of more than 128 tokens: group w has query rows 128 w .. and every key tile.  Items of up to 128: both groups have the same rows and
-// alternate key tiles.  While one group works on its scores, the tensor core does the other's products.  The key tiles of an item are shared
+// One group, and two with more than 128 tokens: group w has query rows 128 w .. and every key tile.  Two groups, up to 128 tokens: both have the same
+// rows and alternate key tiles.  While one group works on its scores, the tensor core does the other's products.  The key tiles of an item are shared
 // by the S CTAs of a cluster, in contiguous ranges, where the items alone would leave SMs idle.  Groups and CTAs that share rows leave (reference,
 // normaliser, O) in shared memory and join them in a fixed order.
 //
@@ -319,6 +319,11 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 //   v' of positions whose exponent is more than 22 below the tile's largest: the item's rows are done anew, one by one, in fp32;
 //   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
 // A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
+//
+// Heads of 128 are bound by the tensor core (its operands' trips through shared memory) and the exponentials together, each two thirds of the
+// time on the SMs in use: 2048 tokens behind 14300 positions, 16 heads, 271 us (948 TFLOP/s; 128 items on 148 SMs), four turns of 384 to 640 tokens behind 1500 to 4000
+// 84 us (750).  Narrower heads are bound by the exponentials and by the latency of a tile's way through the roles: eight prompts of 1024 tokens, 16
+// heads of 64, 60.5 us (284 TFLOP/s); short prompts by an item's set-up, some 4 us: six of 403 to 1001 tokens 33 us, 1024 (run of 128, head) items 33 us.
 namespace {
 constexpr int CH_MAX = 1024;
 struct Runs { int row0[CH_MAX]; uint16_t n[CH_MAX]; };
@@ -956,24 +961,26 @@ static int chunk_clusters(int S) {
 }
 template <int HD>
 static int launch_runs(const Cache& c, const bf16* qkv, int ld, bf16* out, int ldo, float sl2, int max_ctx, const int* row0, const int* len, int n_runs, cudaStream_t st) {
-  // Runs of up to 64 tokens take the kernel of short runs, unless they are few and may lie behind long contexts, whose tiles of 64 positions are too many
-  // trips for it (16 heads of 64, one run of 32 behind 2000 positions, us: 46 / 13 in clusters of four; eight runs 52 / 39; at 500 14 / 10).
   int n_short = 0, most = 0;
   for (int i = 0; i < n_runs; i++) {
     if (row0[i] < 0 || len[i] < 1) { kh_set_error("paged_prefill8: run %d is empty", i); return -1; }
     n_short += len[i] <= P8_ROWS;
     most = len[i] > most ? len[i] : most;
   }
-  const bool split_short = max_ctx <= 1024 || (long)n_short * c.H > 2 * 148;
+  // Runs of up to 64 tokens take the kernel of short runs where a CTA has up to four tiles of the longest context, counting rounds of two CTAs per SM.  us, that kernel / the
+  // one below, 16 heads of 64: 30 fresh runs of 64 9.4 / 14.0, behind 200 positions 26.6 / 22.2; one of 32 behind 1000 9.3 / 10.1, behind 2000 12.8 / 11.9; 8 behind
+  // 500 16.9 / 12.4; 20 behind 2000 88 / 64 (heads of 128: 225 / 103).
+  const int tiles64 = (max_ctx + P8_ROWS - 1) / P8_ROWS;
+  int S_short = 1;                                   // two CTAs per SM, two tiles of the longest context for each
+  while (S_short < 8 && (long)n_short * c.H * S_short * 2 <= 2 * 148 && tiles64 >= 4 * S_short) S_short *= 2;
+  const bool split_short = (tiles64 + S_short - 1) / S_short * (((long)n_short * c.H * S_short + 295) / 296) <= 4;
   int nt = 0;
   if (split_short && n_short) {
     Pieces tiles;
     auto flush = [&]() -> int {
       const int n = nt;
       nt = 0;
-      int S = 1;                                     // two CTAs per SM, two tiles of the longest context for each
-      while (S < 8 && (long)n * c.H * S * 2 <= 2 * 148 && (max_ctx + P8_ROWS - 1) / P8_ROWS >= 4 * S) S *= 2;
-      return n ? launch_clusters(paged_short8_k<HD>, dim3((unsigned)n * S, c.H), 128, 2 * P8_ROWS * (HD * 2 + 16) + P8_ROWS * 8 + 16, S, st, tiles, c, qkv, ld, out, ldo, sl2, max_ctx, S) : 0;
+      return n ? launch_clusters(paged_short8_k<HD>, dim3((unsigned)n * S_short, c.H), 128, 2 * P8_ROWS * (HD * 2 + 16) + P8_ROWS * 8 + 16, S_short, st, tiles, c, qkv, ld, out, ldo, sl2, max_ctx, S_short) : 0;
     };
     for (int i = 0; i < n_runs; i++)
       if (len[i] <= P8_ROWS) {

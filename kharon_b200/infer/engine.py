@@ -38,8 +38,10 @@ class InferEngine:
     def __init__(self, model: GPT, block_size=16, n_blocks=None, max_tokens=None, max_seqs=33, use_graphs=True,
                  persistent_decode=None, attn_splits=None, flash_prefill=True, kv8=False):
         """``kv8``: keys and values are kept in 8 bits (``ops.append_kv8``): half the cache and half the bytes that attention over long contexts
-        reads, for values that are off by up to 2^-4.  Every token, prompts' too, attends to the cache as it is kept, so results do not
-        depend on how steps are composed.  Decode steps take the kernel chain (the persistent kernel reads a bf16 cache)."""
+        reads, for values that are off by up to 2^-4.  Every token, prompts' too, attends to the cache as it is kept, however steps are composed.
+        Decode steps take the kernel chain, the persistent kernel reads a bf16 cache: for long contexts and many sequences.  tok/s, bf16 / 8 bits:
+        L8 d2048, 3000 positions, G = 1 1144 / 1205, 32 7200 / 10530, with a shared prefix 64 19763 / 41032; L24 d1024, 128 to 384 positions, G = 8
+        17754 / 4916 (the chain), 32 30558 / 28649."""
         cfg = model.cfg
         self.model, self.cfg = model, cfg
         self.dev, self.dt = model.device, model.dtype
@@ -233,9 +235,9 @@ class InferEngine:
         ops.append_kv8(qkv, kv, pos, slot, *tail, ntok)
         runs, rest = self._runs
         if runs:
-            ops.paged_prefill8(qkv, kv, att, pos, slot, *tail, runs, self.cfg.seq)
+            ops.paged_prefill8(qkv, kv, att, pos, slot, *tail, runs, self._ctx8)
         for a, b in rest:
-            ops.paged_attn8(qkv[a:b], kv, att[a:b], pos[a:b], slot[a:b], *tail, b - a, self.cfg.seq)
+            ops.paged_attn8(qkv[a:b], kv, att[a:b], pos[a:b], slot[a:b], *tail, b - a, self._ctx8)
 
     def _lin(self, x, w, out, epi=ops.EPI_NONE, bias=None, aux=None):
         """Column-parallel / replicated linear layer: skinny kernel for decode-sized inputs."""
@@ -307,10 +309,13 @@ class InferEngine:
 
     def _runs8(self, ntok, nseq):
         """(runs, rest) of a step over the 8-bit cache: runs = [(first row, length)] of several consecutive positions of a sequence, rest = [(a, b)] the
-        row ranges between them."""
-        if ntok == nseq or self.hd == 16:              # (the run kernels take heads of 32 and more)
+        row ranges between them; the step's longest context is noted in ``_ctx8``."""
+        if ntok == nseq:
             return [], [(0, ntok)]
         pos = self.np_meta[self._o_pos:self._o_pos + ntok]
+        self._ctx8 = int(pos.max()) + 1
+        if self.hd == 16:                              # (the run kernels take heads of 32 and more)
+            return [], [(0, ntok)]
         slot = self.np_meta[self._o_slot:self._o_slot + ntok]
         cuts = (np.flatnonzero((slot[1:] != slot[:-1]) | (pos[1:] != pos[:-1] + 1)) + 1).tolist()
         runs, rest, at = [], [], 0
