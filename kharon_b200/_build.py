@@ -1,10 +1,11 @@
 """In-tree build of the native libraries.
 
-Two shared objects are produced under ``kharon_b200/_lib``:
+Three shared objects are produced under ``kharon_b200/_lib``:
 
 * ``libkharon_rt.so``   -- host runtime (C++17, g++), no CUDA dependency;
 * ``libkharon_cuda.so`` -- every CUDA kernel, compiled by nvcc for ``sm_100a`` only
-  (``-gencode arch=compute_100a,code=sm_100a``); cross-compiles without a GPU.
+  (``-gencode arch=compute_100a,code=sm_100a``); cross-compiles without a GPU;
+* ``kharon_bind.so``    -- Python extension (g++, torch's headers) through which small calls skip ctypes.
 
 Objects are rebuilt only when a source or header is newer than the object.  Run
 ``python -m kharon_b200._build`` to build everything; ``--verbose`` adds ``-Xptxas -v``.
@@ -101,7 +102,26 @@ def build_cuda(force: bool = False, verbose: bool = False) -> Path:
     return out
 
 
+def build_bind(force: bool = False) -> Path:
+    import sysconfig
+    import torch
+    LIB.mkdir(exist_ok=True)
+    out = LIB / "kharon_bind.so"
+    srcs = sorted((CSRC / "bind").glob("*.cpp"))
+    if force or _newer(srcs, out):
+        home = Path(torch.__file__).resolve().parent
+        cuda = Path(nvcc_path()).resolve().parent.parent
+        tmp = out.with_suffix(".so.tmp%d" % os.getpid())
+        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I%s" % (home / "include"),
+              "-I%s" % sysconfig.get_paths()["include"], "-I%s" % (cuda / "include"), "-o", str(tmp)] + [str(x) for x in srcs]
+             + ["-L%s" % (home / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+        os.replace(tmp, out)
+    return out
+
+
 def build_all(force: bool = False, verbose: bool = False):
+    build_bind(force)
     return build_runtime(force), build_cuda(force, verbose)
 
 

@@ -15,6 +15,7 @@ from . import _build
 _lock = threading.Lock()
 _rt = None
 _cuda = None
+_bind = None
 
 i32, i64, u32, u64, f32 = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float
 vp, cp = C.c_void_p, C.c_char_p
@@ -119,3 +120,23 @@ def cuda():
         _sigs.declare(lib)
         _cuda = lib
         return lib
+
+
+def bind():
+    """The Python extension for small calls, with the addresses of the kernel library's entry points."""
+    global _bind
+    if _bind is None:
+        lib = cuda()
+        with _lock:
+            if _bind is None:
+                import importlib.util
+                path = _build.LIB / "kharon_bind.so"
+                if not path.exists():
+                    path = _build.build_bind()
+                spec = importlib.util.spec_from_file_location("kharon_bind", str(path))
+                mod = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+                mod.set_entries(*(C.cast(getattr(lib, n), C.c_void_p).value
+                                  for n in ("kh_append_kv8", "kh_read_kv8", "kh_paged_attn8", "kh_paged_prefill8")))
+                _bind = mod
+    return _bind

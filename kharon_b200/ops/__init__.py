@@ -616,8 +616,7 @@ def kv8_record_bytes(bs, hd):
 
 
 def _kv8_check(name, x, kv, pos, slot, btab, bs, H, hd, ntok):
-    """Argument checks of the 8-bit cache's operators; positions, sequences and blocks are checked in the kernels (status code 8).  Every attribute of a
-    tensor is asked for once: these checks are most of what a small call costs.  Returns the cache's and the table's part of a native call's arguments:
+    """Argument checks of the 8-bit cache's operators; positions, sequences and blocks are checked in the kernels (status code 8).  Returns the cache's and the table's part of a native call's arguments:
     (cache, blocks, bytes of a record), (positions, sequences, table, its rows and columns, bs, H, hd)."""
     if hd not in KV8_HEAD_DIMS or bs < 1:
         raise ValueError("%s: head width %d (of %s) or block size %d is not supported" % (name, hd, KV8_HEAD_DIMS, bs))
@@ -643,9 +642,25 @@ def _kv8_rows(name, x, width, dtype):
     return x.data_ptr(), st[0]
 
 
+def _kv8_direct(t):
+    """The extension that checks and launches a plain call on GPU tensors by itself (a call from Python takes 4 us of the host's time instead of 11), or
+    None: CPU tensors, and calls that a ``LaunchPlan`` records.  What it does not take as it is goes the way below it."""
+    return _native.bind() if _recording is None and t.is_cuda else None
+
+
+def _kv8_done(rc):
+    """Result of a direct call: launched (counted), refused by the entry point (raises), or not taken."""
+    if rc:
+        _chk(rc - 1)
+    return rc
+
+
 def append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok):
     """``append_kv`` into the 8-bit cache: quantises k and v of each listed token (``qkv`` rows q | k | v) and stores them at their positions.
     Two tokens of one call must not share a position of a block."""
+    b = _kv8_direct(kv)
+    if b and _kv8_done(b.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)):
+        return
     cache, table = _kv8_check("append_kv8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
     if _use_reference(qkv):
         return ref.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok)
@@ -655,6 +670,9 @@ def append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, ntok):
 def read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok):
     """The inverse of ``append_kv8``: rows ``k``, ``v`` [ntok, H * hd] (bf16, which holds the stored values exactly, or fp32) of the listed
     positions, for handing a cached sequence on (another engine, another block size, a bf16 cache)."""
+    b = _kv8_direct(kv)
+    if b and _kv8_done(b.read_kv8(kv, k, v, pos, slot, btab, bs, H, hd, ntok)):
+        return
     cache, table = _kv8_check("read_kv8", k, kv, pos, slot, btab, bs, H, hd, ntok)
     dt = k.dtype
     if dt not in (torch.bfloat16, torch.float32) or v.get_device() != k.get_device() or v.shape[0] < ntok or v.stride() != k.stride():
@@ -671,6 +689,9 @@ def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=
     holds them.  ``append``: the kernel first quantises and stores each token's own k, v (valid when no two listed tokens belong to
     one sequence, i.e. decode steps); otherwise ``append_kv8`` must have run.  Few tokens over long contexts: the keys of a
     token are shared out to the thread blocks of a cluster; no workspace."""
+    b = _kv8_direct(kv)
+    if b and _kv8_done(b.paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append)):
+        return
     cache, table = _kv8_check("paged_attn8", qkv, kv, pos, slot, btab, bs, H, hd, ntok)
     if _use_reference(qkv):
         if append:
@@ -686,6 +707,9 @@ def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=
 def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
     """``paged_prefill`` over the 8-bit cache: ``paged_attn8`` for runs of consecutive positions of one sequence each,
     ``runs = [(first row, length), ...]``, whose K/V are in the cache already (``append_kv8``).  Head widths 32, 64 and 128."""
+    b = _kv8_direct(kv)
+    if b and _kv8_done(b.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx)):
+        return
     cache, table = _kv8_check("paged_prefill8", qkv, kv, pos, slot, btab, bs, H, hd, 0)
     if hd == 16:
         raise ValueError("paged_prefill8: head width 16 is not supported")

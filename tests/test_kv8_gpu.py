@@ -369,6 +369,39 @@ def test_infinite_queries_and_queries_near_the_types_ends(hd, bs):
     assert ops.error_word() == 0
 
 
+def test_direct_calls_recorded_ones_and_unusual_arguments_agree():
+    """Calls that the extension launches itself, the same calls recorded and replayed by a launch plan, and calls with arguments that it leaves to Python
+    (NumPy numbers, runs as a tuple): the same bits, and each counted as one launch."""
+    import numpy as np
+    H, hd, bs, n = 3, 64, 5, 90
+    kv, btab, pos, slot, qkv = make(4, [n], H, hd, bs, pad=8)
+    d = H * hd
+    new = lambda: torch.zeros(n, d, device=DEV, dtype=torch.bfloat16)
+
+    def calls(kv, outs, num=int, runs=list):
+        ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, num(n - 1))
+        ops.paged_attn8(qkv[n - 1:], kv, outs[0], pos[n - 1:], slot[n - 1:], btab, bs, H, hd, num(1), num(n), append=True)
+        ops.paged_prefill8(qkv, kv, outs[1], pos, slot, btab, bs, H, hd, runs([(0, 20), (20, 70)]), num(n))
+        ops.read_kv8(kv, outs[2], outs[3], pos, slot, btab, bs, H, hd, num(n))
+    results = []
+    for kw in ({}, dict(num=np.int64), dict(runs=tuple)):
+        c, outs = kv.clone(), [new() for _ in range(4)]
+        before = ops.launch_count
+        calls(c, outs, **kw)
+        assert ops.launch_count == before + 4
+        results.append([c] + outs)
+    c, outs, plan = kv.clone(), [new() for _ in range(4)], ops.LaunchPlan()
+    with plan.record():
+        calls(c, outs)
+    for t in [c] + outs:
+        t.zero_()
+    plan.replay()
+    results.append([c] + outs)
+    for r in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(results[0], r))
+    assert bool(results[0][1][0].abs().max() > 0) and ops.error_word() == 0
+
+
 def test_limits_beyond_the_table_and_calls_without_work():
     H, hd, bs = 2, 64, 16
     kv, btab, pos, slot, qkv = make(3, [40], H, hd, bs)
