@@ -633,28 +633,25 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     const float* s_qe = reinterpret_cast<const float*>(smem + C::QE);
     const uint32_t* s_tmax = reinterpret_cast<const uint32_t*>(smem + C::TMAX);
     {
-      constexpr int LQ = HD / 8, NQ = LQ / G;    // lanes per row of q; loads of a thread for 128 rows, all on their way together
-#pragma unroll 1
-      for (int x = 0; x < nq; x++) {
-        uint4 u[NQ];
+      constexpr int LQ = HD / 8, NQ = LQ;        // lanes per row of q; loads of a thread, all on their way together
+      uint4 u[NQ];
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-          const int r = x * 128 + (tid + i * C::ROWS) / LQ;
-          u[i] = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + tid % LQ * 8) : make_uint4(0, 0, 0, 0);
-        }
+      for (int i = 0; i < NQ; i++) {
+        const int r = (tid + i * C::ROWS) / LQ;
+        u[i] = r < n ? *reinterpret_cast<const uint4*>(qkv + (size_t)(r0 + r) * ld + h * HD + tid % LQ * 8) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-          const int r = (tid + i * C::ROWS) / LQ, ch = tid % LQ;
-          uint32_t m = amax8(u[i]);
+      for (int i = 0; i < NQ; i++) {
+        const int r = (tid + i * C::ROWS) / LQ, ch = tid % LQ;
+        uint32_t m = amax8(u[i]);
 #pragma unroll
-          for (int y = LQ / 2; y > 0; y >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
-          const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
-          const float f = pow2_of((uint32_t)(127 - eq));
-          const f32x2 f2 = mk2(f, f);
-          st_shared_16(tile_chunk(sQ + x * C::TILE, r, ch),
-                       make_uint4(pack_f16(mul2(un2(u[i].x), f2)), pack_f16(mul2(un2(u[i].y), f2)), pack_f16(mul2(un2(u[i].z), f2)), pack_f16(mul2(un2(u[i].w), f2))));
-          if (ch == 0) reinterpret_cast<float*>(smem + C::QE)[x * 128 + r] = pow2_of((uint32_t)(127 + eq));
-        }
+        for (int y = LQ / 2; y > 0; y >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
+        const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
+        const float f = pow2_of((uint32_t)(127 - eq));
+        const f32x2 f2 = mk2(f, f);
+        st_shared_16(tile_chunk(sQ + (r >> 7) * C::TILE, r & 127, ch),
+                     make_uint4(pack_f16(mul2(un2(u[i].x), f2)), pack_f16(mul2(un2(u[i].y), f2)), pack_f16(mul2(un2(u[i].z), f2)), pack_f16(mul2(un2(u[i].w), f2))));
+        if (ch == 0) reinterpret_cast<float*>(smem + C::QE)[r] = pow2_of((uint32_t)(127 + eq));
       }
     }
     fence_proxy_async_smem();
