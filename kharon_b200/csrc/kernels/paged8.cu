@@ -14,8 +14,9 @@
 // ------------------------------------------------------------------------------- append and read back
 // A lane takes sixteen elements of a k row and of the v row beside it: HD / 16 lanes of a warp hold both and find their largest magnitudes with
 // shuffles; the exponents leave as one pair.  The lanes of a token (H HD / 16 of them) lie side by side; a CTA covers 256 of them, of several tokens
-// where one has fewer.  Bound by memory: 6018 tokens of 16 heads of 128 appended in 17.0 us (3.9 TB/s), 39800 positions read back in 74.7 us (5.8 TB/s).
-// With k and v in different lanes (two byte stores for the exponents of a row) 23.6 and 132 us; two or four tokens a lane, fetched together: 16.7 and 80, 21.0 and 81.
+// where one has fewer.  Bound by memory: 6018 tokens of 16 heads of 128 appended in 14.6 us (4.5 TB/s), 39800 positions read back in 74.7 us (5.8 TB/s).
+// With k and v in different lanes (two byte stores for the exponents of a row) 23.6 and 132 us; the largest magnitude element by element instead of by packed
+// maxima 17.0; then two or four tokens a lane, fetched together: 16.7 and 80, 21.0 and 81.
 namespace {
 
 struct Lanes { int per, tpc; };                      // lanes of a token; tokens side by side in a CTA

@@ -35,16 +35,16 @@ __device__ __forceinline__ int block_of(const Cache& c, int sl, int p) {
   return (unsigned)b < (unsigned)c.n_blocks ? b : -1;
 }
 
-// largest magnitude of eight bf16, as its bits; NaN counts as nothing
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// largest magnitude of eight bf16, as its bits; NaN counts as nothing (max gives the other operand, and NaN for two)
 __device__ __forceinline__ uint32_t amax8(const uint4& u) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint32_t a = w[i] & 0x7fffu, b = w[i] >> 16 & 0x7fffu;
-    m = max(m, max(a > 0x7f80u ? 0u : a, b > 0x7f80u ? 0u : b));
-  }
-  return m;
+  constexpr uint32_t M = 0x7fff7fffu;
+  const uint32_t m = max_bf16x2(max_bf16x2(u.x & M, u.y & M), max_bf16x2(u.z & M, u.w & M)), a = m & 0xffffu, b = m >> 16;
+  return max(a > 0x7f80u ? 0u : a, b > 0x7f80u ? 0u : b);
 }
 // exponent byte of a row whose largest magnitude has these bf16 bits: 448 = 1.75 * 2^8
 __device__ __forceinline__ uint32_t exp_byte(uint32_t a) {
