@@ -187,6 +187,34 @@ def test_scales_far_apart_and_scores_far_apart(hd):
     assert ops.error_word() == 0
 
 
+@pytest.mark.parametrize("hd,H,lens", [(32, 6, [384]), (64, 6, [384, 200]), (64, 12, [600, 600, 600, 600]), (32, 12, [600, 600, 600, 600]), (128, 6, [384]), (128, 12, [600, 600, 600, 600]),
+                                       (64, 6, [900]), (128, 6, [900])])
+def test_scores_that_rise_fall_and_jump_along_the_context(hd, H, lens):
+    """The running maximum moves in every tile, in none after the first, or in some rows of a warp alone; by one CTA for all keys and by clusters."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd + H, lens, H, hd, bs)
+    n, d, g = len(pos), H * hd, torch.Generator().manual_seed(hd)
+    j = pos.cpu().float()
+    for h in range(H):
+        u = torch.randint(0, 2, (hd,), generator=g) * 2.0 - 1
+        level = {0: 0.3 * j, 1: -0.3 * j, 2: (j % 97) * 0.8, 3: 60.0 * (j == 333), 4: 40.0 * (j // 64 % 2), 5: 0.0 * j}[h % 6]      # of a score, in log2 units
+        q = 0.5 * u + 0.02 * torch.randn(n, hd, generator=g)
+        q[(j % 8 == 3) & (h % 6 > 1)] *= -1                       # rows for which the jumps go down
+        qkv[:, h * hd:(h + 1) * hd] = q.bfloat16().to(DEV)
+        qkv[:, d + h * hd:d + (h + 1) * hd] = (level[:, None] / (0.5 * math.sqrt(hd) * 1.4427) * u + 0.1 * torch.randn(n, hd, generator=g)).bfloat16().to(DEV)
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one, at, runs = torch.zeros(n, d, device=DEV, dtype=torch.bfloat16), torch.zeros(n, d, device=DEV, dtype=torch.bfloat16), 0, []
+    for m in lens:
+        runs.append((at, m))
+        at += m
+    ops.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max(lens))
+    ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, n, max(lens))
+    rows = [0, 63, 64, 127, 128, 131, 191, lens[0] - 6, lens[0] - 1, n - 1]
+    check_rows(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, p_half_step=2.0 ** -8)
+    check_rows(one, qkv, kv, btab, bs, H, hd, pos, slot, rows)
+    assert ((out.float() - one.float()).norm() / one.float().norm()).item() < 2 * 2.0 ** -8 and ops.error_word() == 0
+
+
 def test_indices_out_of_range_are_recorded_and_skipped():
     H, hd, bs, lens = 2, 64, 4, [10, 6]
     kv, btab, pos, slot, qkv = make(5, lens, H, hd, bs)
