@@ -393,11 +393,11 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
         for (int x = 0; x < 4; x++) o[t][x] *= al;
       R = tm;
     }
-    const float c0 = R == -INFINITY ? 0.f : 14.f - R;
+    const float ref = R == -INFINITY ? 0.f : R;      // (the difference before the 14: of large scores 14 - R is off by whole numbers, and P' would pass f16's end)
     uint32_t pb[4];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      const float p0 = ex2(s[2 * x] + c0), p1 = ex2(s[2 * x + 1] + c0);
+      const float p0 = ex2(s[2 * x] - ref + 14.f), p1 = ex2(s[2 * x + 1] - ref + 14.f);
       l = fmaf(p0, nev[2 * x], fmaf(p1, nev[2 * x + 1], l));
       const uint32_t hi = pack_f16(p0, p1);
       const f32x2 hf = f32x2_of(hi);

@@ -1,0 +1,43 @@
+"""The 8-bit cache's attention where queries, keys or values differ widely in size, against 64 bits with a bound for each key's own terms."""
+import math
+
+import pytest
+import torch
+
+from kharon_b200 import ops
+from kv8_exact import attend_own, rows_of
+from test_kv8_gpu import make
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+# Rounding of the probabilities in runs of more than 64 tokens: half a step of 11 bits; half the smallest step is 2^-32 of the largest probability times 2^(difference of two
+# value rows' exponents), 14 at most.  Single tokens: two such terms, 2^-39 and the same difference.
+RUN, RUN_FLOOR, ONE_FLOOR = 2.0 ** -12, 2.0 ** -18, 2.0 ** -25
+
+
+def check(out, q, kv, btab, bs, H, hd, pos, slot, rows, p_half_step, floor):
+    kv, btab, pos, slot, q, out = kv.cpu(), btab.cpu(), pos.cpu(), slot.cpu(), q.double().cpu(), out.double().cpu()
+    cache = {}
+    for t in rows:
+        s, n = int(slot[t]), int(pos[t]) + 1
+        if s not in cache:
+            cache[s] = rows_of(kv, btab[s], bs, hd, max(int(pos[u]) + 1 for u in rows if int(slot[u]) == s))
+        want, tol = attend_own(q[t, :H * hd].view(H, hd), cache[s][0][:n], cache[s][1][:n], p_half_step, floor)
+        err = (out[t, :H * hd].view(H, hd) - want).abs()
+        assert not bool(want.isnan().any()) and bool((err <= tol).all()), (t, n, float((err / tol).nan_to_num(1e30).max()))
+
+
+@pytest.mark.parametrize("hd,H,lens", [(16, 2, [90]), (32, 2, [300]), (64, 2, [40, 700]), (128, 2, [300])])
+@pytest.mark.parametrize("power", [22, 25, 30, 45, 60])
+def test_scores_beyond_the_integers_of_fp32(hd, H, lens, power):
+    """Scores of some 2^power, where neighbouring numbers of fp32 are more than one apart: one position has all the weight, and no probability is out of range."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd + power, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, d:2 * d] *= 2.0 ** power
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    rows = list(range(0, n, 7)) + [n - 1]
+    one = torch.zeros(n, d, device=DEV, dtype=torch.bfloat16)
+    ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, n, max(lens))
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
+    assert ops.error_word() == 0
