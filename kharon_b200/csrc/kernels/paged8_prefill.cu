@@ -315,7 +315,9 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 //   q = q' 2^eq (row; largest |q'| in [2^14, 2^15)),  k = k' 2^(EK - 7),  v = v' 2^(EV - 7)  with EK, EV the tile's largest exponents,
 //   P' = 2^(s + EV - R),  O = sum P' v' = 2^(7 - R) sum 2^s v,  l = sum over tiles of 2^(EB - EV) sum P' = 2^(EB - R) sum 2^s,
 // where R is the row's running maximum of (largest score + EV), in log2 units, and EB the first tile's EV.  What f16 rounds:
-//   q', k' below 2^-14: off by 2^-25, a score by less than fp32's own rounding of its largest terms;
+//   q', k' below 2^-14: off by 2^-25, and by up to 448 * 2^-25 where a key's exponent is more than 31 below the tile's largest: a score by at most HD times
+//   q' times that.  From 22 below on (until there k' is exact) the fetching warps note the tile's exponent, and rows for which that bound is more than
+//   2^-12 of a log2 unit are done anew in fp32 (typical sizes stay 11 octaves below it, so keys of nearly nothing cost nothing);
 //   v' of positions whose exponent is more than 22 below the tile's largest: the item's rows are done anew, one by one, in fp32;
 //   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
 // A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
@@ -428,7 +430,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   const uint32_t base = smem_u32(smem), sQ = base, sKV = base + G * C::TILE, b0 = base + C::BARS;
   const uint32_t bar_kfull = b0, bar_kfree = bar_kfull + 8 * NS, bar_vfull = bar_kfree + 8 * NS, bar_vfree = bar_vfull + 8 * NS, bar_s = bar_vfree + 8 * NS, bar_p = bar_s + 32, bar_pv = bar_p + 32, bar_o = bar_pv + 16, bar_q = bar_o + 16;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::BARS + 8 * (4 * NS + 13));
-  volatile int* redo = abort_flag + 1;
+  // Rows to be done anew: none (0), all, or those whose q is large beside the keys of a tile with this largest exponent byte (see above).
+  constexpr int REDO_ALL = 256;
+  int* redo = const_cast<int*>(abort_flag) + 1;
+  auto lost = [](int redo, float rq) { return redo >= REDO_ALL || (redo && !(rq * pow2_of(redo - 7) * HD <= 0x1p-11f)); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (4 * NS + 13) + 8);
   uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + C::AGAIN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -579,7 +584,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       pair_barrier(4 + vr);
       const uint32_t tops = __vmaxu2(__vmaxu2(s_wmax[b * 4], s_wmax[b * 4 + 1]), __vmaxu2(s_wmax[b * 4 + 2], s_wmax[b * 4 + 3]));
       const int e = (int)(e_now >> 8 * vr & 0xffu), off = e - (int)(tops >> 16 * vr & 0xffffu);
-      if (vr && e > E_LO && off < -22) *redo = 1;
+      if (off < -22 && e > (vr ? E_LO : 0)) atomicMax(redo, vr ? REDO_ALL : (int)(tops & 0xffffu));      // (e: 0 past the end)
       s_fac[b * 128 + t] = f16_pow2(off + 7) * 0x10001u;
       // K's warps tell the groups both exponents: scores that are there have passed bar_kfull.  (Of four slots this one was last read for the tile
       // four before, whose scores both groups have used: K's stage of the tile two before this one has been freed.)
@@ -826,7 +831,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         }
       }
       if (apart || w == 0) {
-        const bool intact = *abort_flag == 0 && lrow < n, all = *redo != 0;
+        const bool intact = *abort_flag == 0 && lrow < n, all = lost(*redo, rq);
         const float inv = 1.f / sum;
         const float* part = reinterpret_cast<const float*>(smem) + (128 + row) * C::PITCH;
         bf16* dst = out + (size_t)(r0 + lrow) * ldo + h * HD;
@@ -863,11 +868,11 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   if (G == 2 && S > 1) { __syncwarp(); cluster_sync_all(); }
   if (G == 2 && live && S > 1) {
     const int parts = nq == 2 ? S : 2 * S;       // of a row: part i is group i % 2 (or the row's own) of CTA i / 2 (or i)
-    bool all = false;
+    int noted = 0;
     for (int i = 0; i < S; i++) {
       float v[1];
-      ld_cluster(mapa_shared(smem_u32((const void*)redo), i), v);
-      all |= __float_as_uint(v[0]) != 0;
+      ld_cluster(mapa_shared(smem_u32(redo), i), v);
+      noted = max(noted, __float_as_int(v[0]));
     }
     // CTA `rank` joins rows rank, rank + S ...; a thread four columns of a row
     constexpr int TPR = HD / 4;
@@ -888,7 +893,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         const int r = r1 + k * STEP * S;
         if (r >= n) break;
         const float inv = 1.f / den[k];
-        bool anew = all || !(den[k] > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
+        bool anew = lost(noted, sl2 * reinterpret_cast<const float*>(smem + C::QE)[r]) || !(den[k] > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
 #pragma unroll
         for (int e = 0; e < 4; e++) anew |= (__float_as_uint(o[k][e]) & 0x7fffffffu) >= 0x7f800000u;
         if (anew) atomicOr(s_again + (r >> 5), 1u << (r & 31));

@@ -27,6 +27,23 @@ def check(out, q, kv, btab, bs, H, hd, pos, slot, rows, p_half_step, floor):
         assert not bool(want.isnan().any()) and bool((err <= tol).all()), (t, n, float((err / tol).nan_to_num(1e30).max()))
 
 
+def both(qkv, kv, pos, slot, btab, bs, H, hd, lens):
+    """(runs, single tokens) of all rows."""
+    out, one, at, runs = torch.zeros(len(pos), H * hd, device=DEV, dtype=torch.bfloat16), torch.zeros(len(pos), H * hd, device=DEV, dtype=torch.bfloat16), 0, []
+    for n in lens:
+        runs.append((at, n))
+        at += n
+    ops.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max(lens))
+    ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, len(pos), max(lens))
+    torch.cuda.synchronize()
+    assert ops.error_word() == 0
+    return out, one
+
+
+# (head width, heads, lengths): one group of rows, two groups with rows of their own, clusters with shared and with own rows
+SHAPES = [(32, 2, [300]), (64, 2, [300]), (128, 2, [300]), (32, 2, [700]), (64, 2, [100, 700]), (128, 2, [700]), (128, 2, [520, 100]), (64, 12, [600, 600, 600, 600]), (128, 12, [600, 600, 600, 600])]
+
+
 @pytest.mark.parametrize("hd,H,lens", [(16, 2, [90]), (32, 2, [300]), (64, 2, [40, 700]), (128, 2, [300])])
 @pytest.mark.parametrize("power", [22, 25, 30, 45, 60])
 def test_scores_beyond_the_integers_of_fp32(hd, H, lens, power):
@@ -41,3 +58,21 @@ def test_scores_beyond_the_integers_of_fp32(hd, H, lens, power):
     ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, n, max(lens))
     check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
     assert ops.error_word() == 0
+
+
+@pytest.mark.parametrize("hd,H,lens", SHAPES)
+@pytest.mark.parametrize("power", [24, 30, 34, 70, 200])
+def test_one_key_far_larger_than_the_others(hd, H, lens, power):
+    """A key 2^power times the others (2^200: infinite) is as good as absent for the rows before it and for those whose product with it is negative; the others see
+    it alone.  Its neighbours in a tile keep their own scores."""
+    bs, at = 16, (40, 141)
+    kv, btab, pos, slot, qkv = make(hd + power, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    for j in at:
+        m = pos == j
+        qkv[m, d:2 * d] = (qkv[m, d:2 * d].double() * 2.0 ** power).to(torch.bfloat16)
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+    rows = [0, 30, 39, 40, 41, 45, 99, 140, 141, 142, 150, 155, 200, lens[0] - 1, n - 1] if lens[0] > 200 else [5, 39, 40, 60, 99, 100 + 140, 100 + 141, 100 + 150, 100 + 155, 100 + 400, n - 1]
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, RUN_FLOOR)
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
