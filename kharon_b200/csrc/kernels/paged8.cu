@@ -264,7 +264,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
       }
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
+    const int eq = q_exponent(m);
     qf = pow2_of((uint32_t)(127 - eq));
     sc = scale * pow2_of((uint32_t)(127 + eq));
 #pragma unroll

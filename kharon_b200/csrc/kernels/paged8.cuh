@@ -51,6 +51,9 @@ __device__ __forceinline__ uint32_t exp_byte(uint32_t a) {
   const int b = (int)(a >> 7) - 8 + ((a & 0x7fu) > 0x60u);
   return (uint32_t)min(max(b, E_LO), E_HI);
 }
+// eq of a query row whose largest magnitude has these bf16 bits: q = q' 2^eq with the largest |q'| in [2^14, 2^15).  Both 2^eq and 2^-eq are normal numbers; queries that
+// the limit leaves smaller (below 2^-98) have scores below 2^-19 beside any key that the format holds.
+__device__ __forceinline__ int q_exponent(uint32_t m) { return m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -112); }
 __device__ __forceinline__ float pow2_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
   uint16_t r;

@@ -651,7 +651,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         uint32_t m = amax8(u[i]);
 #pragma unroll
         for (int y = LQ / 2; y > 0; y >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
-        const int eq = m == 0 ? 0 : max((int)(m >> 7) - 127 - 14, -48);
+        const int eq = q_exponent(m);
         const float f = pow2_of((uint32_t)(127 - eq));
         const f32x2 f2 = mk2(f, f);
         st_shared_16(tile_chunk(sQ + (r >> 7) * C::TILE, r & 127, ch),

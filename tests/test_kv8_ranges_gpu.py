@@ -76,3 +76,24 @@ def test_one_key_far_larger_than_the_others(hd, H, lens, power):
     rows = [0, 30, 39, 40, 41, 45, 99, 140, 141, 142, 150, 155, 200, lens[0] - 1, n - 1] if lens[0] > 200 else [5, 39, 40, 60, 99, 100 + 140, 100 + 141, 100 + 150, 100 + 155, 100 + 400, n - 1]
     check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, RUN_FLOOR)
     check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
+
+
+@pytest.mark.parametrize("hd,H,lens", [(16, 2, [90]), (32, 2, [300]), (64, 2, [40, 700]), (128, 2, [300])])
+@pytest.mark.parametrize("power", [50, 62, 66, 70])
+def test_small_queries_beside_large_keys(hd, H, lens, power):
+    """Queries of 2^-power and keys of 2^power give ordinary scores."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd + power, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, :d] *= 2.0 ** -power
+    qkv[:, d:2 * d] *= 2.0 ** power / 4
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    rows = [0, 1, 39, 41, 80, n - 40, n - 1]
+    if hd > 16:
+        out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+        check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, RUN_FLOOR)
+    else:
+        one = torch.zeros(n, d, device=DEV, dtype=torch.bfloat16)
+        ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, n, max(lens))
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
+
