@@ -317,7 +317,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
     }
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    R = fmaf(s * sc, pow2_of(ek), (float)((int)ev - 127));
+    R = fmaf(s, sc * pow2_of(ek), (float)((int)ev - 127));
     l = g == 0 ? 16384.f * fv : 0.f;
     if (R == -INFINITY) {                          // (an infinity in q: the position has no weight ..
       l = 0.f;
@@ -366,7 +366,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
 #pragma unroll
     for (int q = 0; q < 4; q++) {
       const uint32_t x = __shfl_sync(0xffffffffu, e, q * 8 + g), ev = x >> 8;
-      s[q] = fmaf(s[q] * sc, pow2_of(x & 0xffu), (float)((int)ev - 127));
+      s[q] = fmaf(s[q], sc * pow2_of(x & 0xffu), (float)((int)ev - 127));      // (both powers first: of opposite size they meet)
       nev[q] = pow2_of(254u - ev);
     }
     if (j0 + 32 > n) {                             // the last chunk: scores past the end are -inf, values zero (a NaN there would count)

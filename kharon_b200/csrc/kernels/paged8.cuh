@@ -102,13 +102,14 @@ namespace {
 template <int HD>
 __device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int h, int p, int sl, float scale, bf16* dst) {
   constexpr int LPK = HD / 16, KPW = 32 / LPK;
+  constexpr float DOWN = 0x1p-24f, UP = 0x1p24f;   // q 2^-24: a sum of codes times the largest q stays finite
   const int lane = threadIdx.x & 31, g = lane / LPK, e0 = lane % LPK * 16, bs = c.bs;
   f32x2 q[8], o[8];
   {
     const uint4 u0 = *reinterpret_cast<const uint4*>(row + e0), u1 = *reinterpret_cast<const uint4*>(row + e0 + 8);
     const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-    for (int i = 0; i < 8; i++) { q[i] = mul2(un2(w[i]), mk2(scale, scale)); o[i] = 0; }
+    for (int i = 0; i < 8; i++) { q[i] = mul2(un2(w[i]), mk2(scale * DOWN, scale * DOWN)); o[i] = 0; }
   }
   float m = -INFINITY, l = 0.f;
 #pragma unroll 1
@@ -125,7 +126,7 @@ __device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int
 #pragma unroll
     for (int x = LPK / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     if (j <= p) {
-      s *= pow2_of(e & 0xffu);
+      s *= pow2_of(e & 0xffu) * UP;
       const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn, sc = ex2(m - ref), pr = ex2(s - ref), pv = pr * pow2_of(e >> 8);
       m = mn;
       l = fmaf(l, sc, pr);

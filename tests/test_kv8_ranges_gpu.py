@@ -97,3 +97,29 @@ def test_small_queries_beside_large_keys(hd, H, lens, power):
         ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, n, max(lens))
     check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
 
+
+
+@pytest.mark.parametrize("hd,H,lens", [(16, 2, [90]), (32, 2, [300]), (64, 2, [40, 700]), (128, 2, [300])])
+def test_queries_near_the_types_end_beside_small_keys(hd, H, lens):
+    """Queries of 3e37 and keys of 1e-17: scores of some 1e20, finite, and one position has all the weight."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, :d] *= 3e37
+    qkv[:, d:2 * d] *= 1e-17
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    rows = [0, 1, 39, 41, 80, n - 40, n - 1]
+    if hd > 16:
+        out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+        check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, RUN_FLOOR)
+    else:
+        one = torch.zeros(n, d, device=DEV, dtype=torch.bfloat16)
+        ops.paged_attn8(qkv, kv, one, pos, slot, btab, bs, H, hd, n, max(lens))
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, ONE_FLOOR)
+    one.zero_()                                                   # the token's own key from its registers
+    last = torch.tensor([sum(lens[:i + 1]) - 1 for i in range(len(lens))], device=DEV)
+    k = len(lens)
+    ops.paged_attn8(qkv[last], kv, one, pos[last].contiguous(), slot[last].contiguous(), btab, bs, H, hd, k, max(lens), append=True)
+    check(one, qkv[last], kv, btab, bs, H, hd, pos[last], slot[last], range(k), 0.0, ONE_FLOOR)
+    assert ops.error_word() == 0
+
