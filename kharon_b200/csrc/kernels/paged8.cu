@@ -146,14 +146,16 @@ extern "C" int kh_read_kv8(const void* kv, int n_blocks, int rec, void* k, void*
 //   O:  A = V^T, B = P: lanes 4 g + i hold 1/8 of the dims, of positions 2 i, 2 i + 1 of each eight; two positions' codes are interleaved by byte permutation.
 // What f16 cannot hold is taken out as powers of two and put back in fp32: q = q' 2^eq (largest |q'| in [2^14, 2^15)), scores times 2^ek, and
 // P' = 2^(s + ev - R + 14) with R the running maximum of s + ev, so that V's codes enter as they are.  P' goes in as two f16 terms, in the even and
-// the odd columns of B (22 bits; 2^-39 of the largest term): nothing is rounded to fewer bits than a sum of the same length in fp32.
+// the odd columns of B (22 bits; 2^-39 of the largest term): nothing is rounded to fewer bits than a sum of the same length in fp32 as long as the exponents of V
+// of positions with weight are not far below the largest, and as q' is exact.  Otherwise (value rows whose sizes differ by 2^10 and more, rows of zeros among them, with the
+// weight on the small ones; a query with an element 2^-29 times its largest) the warp takes its positions again, one by one in fp32: 1.2 ms for the 0.225 below, 38 us for the 17.
 // The block table and the exponents of a chunk are read by one lane per position and passed on by shuffles; the next chunk's K and V replace the
 // current ones in their registers as soon as those are used.
 // With `append` != 0 the item's first warp quantises the token's k and v, writes them into the cache and starts its sums with them.
 // The warps are merged once at the end: shared memory in warp order, then the cluster's shared memory in rank order (no scratch in global
 // memory, one launch).  Bound by memory for wide heads: 128 sequences of 1000 to 4096 positions, 16 heads of 128, 225 us (5.8 TB/s); by
 // issue slots and latency for narrower ones (128 sequences of 3000, 16 heads of 64: 148 us, 5.4 TB/s; of 32: 103 us, 3.9 TB/s); few items by three dependent trips to memory and
-// the join (16 heads of 64 at 16300 positions: 16 us, 2.1 TB/s).
+// the join (16 heads of 64 at 16300 positions: 16.6 us, 2.0 TB/s).
 namespace {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -183,10 +185,13 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// What a lane notes of its positions, as a minimum: ev, in the upper of two bytes; 0 for a query of which f16 loses bits.
+constexpr uint32_t NOTHING = 0xffffu;
+
 // A warp's share of one token and head: R, l (the whole warp's) and o[t] = sums of dims g HD / 8 + t (in every lane of a group of four).
 template <int HD>
 __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, int d, int h, int p, int sl, float scale, int wi, int nw, int append,
-                                               float& R, float& l, float (&out)[HD / 8], bool& bad) {
+                                               float& R, float& l, float (&out)[HD / 8], bool& bad, uint32_t& marks) {
   constexpr int KS = HD == 128 ? 2 : 1, KW = HD / 16 / KS, VW = HD >= 32 ? HD / 32 : 1, NM = HD / 16;       // K: slabs of 64 codes, words per lane; V: words per lane; MMAs across hd
   const int lane = threadIdx.x & 31, g = lane >> 2, i4 = lane & 3, bs = c.bs;
   const int* bt = c.btab + (size_t)sl * c.max_lb;
@@ -252,6 +257,8 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
   uint32_t qa[NM][2];
   float sc, qf;
   {
+    constexpr uint32_t MAG = 0x7fff7fffu, EXP = 0x7c007c00u;
+    uint32_t lost = 0;                             // sign bits: an element of q that is not 0, and below f16's normal numbers as q'
     constexpr int PER = HD / 4 / KS;               // dims of a lane and slab
     uint32_t w[KS][PER / 2], m = 0;
 #pragma unroll
@@ -272,8 +279,11 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
 #pragma unroll
       for (int x = 0; x < PER / 2; x++) {
         const float2 a = unpack_bf16(w[s][x]);
-        qa[s * (PER / 4) + x / 2][x & 1] = pack_f16(a.x * qf, a.y * qf);
+        const uint32_t y = pack_f16(a.x * qf, a.y * qf);
+        qa[s * (PER / 4) + x / 2][x & 1] = y;
+        lost |= ((w[s][x] & MAG) + MAG) & ~((y & EXP) + EXP);
       }
+    if (lost & ~MAG) marks = 0;
   }
   float o[NM][4];
 #pragma unroll
@@ -319,6 +329,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
     for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     R = fmaf(s, sc * pow2_of(ek), (float)((int)ev - 127));
     l = g == 0 ? 16384.f * fv : 0.f;
+    marks = min(marks, ev << 8);
     if (R == -INFINITY) {                          // (an infinity in q: the position has no weight ..
       l = 0.f;
 #pragma unroll
@@ -361,6 +372,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
       s[2 * x] = a[0];
       s[2 * x + 1] = a[2];
     }
+    if (j0 + lane < n) marks = min(marks, e);
     fetch_k();
     float nev[4], tm = -INFINITY;                  // 2^-ev
 #pragma unroll
@@ -433,6 +445,28 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
   }
 }
 
+// The same share in fp32, for exponents that f16 does not suit.
+template <int HD>
+__device__ __forceinline__ void plain_partial(const Cache& c, const bf16* row, int h, int p, int sl, float scale, int wi, int nw, int append, float& R, float& l, float (&out)[HD / 8]) {
+  constexpr int PER = HD / 8;
+  const int g = (threadIdx.x & 31) >> 2;
+  R = -INFINITY;
+  l = 0.f;
+  f32x2 o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  plain_sums8<HD>(c, row, h, sl, scale, wi * 32, append ? p : p + 1, nw * 32, R, l, o);
+  if (append && wi == 0 && block_of(c, sl, p) >= 0) {       // the token's own position, which this warp has just written
+    __syncwarp();
+    plain_sums8<HD>(c, row, h, sl, scale, p, p + 1, 32, R, l, o);
+  }
+  plain_join8<HD>(R, l, o);
+  l *= 16384.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {                   // dims g PER .. of the row are a piece of the sixteen that lane g PER / 16 has
+    const float y = __shfl_sync(0xffffffffu, i & 1 ? hi2(o[i >> 1]) : lo2(o[i >> 1]), g * PER >> 4) * 16384.f;
+    if (i / PER == (g * PER & 15) / PER) out[i % PER] = y;
+  }
+}
+
 }  // namespace
 
 template <int HD, int W>
@@ -450,10 +484,20 @@ paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restr
   // index guard: a context longer than the caller's limit or the block table is recorded (status code 8) and the token skipped
   const bool valid = live && p >= 0 && p < max_ctx && quot(c.div, p) < c.max_lb && sl >= 0 && sl < c.n_slots;      // uniform over the item
   bool bad = live && !valid;
+  uint32_t marks = NOTHING;
   float R = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
   for (int k = 0; k < PER; k++) o[k] = 0.f;
-  if (valid) decode_partial<HD>(c, qkv + (size_t)t * ld + h * HD, d, h, p, sl, scale, wi, W * S, append, R, l, o, bad);
+  if (valid) {
+    decode_partial<HD>(c, qkv + (size_t)t * ld + h * HD, d, h, p, sl, scale, wi, W * S, append, R, l, o, bad, marks);
+    // 2^-25 in P' moves o by 2^-39 sum |v| 2^-ev over sum 2^(s - R): where that may be more than 2^-29 sum |v|, or is not a number, the warp takes its positions again.
+    const uint32_t least = __reduce_min_sync(0xffffffffu, marks);
+    if (least != NOTHING && !(l * pow2_of(least >> 8) >= 16.f)) {
+      const volatile int* pos = c.pos;             // (read again: seldom used, and not kept in registers for it)
+      const volatile int* slot = c.slot;
+      plain_partial<HD>(c, qkv + (size_t)t * ld + h * HD, h, pos[t], slot[t], scale, wi, W * S, append, R, l, o);
+    }
+  }
   if (bad) report(c.err);
   if constexpr (W == 1) {
     if (!valid || (lane & 3)) return;
@@ -485,7 +529,7 @@ paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restr
       const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
       for (int w = 0; w < W; w++) {
-        const float f = ex2(s_part[w * (HD + 2) + HD] - ref);
+        const Weight f(s_part[w * (HD + 2) + HD] - ref);
         den += f * s_part[w * (HD + 2) + HD + 1];
         num += f * s_part[w * (HD + 2) + tid];
       }
@@ -508,7 +552,7 @@ paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restr
 #pragma unroll 4
       for (int r = 0; r < S; r++) {
         const uint32_t a = mapa_shared(base, r);
-        const float f = ex2(ld_cluster_f32(a + HD * 4) - ref);
+        const Weight f(ld_cluster_f32(a + HD * 4) - ref);
         den += f * ld_cluster_f32(a + (HD + 1) * 4);
         num += f * ld_cluster_f32(a + col * 4);
       }

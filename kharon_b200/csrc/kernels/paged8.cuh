@@ -70,6 +70,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// 2^d of a part of a row, as two factors: references hold exponents of values too, so a part whose values are small may have weight although 2^d is below fp32's range.
+struct Weight {
+  float a, b;                                      // b = 1 down to 2^-120
+  __device__ __forceinline__ explicit Weight(float d) : a(ex2(fmaxf(d, -120.f))), b(ex2(fminf(d + 120.f, 0.f))) {}
+  __device__ __forceinline__ float operator*(float x) const { return b * (a * x); }
+};
 // two codes -> two f16 (exact)
 __device__ __forceinline__ uint32_t half2_of(uint32_t codes) {
   uint32_t r;
@@ -99,33 +105,33 @@ inline int make_cache(Cache& c, const char* name, const void* kv, int n_blocks, 
 namespace {
 
 // One token and head by one warp, a position per HD / 16 lanes at a time, in fp32: for the few rows that the tensor cores' formats do not suit.
+// Adds positions first .. first + 31, first + step .. first + step + 31 ... below end to the sums of the lane's group of HD / 16 lanes (o: lane's sixteen dims).
 template <int HD>
-__device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int h, int p, int sl, float scale, bf16* dst) {
+__device__ __forceinline__ void plain_sums8(const Cache& c, const bf16* row, int h, int sl, float scale, int first, int end, int step, float& m, float& l, f32x2 (&o)[8]) {
   constexpr int LPK = HD / 16, KPW = 32 / LPK;
   constexpr float DOWN = 0x1p-24f, UP = 0x1p24f;   // q 2^-24: a sum of codes times the largest q stays finite
   const int lane = threadIdx.x & 31, g = lane / LPK, e0 = lane % LPK * 16, bs = c.bs;
-  f32x2 q[8], o[8];
+  f32x2 q[8];
   {
     const uint4 u0 = *reinterpret_cast<const uint4*>(row + e0), u1 = *reinterpret_cast<const uint4*>(row + e0 + 8);
     const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-    for (int i = 0; i < 8; i++) { q[i] = mul2(un2(w[i]), mk2(scale * DOWN, scale * DOWN)); o[i] = 0; }
+    for (int i = 0; i < 8; i++) q[i] = mul2(un2(w[i]), mk2(scale * DOWN, scale * DOWN));
   }
-  float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-  for (int j0 = 0; j0 <= p; j0 += KPW) {
-    const int j = j0 + g, jj = min(j, p), lb = quot(c.div, jj), at = jj - lb * bs;
+  for (int j0 = first, k = KPW; j0 < end; j0 += k & 31 ? KPW : step - 32 + KPW, k += KPW) {
+    const int j = j0 + g, jj = min(j, end - 1), lb = quot(c.div, jj), at = jj - lb * bs;
     const int b = __ldg(c.btab + (size_t)sl * c.max_lb + lb);
     const uint8_t* rc = record(c, (unsigned)b < (unsigned)c.n_blocks ? b : 0, h);
-    const uint4 k = *reinterpret_cast<const uint4*>(rc + at * HD + e0), v = *reinterpret_cast<const uint4*>(rc + (bs + at) * HD + e0);
-    const uint32_t e = *reinterpret_cast<const uint16_t*>(rc + 2 * bs * HD + 2 * at), kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
+    const uint4 k4 = *reinterpret_cast<const uint4*>(rc + at * HD + e0), v = *reinterpret_cast<const uint4*>(rc + (bs + at) * HD + e0);
+    const uint32_t e = *reinterpret_cast<const uint16_t*>(rc + 2 * bs * HD + 2 * at), kw[4] = {k4.x, k4.y, k4.z, k4.w}, vw[4] = {v.x, v.y, v.z, v.w};
     f32x2 a = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) a = fma2(f32x2_of(half2_of(kw[i >> 1] >> (i & 1) * 16)), q[i], a);
     float s = lo2(a) + hi2(a);
 #pragma unroll
     for (int x = LPK / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (j <= p) {
+    if (j < end) {
       s *= pow2_of(e & 0xffu) * UP;
       const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn, sc = ex2(m - ref), pr = ex2(s - ref), pv = pr * pow2_of(e >> 8);
       m = mn;
@@ -134,8 +140,12 @@ __device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int
       for (int i = 0; i < 8; i++) o[i] = fma2(f32x2_of(half2_of(vw[i >> 1] >> (i & 1) * 16)), mk2(pv, pv), mul2(o[i], mk2(sc, sc)));
     }
   }
+}
+// The groups' sums together, in every group.
+template <int HD>
+__device__ __forceinline__ void plain_join8(float& m, float& l, f32x2 (&o)[8]) {
 #pragma unroll
-  for (int x = LPK; x < 32; x <<= 1) {
+  for (int x = HD / 16; x < 32; x <<= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, x), l2 = __shfl_xor_sync(0xffffffffu, l, x);
     const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn, c1 = ex2(m - ref), c2 = ex2(m2 - ref);
     m = mn;
@@ -143,6 +153,16 @@ __device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] = fma2(o[i], mk2(c1, c1), mul2((f32x2)__shfl_xor_sync(0xffffffffu, o[i], x), mk2(c2, c2)));
   }
+}
+// A whole row: positions 0 .. p.
+template <int HD>
+__device__ __forceinline__ void attend_row8(const Cache& c, const bf16* row, int h, int p, int sl, float scale, bf16* dst) {
+  constexpr int LPK = HD / 16;
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f;
+  f32x2 o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  plain_sums8<HD>(c, row, h, sl, scale, 0, p + 1, 32, m, l, o);
+  plain_join8<HD>(m, l, o);
   const float inv = 1.f / l;
   if (lane < LPK) {
     uint32_t w[8];

@@ -64,13 +64,13 @@ def attend(q, k, v, p_half_step=0.0):
     return o, 2.0 ** -8 * o.abs() + (1 + 2.0 ** -8) * c[:, None] * mag + 1e-30
 
 
-def attend_own(q, k, v, p_half_step=0.0, floor=0.0):
+def attend_own(q, k, v, p_half_step=0.0, floor=0.0, each=0.0):
     """``attend`` with a bound that counts each score by its own terms, so that one large key excuses nothing in the others.
 
     The score of key j is off by at most delta_j = (hd + 4) * 2^-24 * sum |q k_j| / sqrt(hd) + 2^-21 (exponential), so p_j lies between what it is with its own
     score moved one way and all others the other way; o is off by those differences times |v_j|, by ctx * 2^-24 of sum p |v| for the
     sums, and by `p_half_step` of it where the probabilities are rounded before P V.  `floor`: the smallest step of such a rounding, half of it, relative to the
-    largest probability of the row, which every position may be off by.  Output in bf16."""
+    largest probability of the row, which every position may be off by; `each`: the same where the kernel bounds it by itself, as part of a whole.  Output in bf16."""
     hd, ctx = q.shape[-1], k.shape[0]
     s = torch.einsum("he,jhe->hj", q, k) / math.sqrt(hd)
     p = torch.softmax(s, -1)
@@ -82,7 +82,7 @@ def attend_own(q, k, v, p_half_step=0.0, floor=0.0):
     lo = torch.sigmoid((s - d) - others(s + d)) if ctx > 1 else torch.ones_like(p)
     dp = torch.maximum(hi - p, p - lo).clamp(min=0)
     mag = torch.einsum("hj,jhe->he", p, v.abs())
-    err = torch.einsum("hj,jhe->he", dp, v.abs()) + ((ctx + 8) * 2.0 ** -24 + p_half_step) * mag + floor * p.amax(-1)[:, None] * v.abs().sum(0)
+    err = torch.einsum("hj,jhe->he", dp, v.abs()) + ((ctx + 8) * 2.0 ** -24 + p_half_step) * mag + (floor * p.amax(-1)[:, None] + each) * v.abs().sum(0)
     return o, 2.0 ** -8 * o.abs() + (1 + 2.0 ** -8) * err + 1e-30
 
 

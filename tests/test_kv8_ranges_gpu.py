@@ -13,16 +13,18 @@ DEV = "cuda"
 # Rounding of the probabilities in runs of more than 64 tokens: half a step of 11 bits; half the smallest step is 2^-32 of the largest probability times 2^(difference of two
 # value rows' exponents), 14 at most.  Single tokens: two such terms, 2^-39 and the same difference.
 RUN, RUN_FLOOR, ONE_FLOOR = 2.0 ** -12, 2.0 ** -18, 2.0 ** -25
+# What the single-token kernel leaves of it, or takes the positions again.
+ONE_EACH = 2.0 ** -29
 
 
-def check(out, q, kv, btab, bs, H, hd, pos, slot, rows, p_half_step, floor):
+def check(out, q, kv, btab, bs, H, hd, pos, slot, rows, p_half_step, floor, each=0.0):
     kv, btab, pos, slot, q, out = kv.cpu(), btab.cpu(), pos.cpu(), slot.cpu(), q.double().cpu(), out.double().cpu()
     cache = {}
     for t in rows:
         s, n = int(slot[t]), int(pos[t]) + 1
         if s not in cache:
             cache[s] = rows_of(kv, btab[s], bs, hd, max(int(pos[u]) + 1 for u in rows if int(slot[u]) == s))
-        want, tol = attend_own(q[t, :H * hd].view(H, hd), cache[s][0][:n], cache[s][1][:n], p_half_step, floor)
+        want, tol = attend_own(q[t, :H * hd].view(H, hd), cache[s][0][:n], cache[s][1][:n], p_half_step, floor, each)
         err = (out[t, :H * hd].view(H, hd) - want).abs()
         assert not bool(want.isnan().any()) and bool((err <= tol).all()), (t, n, float((err / tol).nan_to_num(1e30).max()))
 
@@ -123,3 +125,39 @@ def test_queries_near_the_types_end_beside_small_keys(hd, H, lens):
     check(one, qkv[last], kv, btab, bs, H, hd, pos[last], slot[last], range(k), 0.0, ONE_FLOOR)
     assert ops.error_word() == 0
 
+
+
+@pytest.mark.parametrize("hd,H,bs,lens", [(16, 2, 16, [1, 2, 90]), (32, 4, 5, [40, 700]), (64, 2, 16, [33, 1000]), (128, 2, 24, [700, 5]), (64, 16, 16, [60] * 150), (128, 2, 16, [3000])])
+@pytest.mark.parametrize("append", [False, True])
+def test_single_tokens_with_an_infinite_value_or_scales_far_apart(hd, H, bs, lens, append):
+    """An infinity in one element of a cached value (head 0: kept as the largest number) leaves the other elements to the other positions; head 1: scales from 2^-30 to 2^30."""
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d, g = len(pos), H * hd, torch.Generator().manual_seed(3)
+    qkv[pos == min(lens[-1] - 1, 20), 2 * d + 2] = math.inf
+    qkv[:, 2 * d + hd:2 * d + 2 * hd] *= (2.0 ** torch.randint(-30, 30, (n, 1), generator=g)).to(DEV)
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    last = torch.tensor([sum(lens[:i + 1]) - 1 for i in range(len(lens))], device=DEV)
+    k = len(lens)
+    q, p, s, out = qkv[last], pos[last].contiguous(), slot[last].contiguous(), torch.zeros(k, d, device=DEV, dtype=torch.bfloat16)
+    ops.paged_attn8(q, kv, out, p, s, btab, bs, H, hd, k, max(lens), append=append)
+    check(out, q, kv, btab, bs, H, hd, p, s, range(min(k, 4)), 0.0, 0.0, ONE_EACH)
+    again = torch.zeros_like(out)
+    ops.paged_attn8(q, kv, again, p, s, btab, bs, H, hd, k, max(lens), append=append)
+    assert torch.equal(out, again) and ops.error_word() == 0
+
+
+@pytest.mark.parametrize("hd,H,bs,lens", [(16, 2, 16, [1, 2, 90]), (32, 4, 5, [40, 700]), (64, 2, 16, [33, 1000]), (128, 2, 24, [700, 5]), (64, 16, 16, [60] * 150), (128, 2, 16, [3000])])
+@pytest.mark.parametrize("append", [False, True])
+def test_single_tokens_whose_query_has_one_element_far_larger_than_the_others(hd, H, bs, lens, append):
+    """The keys are zero where the query is 2^60 times as large: the other elements make the scores."""
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, 3:d:hd] *= 2.0 ** 60
+    qkv[:, d + 3:2 * d:hd] = 0.0
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    last = torch.tensor([sum(lens[:i + 1]) - 1 for i in range(len(lens))], device=DEV)
+    k = len(lens)
+    q, p, s, out = qkv[last], pos[last].contiguous(), slot[last].contiguous(), torch.zeros(k, d, device=DEV, dtype=torch.bfloat16)
+    ops.paged_attn8(q, kv, out, p, s, btab, bs, H, hd, k, max(lens), append=append)
+    check(out, q, kv, btab, bs, H, hd, p, s, range(min(k, 4)), 0.0, 0.0, ONE_EACH)
+    assert ops.error_word() == 0
