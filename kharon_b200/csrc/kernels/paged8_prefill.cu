@@ -318,7 +318,7 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 //   q', k' below 2^-14: off by 2^-25, and by up to 448 * 2^-25 where a key's exponent is more than 31 below the tile's largest: a score by at most HD times
 //   q' times that.  From 22 below on (until there k' is exact) the fetching warps note the tile's exponent, and rows for which that bound is more than
 //   2^-12 of a log2 unit are done anew in fp32 (typical sizes stay 11 octaves below it, so keys of nearly nothing cost nothing);
-//   v' of positions whose exponent is more than 22 below the tile's largest: the item's rows are done anew, one by one, in fp32;
+//   v' of positions whose exponent is more than 22 below the tile's largest (but for rows of zeros): the item's rows are done anew, one by one, in fp32;
 //   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
 // A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
 //
@@ -577,6 +577,15 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       }
       e_now = e_next;
     };
+    auto any_code = [&](uint64_t row) {                    // rows of the smallest exponent: whether it holds numbers or zeros
+      uint32_t any = 0;
+#pragma unroll 1
+      for (int i = 0; i < HD; i += 16) {
+        const uint4 w = ld_early_16(row + i);
+        any |= (w.x | w.y | w.z | w.w) & 0x7f7f7f7fu;
+      }
+      return any != 0;
+    };
     auto factors = [&](int b, int it) {                    // 2^(e - E + 7) of its positions, E the tile's largest exponent
       if ((kt0 + it) * 128 + t >= ctx) e_now = 0;
       const uint32_t mk = __reduce_max_sync(0xffffffffu, e_now & 0xffu), mv = __reduce_max_sync(0xffffffffu, e_now >> 8);
@@ -584,7 +593,10 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       pair_barrier(4 + vr);
       const uint32_t tops = __vmaxu2(__vmaxu2(s_wmax[b * 4], s_wmax[b * 4 + 1]), __vmaxu2(s_wmax[b * 4 + 2], s_wmax[b * 4 + 3]));
       const int e = (int)(e_now >> 8 * vr & 0xffu), off = e - (int)(tops >> 16 * vr & 0xffffu);
-      if (off < -22 && e > (vr ? E_LO : 0)) atomicMax(redo, vr ? REDO_ALL : (int)(tops & 0xffffu));      // (e: 0 past the end)
+      if (off < -22 && e > 0) {                            // (e: 0 past the end)
+        if (!vr) atomicMax(redo, (int)(tops & 0xffffu));
+        else if (e > E_LO || any_code(s_addr[b * 128 + t])) atomicMax(redo, REDO_ALL);
+      }
       s_fac[b * 128 + t] = f16_pow2(off + 7) * 0x10001u;
       // K's warps tell the groups both exponents: scores that are there have passed bar_kfull.  (Of four slots this one was last read for the tile
       // four before, whose scores both groups have used: K's stage of the tile two before this one has been freed.)

@@ -161,3 +161,19 @@ def test_single_tokens_whose_query_has_one_element_far_larger_than_the_others(hd
     ops.paged_attn8(q, kv, out, p, s, btab, bs, H, hd, k, max(lens), append=append)
     check(out, q, kv, btab, bs, H, hd, p, s, range(min(k, 4)), 0.0, 0.0, ONE_EACH)
     assert ops.error_word() == 0
+
+
+@pytest.mark.parametrize("hd,H,lens", SHAPES)
+def test_values_of_the_smallest_scale_beside_ordinary_ones(hd, H, lens):
+    """Position 0's values lie below 448 * 2^-63, where the exponent ends: the row that sees nothing else has them as they are.  Rows of zeros beside them change nothing."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[pos == 0, 2 * d:] *= 2.0 ** -56
+    qkv[(pos > 3) & (pos % 5 == 0), 2 * d:] = 0.0
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+    rows = [0, 1, 5, 80, lens[0] - 1, n - 1]
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, RUN_FLOOR)
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
+
