@@ -45,17 +45,18 @@ __device__ __forceinline__ void join_parts(int parts, A place, float (&den)[NR],
       }
 #pragma unroll
     for (int k = 0; k < NR; k++) {
-      const float m = fmaxf(fmaxf(fmaxf(v[k][0][0], v[k][1][0]), fmaxf(v[k][2][0], v[k][3][0])), mx[k]), ref = m == -INFINITY ? 0.f : m, al = ex2(mx[k] - ref);
+      const float m = fmaxf(fmaxf(fmaxf(v[k][0][0], v[k][1][0]), fmaxf(v[k][2][0], v[k][3][0])), mx[k]), ref = m == -INFINITY ? 0.f : m;
+      const Weight al(mx[k] - ref);
       mx[k] = m;
-      den[k] *= al;
+      den[k] = al * den[k];
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[k][e] *= al;
+      for (int e = 0; e < 4; e++) o[k][e] = al * o[k][e];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float f = i0 + i < parts ? ex2(v[k][i][0] - ref) : 0.f;
-        den[k] = fmaf(f, v[k][i][1], den[k]);
+        const Weight f(i0 + i < parts ? v[k][i][0] - ref : -INFINITY);
+        den[k] += f * v[k][i][1];
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[k][e] = fmaf(f, y[k][i][e], o[k][e]);
+        for (int e = 0; e < 4; e++) o[k][e] += f * y[k][i][e];
       }
     }
   }
@@ -314,13 +315,15 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 // P keeps 11 bits.  f16 has few exponents, so every power of two that is common to a row or a tile is taken out and put back in fp32:
 //   q = q' 2^eq (row; largest |q'| in [2^14, 2^15)),  k = k' 2^(EK - 7),  v = v' 2^(EV - 7)  with EK, EV the tile's largest exponents,
 //   P' = 2^(s + EV - R),  O = sum P' v' = 2^(7 - R) sum 2^s v,  l = sum over tiles of 2^(EB - EV) sum P' = 2^(EB - R) sum 2^s,
-// where R is the row's running maximum of (largest score + EV), in log2 units, and EB the first tile's EV.  What f16 rounds:
+// where R + 7 is the row's running maximum of (largest score + EV), in log2 units (so the largest P' is 2^7 to 2^15), and EB the first tile's EV.  What f16 rounds:
 //   q', k' below 2^-14: off by 2^-25, and by up to 448 * 2^-25 where a key's exponent is more than 31 below the tile's largest: a score by at most HD times
 //   q' times that.  From 22 below on (until there k' is exact) the fetching warps note the tile's exponent, and rows for which that bound is more than
 //   2^-12 of a log2 unit are done anew in fp32 (typical sizes stay 11 octaves below it, so keys of nearly nothing cost nothing);
 //   v' of positions whose exponent is more than 22 below the tile's largest (but for rows of zeros): the item's rows are done anew, one by one, in fp32;
-//   P': half a step of 11 bits, and 2^-25 of the row's largest terms.
-// A row is rescaled only when R would grow by more than 8 (the older R stays the reference, P' up to 2^8).
+//   P': half a step of 11 bits; below 2^-14, 2^-25, which moves o by 2^-25 sum |v| 2^(EB - EV) / l.  Where that may be more than 2^-9 of the mean |v| (largest scores
+//   beside values that are small compared with other tiles') the row is done anew.
+// A row is rescaled only when R would grow by more than 8 (the older R stays the reference).  A row to be done anew leaves NaN as its normaliser, which passes through every
+// join.
 //
 // Heads of 128 are bound by the tensor core (its operands' trips through shared memory) and the exponentials together, each two thirds of the
 // time on the SMs in use: 2048 tokens behind 14300 positions, 16 heads, 273 us (942 TFLOP/s; 128 items on 148 SMs), four turns of 384 to 640 tokens behind 1500 to 4000
@@ -434,6 +437,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   constexpr int REDO_ALL = 256;
   int* redo = const_cast<int*>(abort_flag) + 1;
   auto lost = [](int redo, float rq) { return redo >= REDO_ALL || (redo && !(rq * pow2_of(redo - 7) * HD <= 0x1p-11f)); };
+  uint32_t* least_v = reinterpret_cast<uint32_t*>(redo) + 2;       // smallest EV of the tiles
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (4 * NS + 13) + 8);
   uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + C::AGAIN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -457,6 +461,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     for (int i = 0; i < 4; i++) { mbar_init(bar_s + 8 * i, 1); mbar_init(bar_p + 8 * i, 4); }      // [group][half]
     mbar_init(bar_pv, 1); mbar_init(bar_pv + 8, 1); mbar_init(bar_o, 1); mbar_init(bar_o + 8, 1); mbar_init(bar_q, GW);
     *redo = 0;
+    *least_v = 255;
     *abort_flag = (base & 1023u) ? 6 : 0;         // swizzled tiles need the 1024-byte alignment
     if (base & 1023u) atomicCAS(c.err, 0, 6);
     mbar_fence_init();
@@ -602,6 +607,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       // four before, whose scores both groups have used: K's stage of the tile two before this one has been freed.)
       if (t == 0 && !vr) s_tmax[it & 3] = tops;
       pair_barrier(4 + vr);
+      if (t == 0 && !vr) *least_v = min(*least_v, tops >> 16);
     };
     if (live && kt0 < kt1) {
       look(kt0);
@@ -727,7 +733,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
             }
           }
           const float mt = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl, fev);
-          done = !__any_sync(0xffffffffu, mt > R + 8.f);
+          done = !__any_sync(0xffffffffu, mt > R + 15.f);
           if (done) {
             tmem_st16(tS, pk);                   // over the scores
             tmem_st16(tS + 16, pk + 16);
@@ -767,16 +773,16 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
             mx = fmaxf(m0, m1);
           }
           const float mt = fmaf(mx, sl, fev);
-          const bool grow = mt > R + 8.f;        // (from -inf too)
+          const bool grow = mt > R + 15.f;       // (from -inf too)
           if (__any_sync(0xffffffffu, grow)) {
-            const float al = grow ? ex2(R - mt) : 1.f;
+            const float al = grow ? ex2(R - (mt - 7.f)) : 1.f;
             if (cnt + half > 0) {                // O is there, once the last P V is done (the one before it is: these scores came after it)
               wait(bar_pv + 8 * w, (half ^ 1) & 1);
               tc_fence_after();
               rescale<HD>(tO, al);
             }
             l *= al;
-            if (grow) R = mt;
+            if (grow) R = mt - 7.f;
           }
           const float c0 = fev - (R == -INFINITY ? 0.f : R);
           const f32x2 c2 = mk2(c0, c0);
@@ -807,7 +813,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     }
     if (mine > 0) wait(bar_o + 8 * w, 0);      // (on a barrier of its own: the P V before the last may not be done, and its parity would be taken for the last one's)
     tc_fence_after();
-    const float den = l * pow2_of(261u - eb);    // l 2^(7 - EB)
+    float den = l * pow2_of(261u - eb);          // l 2^(7 - EB)
     // A NaN in V reaches the rows that see its position and no others.  P V multiplies it with the zeros of masked positions too, which leaves a
     // NaN in every row of the tile: such rows are done anew, one by one.
     auto leave = [&]() {                         // (R, normaliser, O) of the group's rows in shared memory, over the tiles
@@ -827,7 +833,9 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
           *reinterpret_cast<uint4*>(part + q + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
     };
-    named_barrier<1, C::ROWS>();                     // no tile is read any more, and `redo` is written
+    named_barrier<1, C::ROWS>();                     // no tile is read any more; `redo` and `least_v` are written
+    // (l beyond 2^100: a first tile of values 2^85 times the later ones', and no weight)
+    if (R > -INFINITY && (lost(*redo, rq) || !(l * pow2_of(127u + *least_v - eb) * 0x1p16f >= ctx) || l > 0x1p100f)) den = __int_as_float(0x7fffffff);
     if (G == 2 && S > 1) leave();
     else {
       float own = 1.f, other = 0.f, sum = den;   // weights of the group's sums and of the second group's for the same rows
@@ -843,7 +851,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         }
       }
       if (apart || w == 0) {
-        const bool intact = *abort_flag == 0 && lrow < n, all = lost(*redo, rq);
+        const bool intact = *abort_flag == 0 && lrow < n;
         const float inv = 1.f / sum;
         const float* part = reinterpret_cast<const float*>(smem) + (128 + row) * C::PITCH;
         bf16* dst = out + (size_t)(r0 + lrow) * ldo + h * HD;
@@ -871,7 +879,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
 #pragma unroll
               for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(dst + q + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
-        const uint32_t again = __ballot_sync(0xffffffffu, intact && (all || top >= 0x7f800000u));
+        const uint32_t again = __ballot_sync(0xffffffffu, intact && top >= 0x7f800000u);
         if (lane == 0) s_again[warp] = again;
       }
     }
@@ -880,12 +888,6 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   if (G == 2 && S > 1) { __syncwarp(); cluster_sync_all(); }
   if (G == 2 && live && S > 1) {
     const int parts = nq == 2 ? S : 2 * S;       // of a row: part i is group i % 2 (or the row's own) of CTA i / 2 (or i)
-    int noted = 0;
-    for (int i = 0; i < S; i++) {
-      float v[1];
-      ld_cluster(mapa_shared(smem_u32(redo), i), v);
-      noted = max(noted, __float_as_int(v[0]));
-    }
     // CTA `rank` joins rows rank, rank + S ...; a thread four columns of a row
     constexpr int TPR = HD / 4;
     const int ch = tid % TPR;
@@ -905,7 +907,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
         const int r = r1 + k * STEP * S;
         if (r >= n) break;
         const float inv = 1.f / den[k];
-        bool anew = lost(noted, sl2 * reinterpret_cast<const float*>(smem + C::QE)[r]) || !(den[k] > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
+        bool anew = !(den[k] > 0.f) || (__float_as_uint(inv) & 0x7fffffffu) >= 0x7f800000u;
 #pragma unroll
         for (int e = 0; e < 4; e++) anew |= (__float_as_uint(o[k][e]) & 0x7fffffffu) >= 0x7f800000u;
         if (anew) atomicOr(s_again + (r >> 5), 1u << (r & 31));

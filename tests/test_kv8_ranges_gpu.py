@@ -15,15 +15,29 @@ DEV = "cuda"
 RUN, RUN_FLOOR, ONE_FLOOR = 2.0 ** -12, 2.0 ** -18, 2.0 ** -25
 # What the single-token kernel leaves of it, or takes the positions again.
 ONE_EACH = 2.0 ** -29
+# What the kernel of long runs leaves of it, of the mean |v|, or computes the row again.
+RUN_MEAN = 2.0 ** -9
 
 
-def check(out, q, kv, btab, bs, H, hd, pos, slot, rows, p_half_step, floor, each=0.0):
+def smallest_step(q, k, ev):
+    """[H]: what half the smallest step of a probability in f16 may move o by, in the kernel of long runs, per unit of sum |v|.  Probabilities are 2^(s + EV - R) with EV the
+    largest exponent of a tile of 128 values' rows (masked ones too) and R at most 7 below the largest s + EV, so the step is 2^-25 2^(R - EV) over sum 2^s."""
+    n, s = k.shape[0], torch.einsum("he,jhe->hj", q, k) / math.sqrt(q.shape[-1]) / math.log(2)
+    tiles = torch.stack([ev[a:a + 128].amax(0) for a in range(0, len(ev), 128)])            # [tiles, H]
+    top = (s + tiles.repeat_interleave(128, 0)[:n].t()).amax(-1)
+    return torch.exp2(-25 + top - 7 - tiles[:(n + 127) // 128].amin(0) - s.mul(math.log(2)).logsumexp(-1) / math.log(2))
+
+
+def check(out, q, kv, btab, bs, H, hd, pos, slot, rows, p_half_step, floor, each=0.0, mean=0.0):
     kv, btab, pos, slot, q, out = kv.cpu(), btab.cpu(), pos.cpu(), slot.cpu(), q.double().cpu(), out.double().cpu()
     cache = {}
     for t in rows:
         s, n = int(slot[t]), int(pos[t]) + 1
         if s not in cache:
             cache[s] = rows_of(kv, btab[s], bs, hd, max(int(pos[u]) + 1 for u in rows if int(slot[u]) == s))
+        if mean:
+            ev = torch.stack([kv[int(btab[s][j // bs]), :, 2 * bs * hd + 2 * (j % bs) + 1].double() - 127 for j in range(len(cache[s][0]))])
+            each = smallest_step(q[t, :H * hd].view(H, hd), cache[s][0][:n], ev).clamp(max=mean / n)[:, None]
         want, tol = attend_own(q[t, :H * hd].view(H, hd), cache[s][0][:n], cache[s][1][:n], p_half_step, floor, each)
         err = (out[t, :H * hd].view(H, hd) - want).abs()
         assert not bool(want.isnan().any()) and bool((err <= tol).all()), (t, n, float((err / tol).nan_to_num(1e30).max()))
@@ -177,3 +191,45 @@ def test_values_of_the_smallest_scale_beside_ordinary_ones(hd, H, lens):
     check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, RUN_FLOOR)
     check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
 
+
+
+@pytest.mark.parametrize("hd,H,lens", SHAPES)
+@pytest.mark.parametrize("power", [8, 12, 14, 17, 20, 22, 40])
+@pytest.mark.parametrize("early", [True, False])
+def test_one_value_row_far_larger_than_the_others(hd, H, lens, power, early):
+    """One row of values 2^power times the others, in one element only: in the first tile, where all later rows see it with next to no weight, or further on, where some must
+    not see it.  The other elements keep their bits."""
+    bs, j = 16, 20 if early else max(lens) - 150
+    kv, btab, pos, slot, qkv = make(hd + power, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    m = pos == j
+    for h in range(H):
+        qkv[m, 2 * d + h * hd:2 * d + (h + 1) * hd] = 0.0
+        qkv[m, 2 * d + h * hd + 1] = 2.0 ** power
+    qkv[m, d:2 * d] = 0.0
+    qkv[pos > j, d:2 * d] *= 0.25
+    if early:
+        qkv[m, d:2 * d] = -qkv[:1, :d] * 4                         # (queries are alike: a score far below the others')
+        qkv[:, :d] = (qkv[:1, :d].float() + 0.3 * qkv[:, :d].float()).bfloat16()
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+    first = n - lens[-1] if lens[-1] == max(lens) else 0
+    rows = [first + t for t in (0, j - 20, j - 1, j, j + 1, j + 60, j + 149, max(lens) - 30, max(lens) - 1)]
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, 0.0, mean=RUN_MEAN)
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
+
+
+@pytest.mark.parametrize("hd,H,lens", [(32, 2, [700]), (64, 2, [700]), (128, 2, [700])])
+def test_values_whose_scales_differ_between_tiles(hd, H, lens):
+    """The first 256 positions' values are 0, the next ones' 2^-60 and the last ones' 2^62: the zeros have their weight."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[pos < 256, 2 * d:] = 0.0
+    qkv[(pos >= 256) & (pos < 512), 2 * d:] *= 2.0 ** -60
+    qkv[pos >= 512, 2 * d:] *= 2.0 ** 62
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+    rows = [0, 255, 256, 300, 511, 512, 600, 699]
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, 0.0, mean=RUN_MEAN)
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
