@@ -322,6 +322,8 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 //   v' of positions whose exponent is more than 22 below the tile's largest (but for rows of zeros): the item's rows are done anew, one by one, in fp32;
 //   P': half a step of 11 bits; below 2^-14, 2^-25, which moves o by 2^-25 sum |v| 2^(EB - EV) / l.  Where that may be more than 2^-9 of the mean |v| (largest scores
 //   beside values that are small compared with other tiles') the row is done anew.
+// Rows whose |q| |k| may give scores beyond 2^23 (HD 2^15 448 2^7 of the products' units) are done anew too: R is off by more than one half there, which P' would have in its
+// exponent, and elements of q' below 2^-14 may be what the score is made of, where a larger one meets zeros.
 // A row is rescaled only when R would grow by more than 8 (the older R stays the reference).  A row to be done anew leaves NaN as its normaliser, which passes through every
 // join.
 //
@@ -437,7 +439,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
   constexpr int REDO_ALL = 256;
   int* redo = const_cast<int*>(abort_flag) + 1;
   auto lost = [](int redo, float rq) { return redo >= REDO_ALL || (redo && !(rq * pow2_of(redo - 7) * HD <= 0x1p-11f)); };
-  uint32_t* least_v = reinterpret_cast<uint32_t*>(redo) + 2;       // smallest EV of the tiles
+  uint32_t* reach = reinterpret_cast<uint32_t*>(redo) + 2;       // of the tiles: largest EK, largest 255 - EV
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BARS + 8 * (4 * NS + 13) + 8);
   uint32_t* s_again = reinterpret_cast<uint32_t*>(smem + C::AGAIN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -461,7 +463,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
     for (int i = 0; i < 4; i++) { mbar_init(bar_s + 8 * i, 1); mbar_init(bar_p + 8 * i, 4); }      // [group][half]
     mbar_init(bar_pv, 1); mbar_init(bar_pv + 8, 1); mbar_init(bar_o, 1); mbar_init(bar_o + 8, 1); mbar_init(bar_q, GW);
     *redo = 0;
-    *least_v = 255;
+    *reach = 0;
     *abort_flag = (base & 1023u) ? 6 : 0;         // swizzled tiles need the 1024-byte alignment
     if (base & 1023u) atomicCAS(c.err, 0, 6);
     mbar_fence_init();
@@ -607,7 +609,7 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
       // four before, whose scores both groups have used: K's stage of the tile two before this one has been freed.)
       if (t == 0 && !vr) s_tmax[it & 3] = tops;
       pair_barrier(4 + vr);
-      if (t == 0 && !vr) *least_v = min(*least_v, tops >> 16);
+      if (t == 0 && !vr) *reach = __vmaxu2(*reach, (tops & 0xffffu) | (255u - (tops >> 16)) << 16);
     };
     if (live && kt0 < kt1) {
       look(kt0);
@@ -833,9 +835,11 @@ paged_chunk8_k(const __grid_constant__ Runs runs, const __grid_constant__ Cache 
           *reinterpret_cast<uint4*>(part + q + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
     };
-    named_barrier<1, C::ROWS>();                     // no tile is read any more; `redo` and `least_v` are written
+    named_barrier<1, C::ROWS>();                     // no tile is read any more; `redo` and `reach` are written
     // (l beyond 2^100: a first tile of values 2^85 times the later ones', and no weight)
-    if (R > -INFINITY && (lost(*redo, rq) || !(l * pow2_of(127u + *least_v - eb) * 0x1p16f >= ctx) || l > 0x1p100f)) den = __int_as_float(0x7fffffff);
+    const uint32_t far = *reach;
+    if (R > -INFINITY && (lost(*redo, rq) || !(rq * pow2_of((far & 0xffffu) - 7) * HD <= 0x1p-8f) || !(l * pow2_of(382u - (far >> 16) - eb) * 0x1p16f >= ctx) || l > 0x1p100f))
+      den = __int_as_float(0x7fffffff);
     if (G == 2 && S > 1) leave();
     else {
       float own = 1.f, other = 0.f, sum = den;   // weights of the group's sums and of the second group's for the same rows

@@ -233,3 +233,31 @@ def test_values_whose_scales_differ_between_tiles(hd, H, lens):
     rows = [0, 255, 256, 300, 511, 512, 600, 699]
     check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, 0.0, mean=RUN_MEAN)
     check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
+
+
+@pytest.mark.parametrize("hd,H,lens", SHAPES)
+@pytest.mark.parametrize("power", [18, 22, 25, 30, 45, 60])
+def test_runs_with_scores_beyond_the_integers_of_fp32(hd, H, lens, power):
+    """Scores of some 2^power, where neighbouring numbers of fp32 are far apart: one position has all the weight, and its values come out as they are."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd + power, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, d:2 * d] *= 2.0 ** power
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, _ = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, list(range(0, min(n, 700), 17)) + [n - 1], RUN, 0.0, mean=RUN_MEAN)
+
+
+@pytest.mark.parametrize("hd,H,lens", SHAPES)
+def test_runs_whose_queries_have_one_element_far_larger_than_the_others(hd, H, lens):
+    """The keys are zero where the query is 2^60 times as large: the other elements make the scores."""
+    bs = 16
+    kv, btab, pos, slot, qkv = make(hd, lens, H, hd, bs)
+    n, d = len(pos), H * hd
+    qkv[:, 3:d:hd] *= 2.0 ** 60
+    qkv[:, d + 3:2 * d:hd] = 0.0
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, lens)
+    rows = [0, 1, 39, 41, 80, n - 40, n - 1]
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, 0.0, mean=RUN_MEAN)
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
