@@ -261,3 +261,23 @@ def test_runs_whose_queries_have_one_element_far_larger_than_the_others(hd, H, l
     rows = [0, 1, 39, 41, 80, n - 40, n - 1]
     check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, RUN, 0.0, mean=RUN_MEAN)
     check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("n,half_step,mean", [(64, 0.0, 0.0), (300, RUN, RUN_MEAN), (700, RUN, RUN_MEAN)])
+def test_probabilities_keep_the_bits_that_are_stated(hd, n, half_step, mean):
+    """All keys but the first have the same score, whose probability over the first's lies halfway between two numbers of eight bits, and the first position's values
+    cancel most of what the others add up to: a rounding of the probabilities is not averaged out, and not hidden by the output's."""
+    H, bs = 2, 16
+    kv, btab, pos, slot, qkv = make(hd, [n], H, hd, bs)
+    x = qkv.zero_().view(n, 3, H, hd)
+    gap = -math.log(194.5 / 256)                                   # of the scores
+    x[:, 0, :, 0] = gap * math.sqrt(hd)
+    x[0, 1, :, 0] = 1.0
+    x[:, 2] = 1.0
+    x[0, 2] = -math.exp(-gap) * (n - 1) * 0.97                     # the last row's sum is what is cancelled
+    ops.append_kv8(qkv, kv, pos, slot, btab, bs, H, hd, n)
+    out, one = both(qkv, kv, pos, slot, btab, bs, H, hd, [n])
+    rows = [n - 1, n - 2, n // 2]
+    check(out, qkv, kv, btab, bs, H, hd, pos, slot, rows, half_step, 0.0, mean=mean)
+    check(one, qkv, kv, btab, bs, H, hd, pos, slot, rows, 0.0, 0.0, ONE_EACH)
