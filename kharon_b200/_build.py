@@ -5,7 +5,8 @@ Three shared objects are produced under ``kharon_b200/_lib``:
 * ``libkharon_rt.so``   -- host runtime (C++17, g++), no CUDA dependency;
 * ``libkharon_cuda.so`` -- every CUDA kernel, compiled by nvcc for ``sm_100a`` only
   (``-gencode arch=compute_100a,code=sm_100a``); cross-compiles without a GPU;
-* ``kharon_bind.so``    -- Python extension (g++, torch's headers) through which small calls skip ctypes.
+* ``kharon_bind-*.so``  -- Python extension (g++, torch's headers) through which small calls skip ctypes.  Its name holds the versions of torch and Python
+  that it was built for; without it every operator still has its way through ctypes.
 
 Objects are rebuilt only when a source or header is newer than the object.  Run
 ``python -m kharon_b200._build`` to build everything; ``--verbose`` adds ``-Xptxas -v``.
@@ -102,11 +103,18 @@ def build_cuda(force: bool = False, verbose: bool = False) -> Path:
     return out
 
 
+def bind_path() -> Path:
+    """The extension's file for this torch and this Python: it reads torch's objects, so another version's must not be loaded."""
+    import sysconfig
+    import torch
+    return LIB / ("kharon_bind-torch%s-%s.so" % (torch.__version__, sysconfig.get_config_var("SOABI")))
+
+
 def build_bind(force: bool = False) -> Path:
     import sysconfig
     import torch
     LIB.mkdir(exist_ok=True)
-    out = LIB / "kharon_bind.so"
+    out = bind_path()
     srcs = sorted((CSRC / "bind").glob("*.cpp"))
     if force or _newer(srcs, out):
         home = Path(torch.__file__).resolve().parent
@@ -121,8 +129,12 @@ def build_bind(force: bool = False) -> Path:
 
 
 def build_all(force: bool = False, verbose: bool = False):
-    build_bind(force)
-    return build_runtime(force), build_cuda(force, verbose)
+    libs = build_runtime(force), build_cuda(force, verbose)
+    try:
+        build_bind(force)
+    except (RuntimeError, OSError) as e:           # (torch without CUDA, no compiler for the host: the libraries above do not need it)
+        print("kharon_b200: the Python extension was not built, calls go through ctypes: %s" % e, file=sys.stderr)
+    return libs
 
 
 if __name__ == "__main__":

@@ -123,14 +123,14 @@ def cuda():
 
 
 def bind():
-    """The Python extension for small calls, with the addresses of the kernel library's entry points."""
+    """The Python extension for small calls, with the addresses of the kernel library's entry points.  Raises where it can be neither loaded nor built."""
     global _bind
     if _bind is None:
         lib = cuda()
         with _lock:
             if _bind is None:
                 import importlib.util
-                path = _build.LIB / "kharon_bind.so"
+                path = _build.bind_path()
                 if not path.exists():
                     path = _build.build_bind()
                 spec = importlib.util.spec_from_file_location("kharon_bind", str(path))

@@ -12,6 +12,7 @@ import array
 import ctypes as C
 import math
 import operator
+import warnings
 
 import torch
 
@@ -642,10 +643,24 @@ def _kv8_rows(name, x, width, dtype):
     return x.data_ptr(), st[0]
 
 
+_extension = None
+
+
 def _kv8_direct(t):
     """The extension that checks and launches a plain call on GPU tensors by itself (a call from Python takes 4 us of the host's time instead of 11), or
-    None: CPU tensors, and calls that a ``LaunchPlan`` records.  What it does not take as it is goes the way below it."""
-    return _native.bind() if _recording is None and t.is_cuda else None
+    None: CPU tensors, calls that a ``LaunchPlan`` records, and where it can be neither loaded nor built (said once).  What it does not take as it is goes the
+    way below it."""
+    global _extension
+    if _recording is not None or not t.is_cuda:
+        return None
+    if _extension is None:
+        try:
+            _extension = _native.bind()
+        except (ImportError, OSError, RuntimeError) as e:
+            _lib()                                 # (the kernels themselves are no option)
+            _extension = False
+            warnings.warn("kharon_b200: calls of the 8-bit cache's operators go through ctypes, 7 us more each: %s" % e, RuntimeWarning, stacklevel=3)
+    return _extension
 
 
 def _kv8_done(rc):
