@@ -21,7 +21,8 @@ from . import reference as ref
 
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_DGELU, EPI_RESID, EPI_GELU = range(7)
 
-#: number of native kernel launches issued through this module (bench.py reports it)
+#: number of native kernel launches issued through this module (bench.py reports it); a call whose number depends on its arguments counts as one (paged_prefill8: two kernels
+#: where runs of up to 64 tokens stand beside longer ones, again for every 1024 pieces)
 launch_count = 0
 
 
@@ -745,14 +746,19 @@ def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
 
 
 def copy_blocks8(kv, pairs, npairs):
-    """kv: [n_layer, n_blocks, H, record]; copies block pairs[2i] -> pairs[2i+1] in all layers."""
-    if kv.dtype != torch.uint8 or kv.dim() != 4 or not kv.is_contiguous() or pairs.dtype != torch.int32 or pairs.numel() < 2 * npairs or pairs.device != kv.device:
-        raise ValueError("copy_blocks8: contiguous uint8 [layers, blocks, H, record] and %d int32 pairs on its device are needed" % npairs)
+    """kv: [n_layer, n_blocks, H, record]; copies block pairs[2i] -> pairs[2i+1] in all layers.  The pairs are copied in no order: no block is written twice, or
+    written and read, in one call.  A pair out of range is recorded (status code 8) and skipped on a GPU, and an IndexError on the CPU."""
+    if (kv.dtype != torch.uint8 or kv.dim() != 4 or not kv.is_contiguous() or pairs.dtype != torch.int32 or not pairs.is_contiguous() or npairs < 0
+            or pairs.numel() < 2 * npairs or pairs.device != kv.device):
+        raise ValueError("copy_blocks8: contiguous uint8 [layers, blocks, H, record] and %d contiguous int32 pairs on its device are needed" % npairs)
     if npairs == 0:
         return
     if not kv.is_cuda:
-        for i in range(npairs):
-            kv[:, int(pairs[2 * i + 1])].copy_(kv[:, int(pairs[2 * i])])
+        flat = pairs.reshape(-1)[:2 * npairs].tolist()
+        if min(flat) < 0 or max(flat) >= kv.shape[1]:
+            raise IndexError("a block outside the cache")
+        for s, d in zip(flat[::2], flat[1::2]):
+            kv[:, d].copy_(kv[:, s])
         return
     if kv.get_device() != _current_device():
         raise ValueError("copy_blocks8: the tensors must be on the current device")
