@@ -10,9 +10,9 @@ from test_kv8_gpu import make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-# Rounding of the probabilities in runs of more than 64 tokens: half a step of 11 bits; half the smallest step is 2^-32 of the largest probability times 2^(difference of two
-# value rows' exponents), 14 at most.  Single tokens: two such terms, 2^-39 and the same difference.
-RUN, RUN_FLOOR, ONE_FLOOR = 2.0 ** -12, 2.0 ** -18, 2.0 ** -25
+# Rounding of the probabilities in runs of more than 64 tokens: they are f16, whose numbers in [1, 2) are 2^-10 apart, so half a step is 2^-11 of the value; half the smallest
+# step is 2^-32 of the largest probability times 2^(difference of two value rows' exponents), 14 at most.  Single tokens: two such terms, 2^-39 and the same difference.
+RUN, RUN_FLOOR, ONE_FLOOR = torch.finfo(torch.float16).eps / 2, 2.0 ** -18, 2.0 ** -25
 # What the single-token kernel leaves of it, or takes the positions again.
 ONE_EACH = 2.0 ** -29
 # What the kernel of long runs leaves of it, of the mean |v|, or computes the row again.
