@@ -148,14 +148,15 @@ extern "C" int kh_read_kv8(const void* kv, int n_blocks, int rec, void* k, void*
 // P' = 2^(s + ev - R + 14) with R the running maximum of s + ev, so that V's codes enter as they are.  P' goes in as two f16 terms, in the even and
 // the odd columns of B (22 bits; 2^-39 of the largest term): nothing is rounded to fewer bits than a sum of the same length in fp32 as long as the exponents of V
 // of positions with weight are not far below the largest, and as q' is exact.  Otherwise (value rows whose sizes differ by 2^10 and more, rows of zeros among them, with the
-// weight on the small ones; a query with an element 2^-29 times its largest) the warp takes its positions again, one by one in fp32: 1.2 ms for the 0.225 below, 38 us for the 17.
+// weight on the small ones; a query with an element 2^-29 times its largest) the warp takes its positions again, one by one in fp32: 1.2 ms for the 0.225 below, 38 us for the 16.
+// A score shares its fp32 number with ev, 63 at most: it is off by 2^-18 of a log2 unit at most.  Scores beyond fp32's range give NaN, as they do in a plain evaluation in fp32.
 // The block table and the exponents of a chunk are read by one lane per position and passed on by shuffles; the next chunk's K and V replace the
 // current ones in their registers as soon as those are used.
 // With `append` != 0 the item's first warp quantises the token's k and v, writes them into the cache and starts its sums with them.
 // The warps are merged once at the end: shared memory in warp order, then the cluster's shared memory in rank order (no scratch in global
 // memory, one launch).  Bound by memory for wide heads: 128 sequences of 1000 to 4096 positions, 16 heads of 128, 225 us (5.8 TB/s); by
-// issue slots and latency for narrower ones (128 sequences of 3000, 16 heads of 64: 148 us, 5.4 TB/s; of 32: 103 us, 3.9 TB/s); few items by three dependent trips to memory and
-// the join (16 heads of 64 at 16300 positions: 16.6 us, 2.0 TB/s).
+// issue slots and latency for narrower ones (128 sequences of 3000, 16 heads of 64: 149 us, 5.4 TB/s; of 32: 106 us, 3.8 TB/s); few items by three dependent trips to memory and
+// the join (16 heads of 64 at 16300 positions: 16.3 us, 2.1 TB/s).
 namespace {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -356,6 +357,7 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
   place(n1);
 #pragma unroll 1
   for (; j0 < n; j0 += step) {                     // uniform over the warp
+    if (j0 + lane < n) marks = min(marks, e);
     n1 = n2;
     n2 = look(j0 + 3 * step);
     float s[4];                                    // of positions 8 q + g
@@ -372,7 +374,6 @@ __device__ __forceinline__ void decode_partial(const Cache& c, const bf16* row, 
       s[2 * x] = a[0];
       s[2 * x + 1] = a[2];
     }
-    if (j0 + lane < n) marks = min(marks, e);
     fetch_k();
     float nev[4], tm = -INFINITY;                  // 2^-ev
 #pragma unroll
@@ -495,7 +496,13 @@ paged_attn8_k(const Cache c, const bf16* __restrict__ qkv, int ld, bf16* __restr
     if (least != NOTHING && !(l * pow2_of(least >> 8) >= 16.f)) {
       const volatile int* pos = c.pos;             // (read again: seldom used, and not kept in registers for it)
       const volatile int* slot = c.slot;
-      plain_partial<HD>(c, qkv + (size_t)t * ld + h * HD, h, pos[t], slot[t], scale, wi, W * S, append, R, l, o);
+      if constexpr (W == 1) {                      // (the row's output at once: fewer registers, 7.6 us for 8.1 at 704 heads of 128 and 40 positions)
+        __syncwarp();                              // (with `append` the token's own position has just been written)
+        attend_row8<HD>(c, qkv + (size_t)t * ld + h * HD, h, pos[t], slot[t], scale, out + (size_t)t * ldo + h * HD);
+        if (bad) report(c.err);
+        return;
+      } else
+        plain_partial<HD>(c, qkv + (size_t)t * ld + h * HD, h, pos[t], slot[t], scale, wi, W * S, append, R, l, o);
     }
   }
   if (bad) report(c.err);
