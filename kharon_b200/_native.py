@@ -1,4 +1,4 @@
-"""ctypes bindings to the two native libraries (host runtime, CUDA kernels).
+"""ctypes bindings to the two native libraries (host runtime, CUDA kernels), and the Python extension for small calls.
 
 ``rt()`` returns the host runtime (built on demand with g++; needs no GPU).  ``cuda()``
 returns the CUDA kernel library; on a machine with a GPU a missing library is a hard

@@ -14,7 +14,7 @@
 // ------------------------------------------------------------------------------- append and read back
 // A lane takes sixteen elements of a k row and of the v row beside it: HD / 16 lanes of a warp hold both and find their largest magnitudes with
 // shuffles; the exponents leave as one pair.  The lanes of a token (H HD / 16 of them) lie side by side; a CTA covers 256 of them, of several tokens
-// where one has fewer.  Bound by memory: 6018 tokens of 16 heads of 128 appended in 14.6 us (4.5 TB/s), 39800 positions read back in 74.7 us (5.8 TB/s).
+// where one has fewer.  Bound by memory: 6018 tokens of 16 heads of 128 appended in 14.6 us (4.5 TB/s), 39800 positions read back in 74.5 us (5.8 TB/s), as fp32 in 183 (4.5).
 // With k and v in different lanes (two byte stores for the exponents of a row) 23.6 and 132 us; the largest magnitude element by element instead of by packed
 // maxima 17.0; then two or four tokens a lane, fetched together: 16.7 and 80, 21.0 and 81.
 namespace {
@@ -155,7 +155,7 @@ extern "C" int kh_read_kv8(const void* kv, int n_blocks, int rec, void* k, void*
 // With `append` != 0 the item's first warp quantises the token's k and v, writes them into the cache and starts its sums with them.
 // The warps are merged once at the end: shared memory in warp order, then the cluster's shared memory in rank order (no scratch in global
 // memory, one launch).  Bound by memory for wide heads: 128 sequences of 1000 to 4096 positions, 16 heads of 128, 225 us (5.8 TB/s); by
-// issue slots and latency for narrower ones (128 sequences of 3000, 16 heads of 64: 149 us, 5.4 TB/s; of 32: 106 us, 3.8 TB/s); few items by three dependent trips to memory and
+// issue slots and latency for narrower ones (128 sequences of 3000, 16 heads of 64: 149 us, 5.4 TB/s; of 32: 106 us, 3.8 TB/s; of 16: 92 us, 2.3 TB/s); few items by three dependent trips to memory and
 // the join (16 heads of 64 at 16300 positions: 16.3 us, 2.1 TB/s).
 namespace {
 
@@ -629,7 +629,8 @@ extern "C" int kh_paged_attn8(const void* qkv, int ld, void* kv, int n_blocks, i
 }
 
 // ------------------------------------------------------------------------------- block copies
-// Whole blocks (all heads' records) src -> dst in every layer: the device half of copy-on-write.
+// Whole blocks (all heads' records) src -> dst in every layer: the device half of copy-on-write.  A CTA a block and layer, bound by memory for many pairs: 24 layers, blocks of
+// 16 positions and 16 heads of 64, one pair 4.7 us, 256 pairs 72 us (5.7 TB/s).
 __global__ void __launch_bounds__(128) copy_blocks8_k(uint8_t* __restrict__ kv, const int* __restrict__ pairs, size_t block_bytes, size_t layer_bytes,
                                                       int n_blocks, int* err) {
   pdl_wait();

@@ -329,8 +329,9 @@ paged_short8_k(const __grid_constant__ Pieces tiles, const __grid_constant__ Cac
 //
 // Heads of 128 are bound by the tensor core (its operands' trips through shared memory) and the exponentials together, each two thirds of the
 // time on the SMs in use: 2048 tokens behind 14300 positions, 16 heads, 273 us (942 TFLOP/s; 128 items on 148 SMs), four turns of 384 to 640 tokens behind 1500 to 4000
-// 83 us (760).  Narrower heads are bound by the exponentials and by the latency of a tile's way through the roles: eight prompts of 1024 tokens, 16
-// heads of 64, 58 us (296 TFLOP/s); short prompts by an item's set-up, some 4 us: six of 403 to 1001 tokens 32.4 us, 1024 (run of 128, head) items 33 us.
+// 82.5 us (765).  Narrower heads are bound by the exponentials and by the latency of a tile's way through the roles: eight prompts of 1024 tokens, 16
+// heads of 64, 58 us (296 TFLOP/s); short prompts by an item's set-up, some 4 us: six of 403 to 1001 tokens 33.4 us, 1024 (run of 128, head) items 33.5 us.
+// Rows done anew cost a warp each over their whole context: all rows of the first example 91 ms, of the second 19, of the prompts 2.
 namespace {
 constexpr int CH_MAX = 1024;
 struct Runs { int row0[CH_MAX]; uint16_t n[CH_MAX]; };

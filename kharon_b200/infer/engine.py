@@ -40,8 +40,8 @@ class InferEngine:
         """``kv8``: keys and values are kept in 8 bits (``ops.append_kv8``): half the cache and half the bytes that attention over long contexts
         reads, for values that are off by up to 2^-4.  Every token, prompts' too, attends to the cache as it is kept, however steps are composed.
         Decode steps take the kernel chain, the persistent kernel reads a bf16 cache: for long contexts and many sequences.  tok/s, bf16 / 8 bits:
-        L8 d2048, 3000 positions, G = 1 1144 / 1205, 32 7200 / 10530, with a shared prefix 64 19763 / 41032; L24 d1024, 128 to 384 positions, G = 8
-        17754 / 4916 (the chain), 32 30558 / 28649."""
+        L8 d2048, 3000 positions, G = 1 1144 / 1206, 32 7200 / 10405, with a shared prefix 64 19763 / 41853; L24 d1024, 128 to 384 positions, G = 8
+        17754 / 4909 (the chain), 32 30558 / 28518: up to 32 short sequences the bf16 cache is the faster one."""
         cfg = model.cfg
         self.model, self.cfg = model, cfg
         self.dev, self.dt = model.device, model.dtype

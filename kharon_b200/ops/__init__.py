@@ -704,7 +704,8 @@ def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=
     """``paged_attn`` over the 8-bit cache: causal attention of each listed token over positions 0..pos of its own sequence as the cache
     holds them.  ``append``: the kernel first quantises and stores each token's own k, v (valid when no two listed tokens belong to
     one sequence, i.e. decode steps); otherwise ``append_kv8`` must have run.  Few tokens over long contexts: the keys of a
-    token are shared out to the thread blocks of a cluster; no workspace."""
+    token are shared out to the thread blocks of a cluster; no workspace.  Sums and probabilities have fp32's precision, or 2^-29 of sum |v|; scores beyond
+    fp32's range give NaN."""
     b = _kv8_direct(kv)
     if b and _kv8_done(b.paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append)):
         return
@@ -722,7 +723,10 @@ def paged_attn8(qkv, kv, out, pos, slot, btab, bs, H, hd, ntok, max_ctx, append=
 
 def paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx):
     """``paged_prefill`` over the 8-bit cache: ``paged_attn8`` for runs of consecutive positions of one sequence each,
-    ``runs = [(first row, length), ...]``, whose K/V are in the cache already (``append_kv8``).  Head widths 32, 64 and 128."""
+    ``runs = [(first row, length), ...]``, whose K/V are in the cache already (``append_kv8``).  Head widths 32, 64 and 128.  In long runs probabilities are
+    rounded to f16 (half a step 2^-11 of the value, or 2^-9 of the mean |v| at most where scores and values of very different sizes meet) and scores are off by up to
+    2^-12; short ones over short contexts keep fp32's precision.  Rows that would lose more (key or value rows of a sequence of very different sizes, scores
+    that could pass 2^23) are computed again in fp32, which is slow."""
     b = _kv8_direct(kv)
     if b and _kv8_done(b.paged_prefill8(qkv, kv, out, pos, slot, btab, bs, H, hd, runs, max_ctx)):
         return
