@@ -132,7 +132,7 @@ def build_all(force: bool = False, verbose: bool = False):
     libs = build_runtime(force), build_cuda(force, verbose)
     try:
         build_bind(force)
-    except (RuntimeError, OSError) as e:           # (torch without CUDA, no compiler for the host: the libraries above do not need it)
+    except (ImportError, OSError, RuntimeError) as e:           # (torch without CUDA, no compiler for the host: the libraries above do not need it)
         print("kharon_b200: the Python extension was not built, calls go through ctypes: %s" % e, file=sys.stderr)
     return libs
 

@@ -11,7 +11,7 @@ from test_kv8_gpu import make
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 # Rounding of the probabilities in runs of more than 64 tokens: they are f16, whose numbers in [1, 2) are 2^-10 apart, so half a step is 2^-11 of the value; half the smallest
-# step is 2^-32 of the largest probability times 2^(difference of two value rows' exponents), 14 at most.  Single tokens: two such terms, 2^-39 and the same difference.
+# step is 2^-32 of the largest probability times 2^(difference of two value rows' exponents), 14 at most as `make` draws them.  Single tokens: two such terms, 2^-39.
 RUN, RUN_FLOOR, ONE_FLOOR = torch.finfo(torch.float16).eps / 2, 2.0 ** -18, 2.0 ** -25
 # What the single-token kernel leaves of it, or takes the positions again.
 ONE_EACH = 2.0 ** -29
