@@ -97,16 +97,17 @@ struct Sum {
 };
 __device__ __forceinline__ uint32_t top8(const uint4& v) { return max2(max2(v.x, v.y), max2(v.z, v.w)); }
 // What a row's gradient is made of: k exp(x - m), k = -slope / sum.  The size of k is a further term of the exponent where that stays below 96 and so loses less than 2^-17 (of a
-// result that is rounded to 2^-8), with f = 0 or -0 for its sign; else f = k.  Results below 2^-126 are 0 in the first form.
+// result that is rounded to 2^-8), with f = 0 or -0 for its sign; else f is k, or k 2^-BELOW, and never 0.  Results below 2^-126 are 0 in the first form, exponentials in the second.
 struct Shape {
   float a, b, f;
 };
 __device__ __forceinline__ Shape shape_of(float m, float k) {
   const Scale s = scale_of(m);
-  if (k == 0.f) return {s.a, -INFINITY, 0.f};
-  const float b = s.b + log2f(fabsf(k));
-  if (!is_far(m) && fabsf(b) <= 96.f) return {s.a, b, copysignf(0.f, k)};
-  return is_far(m) ? Shape{s.a, s.b, k} : Shape{s.a, s.b + BELOW, k * exp2f(-BELOW)};          // (here an exponential below 2^-126 is 0)
+  const bool far = is_far(m);
+  const float b = s.b + log2f(fabsf(k)), f = far ? k : k * exp2f(-BELOW);
+  if (!far && fabsf(b) <= 96.f) return {s.a, b, copysignf(0.f, k)};
+  if (f == 0.f) return {s.a, -INFINITY, 0.f};              // k = 0, or of the smallest fp32 numbers, whose product is 0 in any bf16 column: the first form, with nothing in it
+  return {s.a, far ? s.b : s.b + BELOW, f};
 }
 template <bool FUSED>
 __device__ __forceinline__ uint4 grad8(const uint4& v, const Shape& g) {
