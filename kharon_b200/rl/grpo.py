@@ -179,16 +179,21 @@ class GRPOTrainer:
 
     heartbeat = None        # utils.watchdog.Heartbeat of the job, when the entry point set one up
 
-    def _sync_grads(self):
+    def _sum_ranks(self, t, what):
+        """Sum of ``t`` over the data-parallel ranks, in place; a dead rank is an exception where there is a heartbeat."""
         if self.dp > 1:
             if self.heartbeat is not None:
                 from ..utils.watchdog import guarded
                 self.heartbeat.check()
-                guarded(dist.all_reduce(self.policy.params.g, group=self.dp_group, async_op=True), self.heartbeat,
-                        timeout_s=120.0, group=self.dp_group, what="gradient all-reduce")
+                guarded(dist.all_reduce(t, group=self.dp_group, async_op=True), self.heartbeat,
+                        timeout_s=120.0, group=self.dp_group, what="%s all-reduce" % what)
             else:
-                dist.all_reduce(self.policy.params.g, group=self.dp_group)
-            self.policy.params.g.div_(self.dp)
+                dist.all_reduce(t, group=self.dp_group)
+        return t
+
+    def _sync_grads(self):
+        if self.dp > 1:
+            self._sum_ranks(self.policy.params.g, "gradient").div_(self.dp)
 
     def sft_step(self):
         rows = []
@@ -264,7 +269,7 @@ class GRPOTrainer:
 
     def dpo_step(self, step: int):
         """One update of the preference loss on a rollout batch: of each prompt's G samples (an even number), ordered by reward, the first against the last and so on; pairs of
-        equal reward do not count."""
+        equal reward do not count.  The loss is the mean over the pairs of all data-parallel ranks; where none counts there is no update."""
         if self.G % 2:
             raise ValueError("dpo_step: an even number of samples of each prompt is needed, not %d" % self.G)
         m, B, T, G, P = self.policy, self.B, self.T, self.G, self.B // 2
@@ -275,13 +280,18 @@ class GRPOTrainer:
         rew = self.h_rew[order]
         counts = (rew[0::2] > rew[1::2]).float()
         n = float(counts.sum())
+        if self.dp > 1:
+            n = float(self._sum_ranks(torch.tensor([n], device=self.device), "number of pairs"))
+        self.stats = dict(stats, loss=0.0, pairs=n, pair_accuracy=0.0)
+        if n == 0:
+            return self._share_stats(["mean_reward"])
         self._fill_rows([rows[i] for i in order])
         self._mask_targets()
         if self.pairs is None:
             self.pairs = dict(starts=torch.arange(0, B * T + 1, T, dtype=torch.int32, device=self.device), work=ops.preference_work(B * T, P, self.device),
                               weight=torch.zeros(P, device=self.device), loss=torch.zeros(P, device=self.device), margin=torch.zeros(P, device=self.device))
         q = self.pairs
-        q["weight"].copy_(counts / max(n, 1.0))
+        q["weight"].copy_(counts * self.dp / n)                                  # (the ranks' gradients are averaged)
         self.ref.set_input(self.h_idx, self.h_tgt)
         self.ref.forward(compute_loss=False)
         self.ref.gather_logp(self.d_ref)
@@ -291,6 +301,6 @@ class GRPOTrainer:
             logits, V, tgt, q["starts"], ref_logp=self.d_ref, beta=self.dpo_beta, weight=q["weight"], loss=q["loss"], margin=q["margin"], dlogits=logits,
             work=q["work"]))
         self._update()
-        margin, on = q["margin"].cpu(), counts > 0
-        self.stats = dict(stats, loss=float(q["loss"].sum()), pairs=n, pair_accuracy=float((margin[on] > 0).float().mean()) if n else 0.0)
-        return self._share_stats(["mean_reward", "loss", "pairs", "pair_accuracy"])
+        ordered = float((q["margin"].cpu()[counts > 0] > 0).sum())
+        self.stats.update(loss=float(q["loss"].sum()), pair_accuracy=ordered * self.dp / n)
+        return self._share_stats(["mean_reward", "loss", "pair_accuracy"])
