@@ -87,7 +87,7 @@ class GRPOTrainer:
                  beta=0.02, device="cuda", dtype=torch.bfloat16, dp_group=None, dp_rank=0, dp=1, seed=1337,
                  task_seed=20260530, inner=1, clip_eps=0.0, max_norm=0.0, dpo_beta=0.1):
         """``inner`` updates on each rollout batch, with the ratio to the policy that sampled it held within 1 -+ ``clip_eps`` (0 with one update: the
-        reference's step); ``max_norm`` > 0 bounds the gradient's norm; ``dpo_beta``: the preference loss's."""
+        reference's step); ``max_norm`` > 0 bounds the gradient's norm in every update, the supervised ones too; ``dpo_beta``: the preference loss's."""
         if inner < 1 or not 0 <= clip_eps <= 1 or not max_norm >= 0 or (inner > 1 and clip_eps == 0):
             raise ValueError("inner=%s, clip_eps=%s (0 to 1, above 0 for several updates), max_norm=%s" % (inner, clip_eps, max_norm))
         self.inner, self.clip_eps, self.max_norm, self.dpo_beta = inner, clip_eps, max_norm, dpo_beta
@@ -144,14 +144,14 @@ class GRPOTrainer:
         tg[:, :self.task.plen - 1] = -1
         tg[:, -1] = -1
 
-    def _update(self):
+    def _update(self, lr):
         """Gradient exchange, bound and AdamW step."""
         self._sync_grads()
         factor = None
         if self.grad_list is not None:
             ops.grad_norm(self.grad_list, self.norm_out, max_norm=self.max_norm)
             factor = self.norm_out[1:]
-        self.policy.adamw_step(self.rllr, 0.9, 0.95, 1e-8, 0.0, factor=factor)
+        self.policy.adamw_step(lr, 0.9, 0.95, 1e-8, 0.0, factor=factor)
 
     def _rollout(self, step):
         """Samples G completions of each of this step's prompts: (rows of tokens in prompt order, rewards in ``h_rew``, statistics)."""
@@ -205,8 +205,7 @@ class GRPOTrainer:
         m.set_input(self.h_idx, self.h_tgt)
         m.forward(compute_loss=False)
         m.backward(loss_scale=1.0)
-        self._sync_grads()
-        m.adamw_step(self.lr, 0.9, 0.95, 1e-8, 0.0)
+        self._update(self.lr)
         return m.loss()
 
     def snapshot_reference(self):
@@ -239,7 +238,7 @@ class GRPOTrainer:
         p_ref = ref.gather_prob()
         ops.grpo_coef(self.d_adv, self.d_pcur, p_ref, B, T, task.plen - 1, T - 2, self.beta, self.d_coef)
         m.backward(coef=self.d_coef)
-        self._update()
+        self._update(self.rllr)
         self.stats = stats
         return self._share_stats(["mean_reward"])
 
@@ -260,7 +259,7 @@ class GRPOTrainer:
             m.backward(head_loss=lambda logits, V, tgt: ops.policy_loss(
                 logits, V, tgt, self.d_adv, old_logp=self.d_old if i else None, ref_logp=self.d_ref, clip_lo=self.clip_eps, clip_hi=self.clip_eps,
                 beta=self.beta, uniform=1.0 / n, rowloss=self.d_loss, logp=None if i else self.d_old, kl=self.d_kl, clipped=self.d_clip, dlogits=logits))
-            self._update()
+            self._update(self.rllr)
         for k, v in enumerate((self.d_loss, self.d_kl, self.d_clip)):
             ops.sum_f32(v, self.d_sum[k:k + 1], scale=1.0 if k == 0 else 1.0 / n)
         loss, kl, clipped = self.d_sum[:3].tolist()
@@ -300,7 +299,7 @@ class GRPOTrainer:
         m.backward(head_loss=lambda logits, V, tgt: ops.preference_loss(
             logits, V, tgt, q["starts"], ref_logp=self.d_ref, beta=self.dpo_beta, weight=q["weight"], loss=q["loss"], margin=q["margin"], dlogits=logits,
             work=q["work"]))
-        self._update()
+        self._update(self.rllr)
         ordered = float((q["margin"].cpu()[counts > 0] > 0).sum())
         self.stats.update(loss=float(q["loss"].sum()), pair_accuracy=ordered * self.dp / n)
         return self._share_stats(["mean_reward", "loss", "pair_accuracy"])
