@@ -3,7 +3,7 @@
 --log 20 --sft 200 --rllr 1e-4``.  Additions: ``--task add|reverse`` (single-digit addition as in
 the reference, or reversing a random 8-digit string with a 1/0 reward), ``--seq``, ``--clip-eps`` and
 ``--inner`` (updates per rollout batch with the clipped policy loss), ``--algo dpo`` with
-``--dpo-beta`` (preferences between a prompt's samples), ``--max-norm`` and data
+``--dpo-beta`` (preferences between a prompt's samples, one update per rollout batch), ``--max-norm`` and data
 parallelism over prompts when launched under torchrun (``--prompts`` is per step over all ranks).
 Log lines keep the reference's wording (grpo_train.c:181-182)."""
 from __future__ import annotations
@@ -27,11 +27,13 @@ def main(argv=None):
     hb_s = f.float("heartbeat", 0.0, "seconds after which a silent rank counts as dead (0 = off)")
     dev_flag = f.str("device", "")
     inner, clip_eps = f.int("inner", 1, "updates per rollout batch"), f.float("clip-eps", 0.0, "the ratio to the sampling policy stays within 1 -+ this (0 = one on-policy update)")
-    max_norm = f.float("max-norm", 0.0, "bound on the 2-norm of the gradient (0 = none)")
+    max_norm = f.float("max-norm", 0.0, "bound on the 2-norm of the gradient, in the supervised steps too (0 = none)")
     algo, dpo_beta = f.str("algo", "grpo", "grpo | dpo"), f.float("dpo-beta", 0.1)
     f.maybe_help()
     if algo not in ("grpo", "dpo"):
         raise SystemExit("--algo must be grpo or dpo")
+    if algo == "dpo" and (inner != 1 or clip_eps != 0):
+        raise SystemExit("--algo dpo makes one update of the preference loss a rollout batch: without --inner and --clip-eps")
     rank, world, device = init_distributed(dev_flag or None)
     task = ReverseTask() if task_name == "reverse" else AddTask()
     if NP % world:
