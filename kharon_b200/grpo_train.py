@@ -34,6 +34,8 @@ def main(argv=None):
         raise SystemExit("--algo must be grpo or dpo")
     if algo == "dpo" and (inner != 1 or clip_eps != 0):
         raise SystemExit("--algo dpo makes one update of the preference loss a rollout batch: without --inner and --clip-eps")
+    if algo == "dpo" and G % 2:
+        raise SystemExit("--algo dpo pairs a prompt's samples: --G must be even")
     rank, world, device = init_distributed(dev_flag or None)
     task = ReverseTask() if task_name == "reverse" else AddTask()
     if NP % world:
