@@ -596,8 +596,8 @@ def _bound(name, max_norm):
 
 def grad_norm(grads, out=None, *, max_norm=math.inf, sumsq=None):
     """2-norm over all tensors of a ``TensorList``, summed in 64 bits in a fixed order: ``out`` fp32 [2] receives (norm, factor), where the factor bounds the norm:
-    1 where norm <= ``max_norm``, else max_norm / norm, and NaN where the norm is not finite, at which ``adamw(factor=)`` leaves the step out.  ``sumsq`` (fp64 [1])
-    receives the sum of squares: a model that is spread over ranks sums it over them and takes ``clip_factor``."""
+    1 where norm <= ``max_norm``, else max_norm / norm, and NaN where the norm is not finite (in 64 bits: one beyond fp32's range shows as inf and has its factor), at which
+    ``adamw(factor=)`` leaves the step out.  ``sumsq`` (fp64 [1]) receives the sum of squares: a model that is spread over ranks sums it over them and takes ``clip_factor``."""
     grads._check("grad_norm", out=(out, 2, torch.float32), sumsq=(sumsq, 1, torch.float64))
     top = _bound("grad_norm", max_norm)
     if grads.index < 0:

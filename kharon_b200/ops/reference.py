@@ -234,7 +234,8 @@ def preference_loss(logits, V, target, starts, ref_logp, beta, smoothing, weight
 
 def clip_factor(sumsq, out, max_norm):
     norm = math.sqrt(float(sumsq)) if float(sumsq) >= 0 else math.nan
-    out[0], out[1] = norm, math.nan if not math.isfinite(norm) else 1.0 if norm <= max_norm else max_norm / norm
+    factor = math.nan if not math.isfinite(norm) else 1.0 if norm <= max_norm else max_norm / norm
+    out.view(-1).copy_(torch.tensor([norm, factor], dtype=torch.float64))         # (a norm beyond fp32's range shows as inf)
 
 
 def grad_norm(tensors, out, max_norm, sumsq):
