@@ -247,7 +247,7 @@ def grad_norm(tensors, out, max_norm, sumsq):
 
 
 def scale(src, dst, out):
-    f = float(out[1])
+    f = float(out.view(-1)[1])
     for s, d in zip(src, dst):
         d.view(-1).copy_(s.view(-1) if math.isnan(f) else s.view(-1).float() * f)
 

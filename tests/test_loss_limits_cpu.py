@@ -21,3 +21,10 @@ def test_norm_beyond_the_range_of_fp32(n):
     assert torch.equal(out, first)
     ops.clip_grads(ops.TensorList([t]), 1e38, out)
     assert float(t.double().norm()) == pytest.approx(1e38, rel=1e-6)
+
+
+def test_norm_and_factor_of_another_shape():
+    """``out`` is two values, whatever its shape."""
+    t, out = torch.full((4,), 2.0), torch.zeros(1, 2)
+    ops.clip_grads(ops.TensorList([t]), 1.0, out)
+    assert out.tolist() == [[4.0, 0.25]] and t.tolist() == [0.5] * 4
