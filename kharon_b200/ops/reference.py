@@ -162,6 +162,7 @@ def _log_probs(logits, V, target, on):
     lg = torch.where(on[:, None], logits[:, :V].double(), 0.0)
     ts = target.long().clamp(0, V - 1)
     lse = torch.logsumexp(lg, -1)
+    lse = torch.where(lse == math.inf, math.nan, lse)              # of a row with an infinite logit, whose softmax has inf - inf
     lp = lg.gather(1, ts[:, None])[:, 0] - lse
     return torch.where(on, lp, 0.0), lg, lse, ts
 

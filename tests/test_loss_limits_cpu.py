@@ -1,4 +1,4 @@
-"""The CPU's evaluation at the ends of the range: norms beyond fp32."""
+"""The CPU's evaluation at the ends of the range: norms beyond fp32, rows with an infinite logit."""
 import math
 
 import pytest
@@ -28,3 +28,24 @@ def test_norm_and_factor_of_another_shape():
     t, out = torch.full((4,), 2.0), torch.zeros(1, 2)
     ops.clip_grads(ops.TensorList([t]), 1.0, out)
     assert out.tolist() == [[4.0, 0.25]] and t.tolist() == [0.5] * 4
+
+
+INF = math.inf
+ROWS = [[INF, 0.0, 1.0, 2.0], [0.0, INF, -INF, INF], [-INF] * 4, [math.nan, 0.0, 1.0, 2.0], [0.0, math.nan, INF, 1.0]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [0, 1, 3])
+def test_rows_with_an_infinite_logit_are_nan(t, dtype):
+    """What log softmax gives, whatever the target, on a GPU too; the other rows are as without them."""
+    x = torch.cat([torch.tensor(ROWS), torch.tensor([[0.0, 1.0, 2.0, -INF]])]).to(dtype)
+    R, tgt = x.shape[0], torch.full((x.shape[0],), t, dtype=torch.int32)
+    for kw in (dict(), dict(old_logp=torch.full((R,), -1.0)), dict(old_logp=torch.full((R,), -1.0), ref_logp=torch.full((R,), -1.0), beta=0.5)):
+        out = {k: torch.zeros(R) for k in ("rowloss", "logp")}
+        grad = torch.zeros(R, 8, dtype=dtype)
+        ops.policy_loss(x, 4, tgt, torch.ones(R), dlogits=grad, **out, **kw)
+        assert bool(torch.isnan(out["logp"][:5]).all()) and bool(torch.isnan(out["rowloss"][:5]).all()) and bool(torch.isnan(grad[:5, :4]).all()) and not bool(grad[:, 4:].any())
+        assert float(out["logp"][5]) == pytest.approx(float(torch.log_softmax(x[5].float(), -1)[t]), rel=1e-6)
+    logp, loss, grad = torch.zeros(R), torch.zeros(R // 2), torch.zeros(R, 8, dtype=dtype)
+    ops.preference_loss(x, 4, tgt, torch.arange(R + 1, dtype=torch.int32), loss=loss, logp=logp, dlogits=grad)
+    assert bool(torch.isnan(logp[:5]).all()) and bool(torch.isnan(loss).all()) and bool(torch.isnan(grad[:5, :4]).all())
