@@ -40,6 +40,9 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {      // a NaN
 __device__ __forceinline__ uint32_t cut_word(uint32_t w, int k) { return k <= 0 ? NEG2 : k == 1 ? (w & 0xffffu) | 0xff800000u : w; }
 // -inf in the columns k.. of an 8-column piece
 __device__ __forceinline__ uint4 cut_from(const uint4& v, int k) { return make_uint4(cut_word(v.x, k), cut_word(v.y, k - 2), cut_word(v.z, k - 4), cut_word(v.w, k - 6)); }
+__device__ __forceinline__ uint32_t zero_word(uint32_t w, int k) { return k <= 0 ? 0u : k == 1 ? w & 0xffffu : w; }
+// 0 in the columns k.. of it (of a gradient: what cut_from leaves there times a slope that is not finite is NaN)
+__device__ __forceinline__ uint4 zero_from(const uint4& v, int k) { return make_uint4(zero_word(v.x, k), zero_word(v.y, k - 2), zero_word(v.z, k - 4), zero_word(v.w, k - 6)); }
 __device__ __forceinline__ uint32_t put_word(uint32_t w, int k, uint32_t b) { return k == 0 ? (w & 0xffff0000u) | b : k == 1 ? (w & 0xffffu) | b << 16 : w; }
 // the bits b in column k of it
 __device__ __forceinline__ uint4 put_bits(const uint4& v, int k, uint32_t b) {
@@ -325,6 +328,7 @@ __global__ void __launch_bounds__(256) policy_warp_k(Rows q, Policy a) {
         const int i = j * 32 + lane;
         if (i >= gv) continue;
         uint4 o = grad8(v[j], shape);
+        if (8 * i + 8 > q.V) o = zero_from(o, q.V - 8 * i);
         if (i == t >> 3) o = put_one(o, t & 7, at_t);
         store8(g, i, q.gcols, o);
       }
@@ -423,9 +427,8 @@ __global__ void __launch_bounds__(256, 4) policy_twice_k(Rows q, Policy a) {
   const Shape shape = shape_of(m, -inv);
   grad_pieces(gp, v, min(nv - (cut >= 0), q.gcols / 8), shape);
   if (cut >= 0 && lane == 0) {
-    uint4 y = v[cut];
-    y = cut_from(y, q.V - 8 * cut);
-    store8(g, cut, q.gcols, grad8(y, shape));
+    const uint4 y = v[cut];
+    store8(g, cut, q.gcols, zero_from(grad8(y, shape), q.V - 8 * cut));
   }
   __syncwarp();
   if (lane == 0) g[t] = __float2bfloat16(inv * rest);      // (behind the store of the piece)
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(64 * NP + 32, NP >= 8 ? 1 : 12 / NP) policy_ro
     }
   } else {
     // ---- gradients
-    const int gv = (q.gcols + 7) / 8, whole = min(n, q.gcols / 8 - v0);
+    const int gv = (q.gcols + 7) / 8, whole = min(n, q.gcols / 8 - v0), last = 8 * (v0 + n) > q.V ? n - 1 : n;     // (the piece that sticks out of the vocabulary apart)
     int k = 0, phase = 0;
     for (int base = 0; base < total; base += 32) {
       Block b;
@@ -646,8 +649,8 @@ __global__ void __launch_bounds__(64 * NP + 32, NP >= 8 ? 1 : 12 / NP) policy_ro
         const int tv = (o.t >> 3) - v0;
         for (int c = 0; c < nc; c++) {
           wait(full(k, c), phase);
-          grad_pieces(gp + c * CHUNK, here + c * CHUNK, min(CHUNK, whole - c * CHUNK), o.shape);
-          if (whole < n && c == nc - 1 && lane == 0) store8(g, v0 + whole, q.gcols, grad8(here[whole], o.shape));
+          grad_pieces(gp + c * CHUNK, here + c * CHUNK, min(CHUNK, last - c * CHUNK), o.shape);
+          if (last < n && c == nc - 1 && lane == 0) store8(g, v0 + last, q.gcols, zero_from(grad8(here[last], o.shape), q.V - 8 * (v0 + last)));
           fence_proxy_async_smem();
           __syncwarp();
           if (tv >> 8 == c && tv < n && lane == 0) g[o.t] = __float2bfloat16(o.at_target);                      // (behind the store of the piece)
@@ -979,6 +982,7 @@ __global__ void __launch_bounds__(512) pair_k(Rows q, Pairs b, int C, int* err) 
           const int at = j * 32 + lane;
           if (at >= gv) continue;
           uint4 o = grad8(v[j], shape);
+          if (8 * at + 8 > q.V) o = zero_from(o, q.V - 8 * at);
           if (at == t >> 3) o = put_one(o, t & 7, at_t);
           store8(g, at, q.gcols, o);
         }
@@ -1287,9 +1291,8 @@ __global__ void __launch_bounds__(32 * (WORKERS + 2), 1) stream_k(Rows q, Policy
           const Shape shape = {x.kind == FAR ? 1.f : LOG2E, x.b, x.f};
           grad_pieces(gp, v, min(whole, cut >= 0 ? n - 1 : n), shape);
           if (cut >= 0 && lane == 0) {
-            uint4 y = v[n - 1];
-            y = cut_from(y, q.V - 8 * (m0 + n - 1));
-            store8(g, m0 + n - 1, q.gcols, grad8(y, shape));
+            const uint4 y = v[n - 1];
+            store8(g, m0 + n - 1, q.gcols, zero_from(grad8(y, shape), q.V - 8 * (m0 + n - 1)));
           }
           __syncwarp();
           if (tv >= 0 && tv < n && lane == 0) g[x.t] = __float2bfloat16(x.at_t);          // (behind the store of the piece)

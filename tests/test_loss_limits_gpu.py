@@ -1,4 +1,6 @@
-"""Losses of a policy at the lower end of fp32's range: slopes, and slopes times a row's scale, among and below the smallest normal numbers."""
+"""Losses of a policy at the ends of the range: slopes among and below the smallest normal fp32 numbers, rows with an infinite logit."""
+import math
+
 import pytest
 import torch
 
@@ -49,4 +51,22 @@ def test_preference_loss_with_slopes_at_the_end_of_the_range(V, ld):
     for kw in (dict(beta=1.0), dict(beta=1.0, uniform=0.125), dict(beta=1.0, uniform=3.0)):
         out, want = run_preference(x, V, t, starts, **kw), preference(x, V, t, starts, **kw)
         check_preference(out, want, V, starts, kw["beta"], 0.0, None, kw.get("uniform", 1.0), HALF)
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("V,ld", [(8, 8), (250, 256), (1003, 1008), (2040, 2040), (5000, 5000), (9001, 9008), (50257, 50304), (128256, 128256)])
+def test_rows_with_an_infinite_logit_are_nan(V, ld):
+    """As on the CPU: NaN in all that is written of the row, whatever its target, and in its pair's other row by the pair's slope; zeros beyond the vocabulary."""
+    x = torch.zeros(10, ld, device=DEV, dtype=torch.bfloat16)
+    x[0, 3], x[1, V - 1], x[2, 0], x[3, :V], x[4, V // 2] = math.inf, math.inf, math.inf, -math.inf, math.nan
+    x[1, 4] = -math.inf
+    t = torch.tensor([3, 0, 1, 2, V - 1, 0, 0, 0, 0, 0], device=DEV, dtype=torch.int32)
+    old = torch.full((10,), -8.0, device=DEV)
+    for kw in (dict(), dict(old=old), dict(old=old, ref=old, beta=0.5)):
+        out = run_policy(x, V, t, torch.ones(10, device=DEV), **kw)
+        assert all(bool(torch.isnan(out[k][:5]).all()) and bool(torch.isfinite(out[k][5:]).all()) for k in ("loss", "logp"))
+        assert bool(torch.isnan(out["grad"][:5, :V]).all()) and bool(torch.isfinite(out["grad"][5:]).all()) and not bool(out["grad"][:, V:].any())
+    out = run_preference(x, V, t, starts_of([1] * 10))
+    assert bool(torch.isnan(out["logp"][:5]).all()) and bool(torch.isnan(out["loss"][:3]).all()) and bool(torch.isnan(out["grad"][:6, :V]).all())
+    assert bool(torch.isfinite(out["loss"][3:]).all()) and bool(torch.isfinite(out["grad"][6:]).all()) and not bool(out["grad"][:, V:].any())
     ops.check_device_status()
