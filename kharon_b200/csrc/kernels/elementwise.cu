@@ -1093,11 +1093,22 @@ extern "C" int kh_sum_f32(const void* x, long n, float scale, void* out, int acc
 // One pass over flat fp32 buffers: g' = g * grad_scale; m, v moments; decoupled weight decay
 // on every element; writes the fp32 master, the bf16 compute copy (optional) and clears the
 // gradient (optional) so that the next step can accumulate into it.  FACTOR: g is also multiplied by *factor; NaN there leaves
-// the step out (the gradient is cleared all the same).
-template <bool FACTOR>
+// the step out (the gradient is cleared all the same).  COUNTED: the bias corrections are those of as many steps fewer as *taken.left_out says.
+struct Taken {
+  const int* left_out;
+  int step;
+  double b1, b2;
+};
+__device__ __forceinline__ float bias_correction(double beta, int steps) {                 // 1 - beta^steps, rounded once
+  double p = 1.0;
+  for (int n = max(steps, 1); n; n >>= 1, beta *= beta)
+    if (n & 1) p *= beta;
+  return (float)(1.0 - p);
+}
+template <bool FACTOR, bool COUNTED>
 __global__ void adamw_k(float* __restrict__ p, float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
                         bf16* __restrict__ pb, long n, float lr, float b1, float b2, float eps, float wd, float bc1,
-                        float bc2, float grad_scale, int zero_grad, const float* __restrict__ factor) {
+                        float bc2, float grad_scale, int zero_grad, const float* __restrict__ factor, Taken taken) {
   pdl_wait();
   pdl_launch_dependents();
   const long i4 = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
@@ -1110,12 +1121,17 @@ __global__ void adamw_k(float* __restrict__ p, float* __restrict__ g, float* __r
   }
   if (FACTOR) {
     const float f = *factor;
+    const int left_out = COUNTED ? *taken.left_out : 0;
     if (f != f) {
       if (zero_grad)
         for (long i = i4; i < n && i < i4 + 4; i++) g[i] = 0.f;
       return;
     }
     grad_scale *= f;
+    if (COUNTED && left_out > 0) {           // (few runs have any; a power takes 20 squarings at a million steps)
+      bc1 = bias_correction(taken.b1, taken.step - left_out);
+      bc2 = bias_correction(taken.b2, taken.step - left_out);
+    }
   }
   if (whole) {
     float* pa = &pp.x; float* ga = &gg.x; float* ma = &mm.x; float* va = &vv.x;
@@ -1153,20 +1169,26 @@ extern "C" int kh_adamw(void* p, void* g, void* m, void* v, void* pb, long n, fl
     kh_set_error("adamw: buffers must be 16-byte aligned");
     return -1;
   }
-  KH_LAUNCH(adamw_k<false>, cdiv(cdiv(n, 4), 256), 256, 0, (cudaStream_t)stream, (float*)p, (float*)g, (float*)m, (float*)v, (bf16*)pb,
-                                                                   n, lr, b1, b2, eps, wd, bc1, bc2, grad_scale, zero_grad, nullptr);
+  KH_LAUNCH((adamw_k<false, false>), cdiv(cdiv(n, 4), 256), 256, 0, (cudaStream_t)stream, (float*)p, (float*)g, (float*)m, (float*)v, (bf16*)pb,
+                                                                   n, lr, b1, b2, eps, wd, bc1, bc2, grad_scale, zero_grad, nullptr, Taken{});
   KH_LAUNCH_CHECK("adamw");
   return 0;
 }
 extern "C" int kh_adamw_factor(void* p, void* g, void* m, void* v, void* pb, long n, float lr, float b1, float b2, float eps, float wd, float bc1,
-                               float bc2, float grad_scale, int zero_grad, const void* factor, void* stream) {
+                               float bc2, float grad_scale, int zero_grad, const void* factor, const void* left_out, int step, double beta1, double beta2, void* stream) {
   if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15 || ((uintptr_t)pb & 7)) {
     kh_set_error("adamw: buffers must be 16-byte aligned");
     return -1;
   }
   if (n <= 0) return 0;
-  KH_LAUNCH(adamw_k<true>, cdiv(cdiv(n, 4), 256), 256, 0, (cudaStream_t)stream, (float*)p, (float*)g, (float*)m, (float*)v, (bf16*)pb,
-                                                                  n, lr, b1, b2, eps, wd, bc1, bc2, grad_scale, zero_grad, (const float*)factor);
+  const Taken taken = {(const int*)left_out, step, beta1, beta2};
+  const int grid = cdiv(cdiv(n, 4), 256);
+  if (left_out)
+    KH_LAUNCH((adamw_k<true, true>), grid, 256, 0, (cudaStream_t)stream, (float*)p, (float*)g, (float*)m, (float*)v, (bf16*)pb, n, lr, b1, b2, eps, wd, bc1, bc2, grad_scale,
+              zero_grad, (const float*)factor, taken);
+  else
+    KH_LAUNCH((adamw_k<true, false>), grid, 256, 0, (cudaStream_t)stream, (float*)p, (float*)g, (float*)m, (float*)v, (bf16*)pb, n, lr, b1, b2, eps, wd, bc1, bc2, grad_scale,
+              zero_grad, (const float*)factor, taken);
   KH_LAUNCH_CHECK("adamw");
   return 0;
 }

@@ -35,9 +35,10 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// norm and factor from the sum of squares
-__device__ __forceinline__ void put_norm(double sum, float max_norm, float* out) {
+// norm and factor from the sum of squares; a step that is to be left out is counted
+__device__ __forceinline__ void put_norm(double sum, float max_norm, float* out, int* left_out) {
   const double norm = sqrt(sum);
+  if (left_out && !isfinite(norm)) ++*left_out;
   out[0] = (float)norm;
   out[1] = !isfinite(norm) ? NAN : norm <= (double)max_norm ? 1.f : (float)((double)max_norm / norm);
 }
@@ -92,7 +93,7 @@ __device__ __forceinline__ void share_of(long pieces, long& k0, long& k1) {
   k0 = b * per + min(b, more);
   k1 = k0 + per + (b < more);
 }
-__global__ void __launch_bounds__(T, 4) norm_k(const Entry* table, int n, long pieces, int piece, float max_norm, double* work, float* out, double* sumsq) {
+__global__ void __launch_bounds__(T, 4) norm_k(const Entry* table, int n, long pieces, int piece, float max_norm, double* work, float* out, double* sumsq, int* left_out) {
   __shared__ double s_s[8];
   __shared__ long s_before[TABLE];
   __shared__ int s_last;
@@ -135,13 +136,13 @@ __global__ void __launch_bounds__(T, 4) norm_k(const Entry* table, int n, long p
     s = 0.0;
     for (int k = 0; k < 8; k++) s += s_s[k];
     if (sumsq) *sumsq = s;
-    if (out) put_norm(s, max_norm, out);
+    if (out) put_norm(s, max_norm, out, left_out);
   }
 }
-__global__ void clip_factor_k(const double* sumsq, float max_norm, float* out) {
+__global__ void clip_factor_k(const double* sumsq, float max_norm, float* out, int* left_out) {
   pdl_wait();
   pdl_launch_dependents();
-  put_norm(*sumsq, max_norm, out);
+  put_norm(*sumsq, max_norm, out, left_out);
 }
 // n elements of one type times f to another place, 16 bytes at a time where both allow it
 template <int E, typename V, typename F>
@@ -227,14 +228,14 @@ bool good(int n, long pieces, int piece) { return n >= 0 && pieces >= 0 && (piec
 extern "C" int kh_grad_share() { return SHARE; }
 extern "C" int kh_grad_piece(long shares) { return shares <= most_ctas() ? SHARE : FINE; }
 extern "C" long kh_grad_work_bytes() { return 16 + 8L * PARTS; }
-extern "C" int kh_grad_norm(const void* table, int n, long pieces, int piece, float max_norm, void* work, void* out, void* sumsq, void* stream) {
+extern "C" int kh_grad_norm(const void* table, int n, long pieces, int piece, float max_norm, void* work, void* out, void* sumsq, void* left_out, void* stream) {
   if (!good(n, pieces, piece)) { kh_set_error("grad_norm: a table of %d tensors, %ld pieces of %d bytes", n, pieces, piece); return -1; }
-  KH_LAUNCH(norm_k, grid_for(pieces, piece), T, 0, (cudaStream_t)stream, (const Entry*)table, n, pieces, piece, max_norm, (double*)work, (float*)out, (double*)sumsq);
+  KH_LAUNCH(norm_k, grid_for(pieces, piece), T, 0, (cudaStream_t)stream, (const Entry*)table, n, pieces, piece, max_norm, (double*)work, (float*)out, (double*)sumsq, (int*)left_out);
   KH_LAUNCH_CHECK("grad_norm");
   return 0;
 }
-extern "C" int kh_clip_factor(const void* sumsq, float max_norm, void* out, void* stream) {
-  KH_LAUNCH(clip_factor_k, 1, 1, 0, (cudaStream_t)stream, (const double*)sumsq, max_norm, (float*)out);
+extern "C" int kh_clip_factor(const void* sumsq, float max_norm, void* out, void* left_out, void* stream) {
+  KH_LAUNCH(clip_factor_k, 1, 1, 0, (cudaStream_t)stream, (const double*)sumsq, max_norm, (float*)out, (int*)left_out);
   KH_LAUNCH_CHECK("clip_factor");
   return 0;
 }

@@ -89,7 +89,8 @@ class TrainEngine:
                  fuse_microbatches=False, seed=1337, init="host", fused_comm=False, trace=False, heartbeat=None, pp_split=None, vocab_parallel=True,
                  defer_dw=None, eager_p2p=None, bucket_optimizer=True, sp=None, pp_fuse=1, max_norm=0.0):
         """``max_norm`` > 0 bounds the 2-norm of each step's gradient (over all parameters of the model, whatever the mesh): the norm has to be known
-        before any weight is updated, so the layers are not updated under the backward pass then, and ZeRO-1 reduces the gradients by the collective."""
+        before any weight is updated, so the layers are not updated under the backward pass then, and ZeRO-1 reduces the gradients by the collective.  A step whose norm is
+        not finite is left out, for the bias corrections too; ``model.step`` counts it, the step of a checkpoint doesn't."""
         from .utils.trace import Tracer
         self.mesh = mesh or Mesh.single()
         # The in-kernel collectives move bf16 activations / weights; an fp32 model (the oracle
@@ -217,6 +218,7 @@ class TrainEngine:
             self.grad_list = ops.TensorList(self._counted_grads())
             self.norm_out = torch.zeros(2, dtype=torch.float32, device=dev)        # norm of the last step's gradient, its factor
             self.sumsq = torch.zeros(1, dtype=torch.float64, device=dev)
+            self.model.left_out = torch.zeros(1, dtype=torch.int32, device=dev)
         self._opt_pending = False
         if self.bucketed:
             self.opt_stream = torch.cuda.Stream(self.device)
@@ -262,11 +264,11 @@ class TrainEngine:
         if self.grad_list is None:
             return None
         if self.mesh.world == 1:
-            ops.grad_norm(self.grad_list, self.norm_out, max_norm=self.max_norm)
+            ops.grad_norm(self.grad_list, self.norm_out, max_norm=self.max_norm, left_out=self.model.left_out)
         else:
             ops.grad_norm(self.grad_list, sumsq=self.sumsq)
             dist.all_reduce(self.sumsq)
-            ops.clip_factor(self.sumsq, self.norm_out, self.max_norm)
+            ops.clip_factor(self.sumsq, self.norm_out, self.max_norm, left_out=self.model.left_out)
         return self.norm_out[1:]
 
     def grad_norm(self) -> float:
@@ -487,7 +489,7 @@ class TrainEngine:
         lo, hi = self.lo, self.lo + self.shard
         wb = None if ps.wb is ps.w else ps.wb[lo:hi]
         ops.adamw(ps.w[lo:hi], self.g_shard, ps.m, ps.v, wb, lr=o["lr"], beta1=o["beta1"], beta2=o["beta2"],
-                  eps=o["eps"], wd=o["wd"], step=m.step, grad_scale=1.0, zero_grad=False, factor=self._bound_gradient())
+                  eps=o["eps"], wd=o["wd"], step=m.step, grad_scale=1.0, zero_grad=False, factor=self._bound_gradient(), left_out=m.left_out)
         ps.g.zero_()
         # only the compute copy travels; the fp32 master stays sharded
         tgt_full = ps.wb if ps.wb is not ps.w else ps.w

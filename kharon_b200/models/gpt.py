@@ -164,6 +164,7 @@ class GPT:
         self.params = ParamStore(cfg, device, dtype, tp, self.has_head, pad_to=4 * dp if dp > 1 else 1, alloc=alloc)
         self.params.alloc_moments()
         self.step = 0
+        self.left_out = None          # int32 [1] on the device where the gradient is bounded: how many of the steps were left out
         self.Vp = _pad64(cfg.vocab)
         # deferred weight gradients: backward only stores each layer's output gradients; flush_dw()
         # forms all weight and bias gradients of the step in one pass over every micro-batch
@@ -674,7 +675,8 @@ class GPT:
         """Fused AdamW over the flat arena (src/core/adamw.c:9-16), or over elements [lo, hi) of it; also
         refreshes the bf16 compute copy and clears the gradients for the next accumulation.  The update
         is elementwise, so any partition of the arena into ranges gives the same bits as one sweep.
-        ``factor``: the device value by which ``ops.grad_norm`` bounds the gradient."""
+        ``factor``: the device value by which ``ops.grad_norm`` bounds the gradient (with ``left_out``, if the model has
+        that count, for the bias corrections)."""
         if advance:
             self.step += 1
         ps = self.params
@@ -683,7 +685,8 @@ class GPT:
             return
         wb = None if ps.wb is ps.w else ps.wb[lo:hi]
         ops.adamw(ps.w[lo:hi], ps.g[lo:hi], ps.m[lo:hi], ps.v[lo:hi], wb, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
-                  wd=wd, step=self.step, grad_scale=grad_scale, zero_grad=True, factor=factor)
+                  wd=wd, step=self.step, grad_scale=grad_scale, zero_grad=True, factor=factor,
+                  left_out=self.left_out if factor is not None else None)
 
     def layer_range(self, l):
         """Elements [lo, hi) of the flat arena that belong to layer l (alignment gaps included)."""
@@ -697,13 +700,16 @@ class GPT:
         from ..utils import ckpt
         ps = self.params
         m, v = moments if moments is not None else (ps.m[:ps.n_flat], ps.v[:ps.n_flat])
-        ckpt.save(path, self.cfg.as_list(), self.step, rng_state, ps.w[:ps.n_flat], m, v)
+        step = self.step - (int(self.left_out) if self.left_out is not None else 0)        # the updates that the moments have seen
+        ckpt.save(path, self.cfg.as_list(), step, rng_state, ps.w[:ps.n_flat], m, v)
 
     def load(self, path, moments=None):
         from ..utils import ckpt
         ps = self.params
         m, v = moments if moments is not None else (ps.m[:ps.n_flat], ps.v[:ps.n_flat])
         self.step, rng = ckpt.load(path, self.cfg.as_list(), ps.w[:ps.n_flat], m, v)
+        if self.left_out is not None:
+            self.left_out.zero_()
         ps.sync_compute_copy()
         return rng
 

@@ -594,26 +594,36 @@ def _bound(name, max_norm):
     return float(max_norm)
 
 
-def grad_norm(grads, out=None, *, max_norm=math.inf, sumsq=None):
+def _count_of(name, left_out, like):
+    if left_out is not None and (left_out.dtype is not torch.int32 or left_out.numel() != 1 or left_out.get_device() != like.get_device()):
+        raise ValueError("%s: left_out must be int32 [1] on the same device" % name)
+
+
+def grad_norm(grads, out=None, *, max_norm=math.inf, sumsq=None, left_out=None):
     """2-norm over all tensors of a ``TensorList``, summed in 64 bits in a fixed order: ``out`` fp32 [2] receives (norm, factor), where the factor bounds the norm:
     1 where norm <= ``max_norm``, else max_norm / norm, and NaN where the norm is not finite (in 64 bits: one beyond fp32's range shows as inf and has its factor), at which
-    ``adamw(factor=)`` leaves the step out.  ``sumsq`` (fp64 [1]) receives the sum of squares: a model that is spread over ranks sums it over them and takes ``clip_factor``."""
-    grads._check("grad_norm", out=(out, 2, torch.float32), sumsq=(sumsq, 1, torch.float64))
+    ``adamw(factor=)`` leaves the step out.  ``sumsq`` (fp64 [1]) receives the sum of squares: a model that is spread over ranks sums it over them and takes ``clip_factor``.
+    ``left_out`` (int32 [1], 0 at first) goes up by 1 where the factor is NaN: the count that ``adamw(left_out=)`` wants."""
+    grads._check("grad_norm", out=(out, 2, torch.float32), sumsq=(sumsq, 1, torch.float64), left_out=(left_out, 1, torch.int32))
     top = _bound("grad_norm", max_norm)
+    if out is None and left_out is not None:
+        raise ValueError("grad_norm: left_out counts factors, which need out")
     if grads.index < 0:
-        return ref.grad_norm(grads.tensors, out, top, sumsq)
-    _call_keeping(grads, _lib().kh_grad_norm, 1, grads.table.data_ptr(), grads.entries, grads.pieces, grads.piece, top, grads.work.data_ptr(), _p(out), _p(sumsq), _stream())
+        return ref.grad_norm(grads.tensors, out, top, sumsq, left_out)
+    _call_keeping(grads, _lib().kh_grad_norm, 1, grads.table.data_ptr(), grads.entries, grads.pieces, grads.piece, top, grads.work.data_ptr(), _p(out), _p(sumsq), _p(left_out),
+                  _stream())
 
 
-def clip_factor(sumsq, out, max_norm):
-    """``out`` = (norm, factor) of ``grad_norm`` from a sum of squares (fp64 [1], on the device)."""
+def clip_factor(sumsq, out, max_norm, *, left_out=None):
+    """``out`` = (norm, factor) of ``grad_norm`` from a sum of squares (fp64 [1], on the device); ``left_out`` as there."""
     top = _bound("clip_factor", max_norm)
     if (sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or out.dtype is not torch.float32 or out.numel() != 2 or not out.is_contiguous()
             or out.get_device() != sumsq.get_device() or (sumsq.is_cuda and sumsq.get_device() != _current_device())):
         raise ValueError("clip_factor: fp64 [1] and fp32 [2] on the current device are needed")
+    _count_of("clip_factor", left_out, sumsq)
     if not sumsq.is_cuda:
-        return ref.clip_factor(sumsq, out, top)
-    _call(_lib().kh_clip_factor, 1, sumsq.data_ptr(), top, out.data_ptr(), _stream())
+        return ref.clip_factor(sumsq, out, top, left_out)
+    _call(_lib().kh_clip_factor, 1, sumsq.data_ptr(), top, out.data_ptr(), _p(left_out), _stream())
 
 
 def clip_grads(grads, max_norm, out, dst=None):
@@ -633,11 +643,17 @@ def clip_grads(grads, max_norm, out, dst=None):
 
 
 # ---------------------------------------------------------------------------------- AdamW
-def adamw(p, g, m, v, pb, *, lr, beta1, beta2, eps, wd, step, grad_scale=1.0, zero_grad=True, factor=None):
+def adamw(p, g, m, v, pb, *, lr, beta1, beta2, eps, wd, step, grad_scale=1.0, zero_grad=True, factor=None, left_out=None):
     """One fused pass: moments, decoupled decay on every element, fp32 master update, bf16
     compute copy (``pb``, may be None) and gradient clear.  ``step`` is 1-based.  ``factor`` (fp32 [1] on the
     device, ``grad_norm``'s): the gradient is multiplied by it too; where it is NaN the step is left out (weights and
-    moments stay, the gradient is cleared)."""
+    moments stay, the gradient is cleared).  ``left_out`` (int32 [1] on the device, ``grad_norm``'s): how many of the ``step``
+    steps were left out; the bias corrections are those of the others.  Without it every step counts, those left out too."""
+    if left_out is not None and factor is None:
+        raise ValueError("adamw: left_out goes with a factor")
+    _count_of("adamw", left_out, p)
+    if left_out is not None and not p.is_cuda:
+        step = max(step - int(left_out), 1)
     bc1 = 1.0 - beta1 ** step
     bc2 = 1.0 - beta2 ** step
     if factor is not None and (factor.dtype is not torch.float32 or factor.numel() != 1 or factor.get_device() != p.get_device()):
@@ -650,7 +666,7 @@ def adamw(p, g, m, v, pb, *, lr, beta1, beta2, eps, wd, step, grad_scale=1.0, ze
         return ref.adamw(p, g, m, v, pb, lr, beta1, beta2, eps, wd, bc1, bc2, grad_scale, zero_grad)
     if factor is not None:
         _call(_lib().kh_adamw_factor, 1, p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _p(pb), p.numel(), lr, beta1, beta2,
-              eps, wd, bc1, bc2, grad_scale, int(zero_grad), factor.data_ptr(), _stream())
+              eps, wd, bc1, bc2, grad_scale, int(zero_grad), factor.data_ptr(), _p(left_out), step, beta1, beta2, _stream())
         return
     _call(_lib().kh_adamw, 1, p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _p(pb), p.numel(), lr, beta1, beta2,
                          eps, wd, bc1, bc2, grad_scale, int(zero_grad), _stream())

@@ -1,7 +1,7 @@
 """ctypes prototypes of the CUDA kernel library (``libkharon_cuda.so``)."""
 import ctypes as C
 
-i32, i64, f32, u32 = C.c_int32, C.c_int64, C.c_float, C.c_uint32
+i32, i64, f32, f64, u32 = C.c_int32, C.c_int64, C.c_float, C.c_double, C.c_uint32
 vp, cp, long_ = C.c_void_p, C.c_char_p, C.c_long
 
 
@@ -50,10 +50,10 @@ _OPTIONAL = {
     "kh_grad_share": (i32,),
     "kh_grad_piece": (i32, long_),
     "kh_grad_work_bytes": (long_,),
-    "kh_grad_norm": (i32, vp, i32, long_, i32, f32, vp, vp, vp, vp),
-    "kh_clip_factor": (i32, vp, f32, vp, vp),
+    "kh_grad_norm": (i32, vp, i32, long_, i32, f32, vp, vp, vp, vp, vp),
+    "kh_clip_factor": (i32, vp, f32, vp, vp, vp),
     "kh_grad_scale": (i32, vp, vp, i32, long_, i32, vp, vp),
-    "kh_adamw_factor": (i32, vp, vp, vp, vp, vp, long_, f32, f32, f32, f32, f32, f32, f32, f32, i32, vp, vp),
+    "kh_adamw_factor": (i32, vp, vp, vp, vp, vp, long_, f32, f32, f32, f32, f32, f32, f32, f32, i32, vp, vp, i32, f64, f64, vp),
     "kh_wait_probe": (i32, vp, u32, u32, vp, vp),
     "kh_gemm_skinny": (i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp),
     "kh_gemm_skinny2": (i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp, i32, vp),

@@ -233,18 +233,20 @@ def preference_loss(logits, V, target, starts, ref_logp, beta, smoothing, weight
         _put_gradient(dlogits[a:b], V, on, torch.stack([slope, -slope], 1).view(-1)[seq], lg, lse, ts)
 
 
-def clip_factor(sumsq, out, max_norm):
+def clip_factor(sumsq, out, max_norm, left_out=None):
     norm = math.sqrt(float(sumsq)) if float(sumsq) >= 0 else math.nan
     factor = math.nan if not math.isfinite(norm) else 1.0 if norm <= max_norm else max_norm / norm
     out.view(-1).copy_(torch.tensor([norm, factor], dtype=torch.float64))         # (a norm beyond fp32's range shows as inf)
+    if left_out is not None and math.isnan(factor):
+        left_out += 1
 
 
-def grad_norm(tensors, out, max_norm, sumsq):
+def grad_norm(tensors, out, max_norm, sumsq, left_out=None):
     total = torch.tensor([sum(float(t.double().square().sum()) for t in tensors)], dtype=torch.float64)
     if sumsq is not None:
         sumsq.copy_(total)
     if out is not None:
-        clip_factor(total, out, max_norm)
+        clip_factor(total, out, max_norm, left_out)
 
 
 def scale(src, dst, out):

@@ -119,6 +119,8 @@ class GRPOTrainer:
         self.d_old, self.d_ref, self.d_kl, self.d_clip, self.d_loss, self.d_sum = vec(), vec(), vec(), vec(), vec(), vec(4)
         self.grad_list = ops.TensorList([self.policy.params.g]) if max_norm > 0 else None
         self.norm_out = vec(2)
+        if max_norm > 0:
+            self.policy.left_out = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.pairs = None
         self.stats = {}
 
@@ -149,7 +151,7 @@ class GRPOTrainer:
         self._sync_grads()
         factor = None
         if self.grad_list is not None:
-            ops.grad_norm(self.grad_list, self.norm_out, max_norm=self.max_norm)
+            ops.grad_norm(self.grad_list, self.norm_out, max_norm=self.max_norm, left_out=self.policy.left_out)
             factor = self.norm_out[1:]
         self.policy.adamw_step(lr, 0.9, 0.95, 1e-8, 0.0, factor=factor)
 
