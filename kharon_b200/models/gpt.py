@@ -470,9 +470,11 @@ class GPT:
         same pass over the logits also produces the loss (mean CE x loss_scale into ``loss_acc``),
         so a training step reads the logits once.  ``head_loss(logits, vocab, target)`` takes the place of the
         cross-entropy: it leaves the gradient of another loss in the logits (``ops.policy_loss``, ``ops.preference_loss``
-        with ``dlogits=logits``); for a head that is not split over its vocabulary."""
+        with ``dlogits=logits``), with weights of its own; for a head that is not split over its vocabulary."""
         if head_loss is not None and (self.sp is not None or self.vp_group is not None or not self.last):
             raise ValueError("backward: another loss needs a last stage whose head is whole")
+        if head_loss is not None and (coef is not None or loss_scale is not None or inv_mb != 1.0 or accumulate_loss):
+            raise ValueError("backward: coef, inv_mb, loss_scale and accumulate_loss are the cross-entropy's; another loss has its own weights and outputs")
         if self.sp is not None:
             return self._backward_sp(slot, dx_out, inv_mb, coef, loss_scale, accumulate_loss)
         s = self.slots[slot]
@@ -485,7 +487,7 @@ class GPT:
         if defer:       # the gradient w.r.t. the stage output lands in the top layer's stash
             dx = s.layers[cfg.n_layer - 1]["d_out"]
         if self.last:
-            want_loss = loss_scale is not None and not self.skip_loss and head_loss is None
+            want_loss = loss_scale is not None and not self.skip_loss
             if self.vp_group is None:
                 if head_loss is not None:
                     head_loss(s.logits, V, s.tgt)
