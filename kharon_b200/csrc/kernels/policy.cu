@@ -40,9 +40,6 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {      // a NaN
 __device__ __forceinline__ uint32_t cut_word(uint32_t w, int k) { return k <= 0 ? NEG2 : k == 1 ? (w & 0xffffu) | 0xff800000u : w; }
 // -inf in the columns k.. of an 8-column piece
 __device__ __forceinline__ uint4 cut_from(const uint4& v, int k) { return make_uint4(cut_word(v.x, k), cut_word(v.y, k - 2), cut_word(v.z, k - 4), cut_word(v.w, k - 6)); }
-__device__ __forceinline__ uint32_t zero_word(uint32_t w, int k) { return k <= 0 ? 0u : k == 1 ? w & 0xffffu : w; }
-// 0 in the columns k.. of it (of a gradient: what cut_from leaves there times a slope that is not finite is NaN)
-__device__ __forceinline__ uint4 zero_from(const uint4& v, int k) { return make_uint4(zero_word(v.x, k), zero_word(v.y, k - 2), zero_word(v.z, k - 4), zero_word(v.w, k - 6)); }
 __device__ __forceinline__ uint32_t put_word(uint32_t w, int k, uint32_t b) { return k == 0 ? (w & 0xffff0000u) | b : k == 1 ? (w & 0xffffu) | b << 16 : w; }
 // the bits b in column k of it
 __device__ __forceinline__ uint4 put_bits(const uint4& v, int k, uint32_t b) {
@@ -101,16 +98,16 @@ struct Sum {
 __device__ __forceinline__ uint32_t top8(const uint4& v) { return max2(max2(v.x, v.y), max2(v.z, v.w)); }
 // What a row's gradient is made of: k exp(x - m), k = -slope / sum.  The size of k is a further term of the exponent where that stays below 96 and so loses less than 2^-17 (of a
 // result that is rounded to 2^-8), with f = 0 or -0 for its sign; else f is k, or k 2^-BELOW, and never 0.  Results below 2^-126 are 0 in the first form, exponentials in the second.
+constexpr float LEAST = 0x1p-147f;             // k up to that is 0 times 2^-BELOW in fp32, and no bf16 number times an exponential
 struct Shape {
   float a, b, f;
 };
 __device__ __forceinline__ Shape shape_of(float m, float k) {
   const Scale s = scale_of(m);
-  const bool far = is_far(m);
-  const float b = s.b + log2f(fabsf(k)), f = far ? k : k * exp2f(-BELOW);
-  if (!far && fabsf(b) <= 96.f) return {s.a, b, copysignf(0.f, k)};
-  if (f == 0.f) return {s.a, -INFINITY, 0.f};              // k = 0, or of the smallest fp32 numbers, whose product is 0 in any bf16 column: the first form, with nothing in it
-  return {s.a, far ? s.b : s.b + BELOW, f};
+  if (fabsf(k) <= LEAST) return {s.a, -INFINITY, 0.f};
+  const float b = s.b + log2f(fabsf(k));
+  if (!is_far(m) && fabsf(b) <= 96.f) return {s.a, b, copysignf(0.f, k)};
+  return is_far(m) ? Shape{s.a, s.b, k} : Shape{s.a, s.b + BELOW, k * exp2f(-BELOW)};
 }
 template <bool FUSED>
 __device__ __forceinline__ uint4 grad8(const uint4& v, const Shape& g) {
@@ -163,6 +160,15 @@ struct Rows {                                // logits in, gradient out
   long ldg;
   int gcols, rows;
 };
+// A row whose slope is not finite: 0 in its columns from V on too, where the padding's exponentials of 0 times that are NaN.  By a warp, behind its stores of the row's last piece.
+// (Out of line: inside the kernels it cost pair_k up to 9 %.)
+__device__ __noinline__ void clear_columns(bf16* g, int from, int to) {
+  __syncwarp();
+  for (int c = from + (int)(threadIdx.x & 31); c < to; c += 32) g[c] = __float2bfloat16(0.f);
+}
+__device__ __forceinline__ void clear_behind(const Rows& q, bf16* g, const Shape& shape) {
+  if (!(fabsf(shape.f) < INFINITY)) clear_columns(g, q.V, q.gcols);
+}
 struct Policy {
   const float *adv, *old_lp, *ref_lp, *weight;
   int adv_rows;                              // rows of an advantage
@@ -328,10 +334,10 @@ __global__ void __launch_bounds__(256) policy_warp_k(Rows q, Policy a) {
         const int i = j * 32 + lane;
         if (i >= gv) continue;
         uint4 o = grad8(v[j], shape);
-        if (8 * i + 8 > q.V) o = zero_from(o, q.V - 8 * i);
         if (i == t >> 3) o = put_one(o, t & 7, at_t);
         store8(g, i, q.gcols, o);
       }
+      clear_behind(q, g, shape);
     }
     for (int i = (t >= 0 ? NC * 32 : 0) + lane; i < gv; i += 32) store8(g, i, q.gcols, make_uint4(0, 0, 0, 0));
   }
@@ -427,9 +433,11 @@ __global__ void __launch_bounds__(256, 4) policy_twice_k(Rows q, Policy a) {
   const Shape shape = shape_of(m, -inv);
   grad_pieces(gp, v, min(nv - (cut >= 0), q.gcols / 8), shape);
   if (cut >= 0 && lane == 0) {
-    const uint4 y = v[cut];
-    store8(g, cut, q.gcols, zero_from(grad8(y, shape), q.V - 8 * cut));
+    uint4 y = v[cut];
+    y = cut_from(y, q.V - 8 * cut);
+    store8(g, cut, q.gcols, grad8(y, shape));
   }
+  clear_behind(q, g, shape);
   __syncwarp();
   if (lane == 0) g[t] = __float2bfloat16(inv * rest);      // (behind the store of the piece)
   for (int i = nv + lane; i < gv; i += 32) store8(g, i, q.gcols, make_uint4(0, 0, 0, 0));
@@ -626,7 +634,8 @@ __global__ void __launch_bounds__(64 * NP + 32, NP >= 8 ? 1 : 12 / NP) policy_ro
     }
   } else {
     // ---- gradients
-    const int gv = (q.gcols + 7) / 8, whole = min(n, q.gcols / 8 - v0), last = 8 * (v0 + n) > q.V ? n - 1 : n;     // (the piece that sticks out of the vocabulary apart)
+    const int gv = (q.gcols + 7) / 8, whole = min(n, q.gcols / 8 - v0);
+    const bool sticks = 8 * (v0 + n) > q.V;                // the part ends behind the vocabulary
     int k = 0, phase = 0;
     for (int base = 0; base < total; base += 32) {
       Block b;
@@ -649,13 +658,14 @@ __global__ void __launch_bounds__(64 * NP + 32, NP >= 8 ? 1 : 12 / NP) policy_ro
         const int tv = (o.t >> 3) - v0;
         for (int c = 0; c < nc; c++) {
           wait(full(k, c), phase);
-          grad_pieces(gp + c * CHUNK, here + c * CHUNK, min(CHUNK, last - c * CHUNK), o.shape);
-          if (last < n && c == nc - 1 && lane == 0) store8(g, v0 + last, q.gcols, zero_from(grad8(here[last], o.shape), q.V - 8 * (v0 + last)));
+          grad_pieces(gp + c * CHUNK, here + c * CHUNK, min(CHUNK, whole - c * CHUNK), o.shape);
+          if (whole < n && c == nc - 1 && lane == 0) store8(g, v0 + whole, q.gcols, grad8(here[whole], o.shape));
           fence_proxy_async_smem();
           __syncwarp();
           if (tv >> 8 == c && tv < n && lane == 0) g[o.t] = __float2bfloat16(o.at_target);                      // (behind the store of the piece)
           if (rn >= 0) fetch(xn, k, c);
         }
+        if (sticks) clear_behind(q, g, o.shape);
         if (++k == NS) { k = 0; phase ^= 1; }
       }
     }
@@ -982,10 +992,10 @@ __global__ void __launch_bounds__(512) pair_k(Rows q, Pairs b, int C, int* err) 
           const int at = j * 32 + lane;
           if (at >= gv) continue;
           uint4 o = grad8(v[j], shape);
-          if (8 * at + 8 > q.V) o = zero_from(o, q.V - 8 * at);
           if (at == t >> 3) o = put_one(o, t & 7, at_t);
           store8(g, at, q.gcols, o);
         }
+        clear_behind(q, g, shape);
         for (int at = NC * 32 + lane; at < gv; at += 32) store8(g, at, q.gcols, make_uint4(0, 0, 0, 0));
       }
       __syncwarp();
@@ -1291,9 +1301,11 @@ __global__ void __launch_bounds__(32 * (WORKERS + 2), 1) stream_k(Rows q, Policy
           const Shape shape = {x.kind == FAR ? 1.f : LOG2E, x.b, x.f};
           grad_pieces(gp, v, min(whole, cut >= 0 ? n - 1 : n), shape);
           if (cut >= 0 && lane == 0) {
-            const uint4 y = v[n - 1];
-            store8(g, m0 + n - 1, q.gcols, zero_from(grad8(y, shape), q.V - 8 * (m0 + n - 1)));
+            uint4 y = v[n - 1];
+            y = cut_from(y, q.V - 8 * (m0 + n - 1));
+            store8(g, m0 + n - 1, q.gcols, grad8(y, shape));
           }
+          if (cut >= 0) clear_behind(q, g, shape);
           __syncwarp();
           if (tv >= 0 && tv < n && lane == 0) g[x.t] = __float2bfloat16(x.at_t);          // (behind the store of the piece)
         }
