@@ -3,8 +3,8 @@
 // A list of tensors is a table of {address, elements, pieces before it, type}; a CTA takes an equal share of all pieces in one run, sums squares in 64 bits (whose range
 // holds every square of an fp32 number, and whose additions lose nothing that fp32 could show), and the last CTA adds the CTAs' sums in order.  Bound by memory: each
 // element is read once.  The tensors are multiplied in the same shares, from their ends back to their beginnings, so that what the norm read last comes from L2.
-// 5.25 GB of fp32 in 292 tensors: 740 us, 7.1 TB/s, as reads alone go; 55 MB in 76 tensors of both types with the multiplication: 36 us, half of it either kernel's start, end and trips; 204 MB: 109 us,
-// 0.85 of the copy rate for three passes.
+// 5.25 GB of fp32 in 292 tensors: 740 us, 7.1 TB/s, as reads alone go; 55 MB in 76 tensors of both types multiplied into other buffers: 36 us, half of it either kernel's start, end and trips; 204 MB: 110 us,
+// 0.85 of the copy rate for three passes.  In place, behind a flushed L2: 40 and 113 us, into other buffers 42 and 116.
 #include <algorithm>
 
 #include "common.cuh"

@@ -257,8 +257,8 @@ __device__ __forceinline__ uint64_t l2_pass() {
 
 // Up to 1024 columns: a warp takes K rows at a time (NC pieces of 8 x 32 columns each), and a lane each the terms of a row, which cost a warp more instructions than the
 // exponentials of 1024 columns.  One row stays in registers for its gradient; of several the pieces are read again, from L1 or L2 (kept in registers they cost the warps that hide
-// the terms' latency).  Bound by the issue of instructions (63 % of the slots) and by latency, not by memory: 60000 x 256, all rows counting, 28.7 us with K = 4, 31.7 with 1;
-// 20000 x 1003 23.9 us with K = 1, 29.7 with 4.
+// the terms' latency).  Bound by the issue of instructions (72 % of the slots; every exponential is taken twice, for the sum and for the gradient) and by latency, not by memory:
+// 60000 x 256, three quarters of the rows counting, 28.7 us with K = 4 (all counting: 31), 31.7 with 1; 20000 x 1003 24.5 us with K = 1, 29.7 with 4.
 template <int NC, int K>
 __global__ void __launch_bounds__(256) policy_warp_k(Rows q, Policy a) {
   pdl_wait();
@@ -844,8 +844,8 @@ __device__ __noinline__ void end_pair(const Pairs& b, int p, volatile int* abort
 
 // Small vocabularies and pairs: a CTA per pair, or a cluster of C where the pairs are fewer than the SMs, a warp per row (NC pieces of 8 x 32 columns in registers), read once for
 // the sums and once more, from L1 or L2, for the gradients.  32 rows of a warp at a time, so that their terms are taken side by side.  64 pairs of 36 rows x 256: 6.7 us, a chain of
-// dependent trips (starts, targets, rows, the pair's sums, its slope); 32 pairs, 6400 x 1003: 17 us, with a CTA a pair 52; 200 pairs, 100000 x 256: 58 us, as a stream (below) 176, but
-// 50 pairs, 25000 x 2000: 78 us, 73 as a stream.
+// dependent trips (starts, targets, rows, the pair's sums, its slope); 32 pairs, 6400 x 1003: 15 us, with a CTA a pair 52; 200 pairs, 100000 x 256: 56 us, as a stream (below) 176, but
+// 50 pairs, 25000 x 2000: 78 us, 73 as a stream.  The rule goes by the average: one pair of 50000 rows among 500 of 40 has its CTA alone (3.5 ms, where the two lists by themselves take 17 and 274 us).
 constexpr long PAIR_ROWS[2] = {2048, 128};   // rows of a pair, on average, for each of its CTAs, up to which that is so: with 1024 columns at most, with more
 constexpr int KEPT = 1024;                   // rows of a CTA whose numbers stay in shared memory; others' go through the workspace
 template <int NC>
